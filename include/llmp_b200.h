@@ -48,6 +48,10 @@ extern "C" {
 #define LLMP_B200_TYPE_Q5_K 13
 #define LLMP_B200_TYPE_Q6_K 14
 #define LLMP_B200_TYPE_IQ4_NL 20
+/* Element types of the operators that take F32, F16 or BF16 (GGML's numbers too). */
+#define LLMP_B200_TYPE_F32 0
+#define LLMP_B200_TYPE_F16 1
+#define LLMP_B200_TYPE_BF16 30
 
 /* VecQGlu (src/kernels/ggml/llmp_ops.h:1072). */
 #define LLMP_B200_GLU_NONE 0
@@ -643,6 +647,140 @@ int llmp_b200_mxfp8_gemm_variant(const llmp_b200_mxfp8_gemm_desc* gemm, int sms,
                                  void* stream);
 /* How many CTA pairs of the pair kernel the current device holds at once (0: none). */
 int llmp_b200_mxfp8_gemm_resident_pairs(void);
+
+/* ------------------------------------------------------------------ 4-bit weights, group scales */
+/* No counterpart among the reference's templates (its affine decoders, src/kernels/decode, are the
+ * nearest).  A matrix of n rows of k values, value (r, i) = scale[r][i / group] * (code[r][i] -
+ * zero[r][i / group]): codes of 0..15, two a byte (value 2 i in byte i's low nibble); F16 or BF16
+ * scales, one a group of 32, 64 or 128 values; zero points of 0..15, two a byte (group 2 i in
+ * the low nibble), or none: 8.  Strides are those of the arrays as they lie: bytes between rows
+ * and experts of codes and zero points, elements between those of scales.  The codes and zero
+ * points may begin at any byte. */
+typedef struct llmp_b200_w4_source {
+  const uint8_t* codes;
+  int64_t code_row, code_expert;
+  const void* scales;
+  int64_t scale_row, scale_expert;
+  const uint8_t* zeros; /* or NULL */
+  int64_t zero_row, zero_expert;
+} llmp_b200_w4_source;
+/* The matrix as the products read it: the slab that llmp_b200_w4_relayout made of the source. */
+typedef struct llmp_b200_w4_matrix {
+  const void* slab;  /* llmp_b200_w4_slab_bytes(), 256-byte aligned */
+  int n, k;          /* rows (glu: gate rows, then as many up rows) and values a row, a multiple of the group */
+  int group;         /* 32, 64 or 128 */
+  int experts;       /* matrices, one after the other in the slab; 1 for a plain product */
+  int scale_type;    /* LLMP_B200_TYPE_F16 / _BF16 */
+  int glu;           /* 1: gate and up rows interleaved, for the products with a GLU */
+} llmp_b200_w4_matrix;
+size_t llmp_b200_w4_slab_bytes(int n, int k, int group, int experts, int glu);
+/* Source to slab, once at load time: lossless, the values only change places (1.06 to 1.25 bytes a
+ * code byte).  Queues one ordinary launch; a product after it on the stream sees the whole slab. */
+int llmp_b200_w4_relayout(const llmp_b200_w4_source* source, const llmp_b200_w4_matrix* matrix, void* stream);
+/* y[t] = W x[t] for 1 to 16 rows of activations (0: nothing is queued); with a GLU slab glu(gate x[t], up x[t]).
+ * Codes and activations multiply exactly, sums are F32 (an F16 or F32 activation enters as the
+ * bf16 values whose sum it is), the result is rounded once, to y's type.  y apart from x. */
+typedef struct llmp_b200_w4_product {
+  llmp_b200_w4_matrix w;
+  const void* x;
+  int64_t x_stride;  /* elements between rows, at least k */
+  void* y;
+  int64_t y_stride;
+  int rows;
+  int x_type, y_type; /* LLMP_B200_TYPE_F32 / _F16 / _BF16 */
+  int glu;            /* LLMP_B200_GLU_*; _NONE exactly when the slab is a plain one */
+  float limit;
+} llmp_b200_w4_product;
+int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream);
+
+/* A whole mixture-of-experts layer for 1 to 16 tokens (0: nothing is queued) in two kernels.  Where
+ * llmp_b200_moe_decode takes the choice of experts, this makes it:
+ *   logits[t] = router x[t];  p = softmax(logits) over all experts, or sigmoid of each
+ *   the `used` experts of the greatest logit (with a bias: of the greatest p + bias), best first,
+ *     ties to the lowest index, a NaN below everything
+ *   weights = p of those (renormalize: over their sum) * scale
+ *   y[t] = sum_j weights[j] * down_e glu(gate_e x[t], up_e x[t]),  e = ids[t][j], added in slot order
+ * Logits are exact products added in 64 bits block by block; expert sums are as llmp_b200_w4_vector's,
+ * the GLU rows stay 16 bits wide (F32 activations: 24).  A token's results do not depend on the
+ * others of the call, up to the passes that x takes through shared memory.  Each call that may overlap another
+ * brings its own scratch; nothing in it outlives the call. */
+#define LLMP_B200_SCORE_SOFTMAX 0
+#define LLMP_B200_SCORE_SIGMOID 1
+typedef struct llmp_b200_moe_layer_desc {
+  const void* x;         /* [tokens, hidden], rows x_stride elements apart */
+  int64_t x_stride;
+  const void* router;    /* [experts, hidden], rows router_stride elements apart */
+  int64_t router_stride;
+  const float* bias;     /* F32 [experts] or NULL: added to p for the choice alone */
+  llmp_b200_w4_matrix gate_up; /* glu 1: n = 2 * inter, k = hidden (up to 16384), up to 512 experts */
+  llmp_b200_w4_matrix down;    /* n = hidden, k = inter */
+  void* y;               /* [tokens, hidden], apart from x */
+  int64_t y_stride;
+  int32_t* ids;          /* out: I32 [tokens, used], packed */
+  float* weights;        /* out: F32 [tokens, used], packed */
+  void* scratch;         /* llmp_b200_moe_layer_scratch() bytes, 256-byte aligned, of any content */
+  int x_type, router_type, y_type;
+  int tokens, used;      /* used: 1 to 16 */
+  int score, renormalize;
+  float scale;
+  int glu;               /* LLMP_B200_GLU_SWIGLU / _SWIGLU_CLAMP / _GEGLU */
+  float limit;
+} llmp_b200_moe_layer_desc;
+size_t llmp_b200_moe_layer_scratch(int used, int tokens, int inter);
+int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream);
+
+/* ------------------------------------------------------------------ between the products */
+/* The RMS norms after a block and before the next with what lies between, one kernel:
+ *   u = block * rsqrt(mean(block^2) + eps) * (offset + post)    post NULL: u = block
+ *   r = residual + scale * gate * u                              NULL: without it
+ *   h = r * rsqrt(mean(r^2) + eps) * (offset + pre)
+ * in F32, r and h rounded when stored (h is of the unrounded r).  out_residual may be residual, and
+ * either output may be block (whole rows, the same stride). */
+typedef struct llmp_b200_block_norm_desc {
+  const void* block;     /* [rows, width], rows block_stride elements apart (0: one row for all) */
+  int64_t block_stride;
+  const void* residual;
+  int64_t residual_stride;
+  const void* gate;      /* a row of factors, gate_stride elements to the next row's (0: one for all) */
+  int64_t gate_stride;
+  const void* post;      /* [width] */
+  const void* pre;       /* [width], or NULL: r is all that is wanted */
+  void* out_residual;    /* r, or NULL */
+  int64_t out_residual_stride;
+  void* out;             /* h, or NULL */
+  int64_t out_stride;
+  void* q8;              /* F32 rows: h's Q8_1 rows as llmp_b200_q8_1_quantize makes them, packed, or NULL */
+  int64_t rows;          /* 0: nothing is queued */
+  int width;             /* up to 32768 */
+  int type, weight_type; /* of the rows and the gate; of post and pre: the same or F32 */
+  float scale, offset, eps;
+} llmp_b200_block_norm_desc;
+int llmp_b200_block_norm(const llmp_b200_block_norm_desc* desc, void* stream);
+
+/* What a server answers with beside the tokens, from a head's logits; x = logit / temperature:
+ *   logprobs[row][j] = x[token] - log sum e^x of tokens[row][j], ranks[row][j] = 1 + the logits above its own
+ *   entropy[row] = -sum p log p
+ *   top_ids / top_logprobs[row]: the `top` largest logits, best first, ties to the lowest index
+ * A masked logit is -inf: its log probability is -inf, and so are all of a row that has nothing else (entropy 0).
+ * A NaN or +inf makes a row's log probabilities and entropy NaN; in the order a NaN is below -inf.  A
+ * token outside the vocabulary has NaN and rank 0. */
+typedef struct llmp_b200_logprobs_desc {
+  const void* logits;    /* [rows, vocab], rows stride elements apart */
+  int64_t stride;
+  const int32_t* tokens; /* [rows, given], packed */
+  float* logprobs;       /* [rows, given] */
+  int32_t* ranks;        /* [rows, given] */
+  float* entropy;        /* [rows] */
+  int32_t* top_ids;      /* [rows, top] */
+  float* top_logprobs;   /* [rows, top] */
+  int64_t rows;          /* 0: nothing is queued */
+  int type;              /* LLMP_B200_TYPE_F32 / _F16 / _BF16 */
+  int vocab;             /* up to 2^24 */
+  int given;             /* 0 to 16 */
+  int top;               /* 0 to 32 */
+  float temperature;     /* 1e-6 to 1e6 */
+} llmp_b200_logprobs_desc;
+int llmp_b200_logprobs(const llmp_b200_logprobs_desc* desc, void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,9 @@ LIB_PATH = os.path.join(_HERE, "_lib", "libllmp_b200.so")
 
 OK, REJECTED, NO_DEVICE = 0, 1, 2
 TYPE_Q8_0, TYPE_Q8_1, TYPE_Q4_K = 8, 9, 12
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
 GLU_NONE, GLU_SWIGLU, GLU_SWIGLU_CLAMP, GLU_GEGLU = 0, 1, 2, 3
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 
 class NativeLibraryMissing(ImportError):
@@ -115,6 +117,53 @@ class GroupedGemmDesc(C.Structure):
                 ("weights_slab", C.c_void_p)]
 
 
+class W4Source(C.Structure):
+    """llmp_b200_w4_source (include/llmp_b200.h)."""
+    _fields_ = [("codes", C.c_void_p), ("code_row", C.c_int64), ("code_expert", C.c_int64),
+                ("scales", C.c_void_p), ("scale_row", C.c_int64), ("scale_expert", C.c_int64),
+                ("zeros", C.c_void_p), ("zero_row", C.c_int64), ("zero_expert", C.c_int64)]
+
+
+class W4MatrixDesc(C.Structure):
+    """llmp_b200_w4_matrix (include/llmp_b200.h)."""
+    _fields_ = [("slab", C.c_void_p)] + [(n, C.c_int) for n in ("n", "k", "group", "experts", "scale_type", "glu")]
+
+
+class W4Product(C.Structure):
+    """llmp_b200_w4_product (include/llmp_b200.h)."""
+    _fields_ = [("w", W4MatrixDesc), ("x", C.c_void_p), ("x_stride", C.c_int64), ("y", C.c_void_p),
+                ("y_stride", C.c_int64), ("rows", C.c_int), ("x_type", C.c_int), ("y_type", C.c_int),
+                ("glu", C.c_int), ("limit", C.c_float)]
+
+
+class MoeLayerDesc(C.Structure):
+    """llmp_b200_moe_layer_desc (include/llmp_b200.h)."""
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("router", C.c_void_p), ("router_stride", C.c_int64),
+                ("bias", C.c_void_p), ("gate_up", W4MatrixDesc), ("down", W4MatrixDesc), ("y", C.c_void_p),
+                ("y_stride", C.c_int64), ("ids", C.c_void_p), ("weights", C.c_void_p), ("scratch", C.c_void_p)] + [
+                    (n, C.c_int) for n in ("x_type", "router_type", "y_type", "tokens", "used", "score",
+                                           "renormalize")] + [
+                    ("scale", C.c_float), ("glu", C.c_int), ("limit", C.c_float)]
+
+
+class BlockNormDesc(C.Structure):
+    """llmp_b200_block_norm_desc (include/llmp_b200.h)."""
+    _fields_ = [("block", C.c_void_p), ("block_stride", C.c_int64), ("residual", C.c_void_p),
+                ("residual_stride", C.c_int64), ("gate", C.c_void_p), ("gate_stride", C.c_int64),
+                ("post", C.c_void_p), ("pre", C.c_void_p), ("out_residual", C.c_void_p),
+                ("out_residual_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("q8", C.c_void_p), ("rows", C.c_int64), ("width", C.c_int), ("type", C.c_int),
+                ("weight_type", C.c_int), ("scale", C.c_float), ("offset", C.c_float), ("eps", C.c_float)]
+
+
+class LogprobsDesc(C.Structure):
+    """llmp_b200_logprobs_desc (include/llmp_b200.h)."""
+    _fields_ = [("logits", C.c_void_p), ("stride", C.c_int64), ("tokens", C.c_void_p), ("logprobs", C.c_void_p),
+                ("ranks", C.c_void_p), ("entropy", C.c_void_p), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("rows", C.c_int64), ("type", C.c_int), ("vocab", C.c_int),
+                ("given", C.c_int), ("top", C.c_int), ("temperature", C.c_float)]
+
+
 # name -> (restype, argtypes): every symbol include/llmp_b200.h declares.
 SIGNATURES = {
     "llmp_b200_available": (C.c_int, []),
@@ -206,6 +255,13 @@ SIGNATURES = {
                                         C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p]),
     "llmp_b200_decode_matrix": (C.c_int, [C.POINTER(DecodeProduct), C.c_void_p]),
     "llmp_b200_decode_grouped": (C.c_int, [C.POINTER(DecodeGroupedProduct), C.c_void_p]),
+    "llmp_b200_w4_slab_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "llmp_b200_w4_relayout": (C.c_int, [C.POINTER(W4Source), C.POINTER(W4MatrixDesc), C.c_void_p]),
+    "llmp_b200_w4_vector": (C.c_int, [C.POINTER(W4Product), C.c_void_p]),
+    "llmp_b200_moe_layer_scratch": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "llmp_b200_moe_layer": (C.c_int, [C.POINTER(MoeLayerDesc), C.c_void_p]),
+    "llmp_b200_block_norm": (C.c_int, [C.POINTER(BlockNormDesc), C.c_void_p]),
+    "llmp_b200_logprobs": (C.c_int, [C.POINTER(LogprobsDesc), C.c_void_p]),
     "llmp_b200_mmvq_scratch": (C.c_size_t, [C.c_int, C.c_int]),
     "llmp_b200_mmvq": (C.c_int, [C.POINTER(MmvqDesc), C.c_void_p]),
     "llmp_b200_mmvq_prepared": (C.c_int, [C.POINTER(MmvqDesc), C.c_void_p]),

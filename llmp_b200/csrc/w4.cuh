@@ -1,0 +1,264 @@
+// 4-bit weights with group scales: the slab that the products read, and the product of a tile.
+//
+// A weight is scale * (code - zero), code and zero in 0..15, one scale and zero a group of 32, 64
+// or 128 values of a row.  The slab (llmp_b200_w4_relayout, once at load time) holds, per expert,
+// tiles of 16 weight rows x steps of 128 values, steps of a tile back to back, each
+//
+//   [2][32 lanes][16 bytes]  codes: lane (g, t) = (lane / 4, lane % 4) holds row g's and row g + 8's
+//                            values 32 i + 8 t .. + 7 of the step in word i = 0..3, the even values'
+//                            nibbles in the low half and the odd ones' in the high half
+//   [16 rows][128 / group]   words: the scale's 16 bits, and above them 128 + zero as a bf16
+//
+// so a warp reads a step with two 16-byte loads a lane and one load of its rows' words, and word
+// i >> 4 j & 0x000f000f is a pair of neighbouring codes.  Or'ed with 0x4300 (128 in bf16, whose
+// last four mantissa bits then are the code) and less 128 + zero they are two exact bf16 values:
+// the A fragment of mma.sync.m16n8k16, whose k order is free as long as B's is the same.  With a
+// GLU a tile's rows 0..7 are gate rows and 8..15 the same rows of up, so a lane's sums hold both.
+//
+// A group's sum comes before its scale: up to 15 * 128 times the activations, which enter 2^-11
+// smaller where their type reaches F32's range (exact down to 2^-98) and whose results leave 2^11 larger, so
+// that nothing overflows that the scaled product would not.
+//
+// The tokens are the MMA's 8 columns.  A product is exact (code - zero has 5 bits, a bf16 column
+// 8), sums are F32, and the scale multiplies a group's F32 sum, so nothing is rounded to fewer
+// bits.  F16 and F32 activations are split into 2 and 3 bf16 columns whose sum they are, exactly
+// (11 and 24 significant bits in pieces of 8); a token takes kCols = 1, 2 or 4 columns (one of
+// the 4 is zero).
+#ifndef LLMP_B200_CSRC_W4_CUH_
+#define LLMP_B200_CSRC_W4_CUH_
+
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace llmp_b200 {
+namespace w4 {
+
+constexpr int kStep = 128;       // values of a row in a step
+constexpr int kTileRows = 16;
+
+__host__ __device__ constexpr int BlockBytes(int group) { return 1024 + (64 * (kStep / group)); }
+__host__ __device__ constexpr int Steps(int k) { return (k + kStep - 1) / kStep; }
+// Tiles of a matrix of n rows (with a GLU: n / 2 gate rows, then n / 2 up rows).
+__host__ __device__ constexpr int Tiles(int n, int glu) {
+  return glu ? ((n / 2) + 7) / 8 : (n + 15) / 16;
+}
+
+// Element types of activations and outputs (GGML's numbers).
+constexpr int kF32 = LLMP_B200_TYPE_F32, kF16 = LLMP_B200_TYPE_F16, kBF16 = LLMP_B200_TYPE_BF16;
+inline bool FloatType(int t) { return t == kF32 || t == kF16 || t == kBF16; }
+__host__ __device__ constexpr int TypeBytes(int t) { return t == kF32 ? 4 : 2; }
+// bf16 pieces that a value of the type is the sum of.
+__host__ __device__ constexpr int Pieces(int t) { return t == kF32 ? 3 : t == kF16 ? 2 : 1; }
+
+// Activations enter this much smaller, results leave this much larger.
+__host__ __device__ constexpr float Down(int t) { return t == kF16 ? 1.0f : 0x1p-11f; }
+__host__ __device__ constexpr float Up(int t) { return t == kF16 ? 1.0f : 0x1p+11f; }
+
+// Shape and alignment of a matrix whose slab a product reads: 0 or a refusal.
+int CheckMatrix(const llmp_b200_w4_matrix& m, const char* what);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float LoadValue(const void* p, std::int64_t i, int type) {
+  if (type == kF32) return static_cast<const float*>(p)[i];
+  const std::uint32_t bits = static_cast<const unsigned short*>(p)[i];
+  return type == kBF16 ? __uint_as_float(bits << 16) : HalfBitsToFloat(bits);
+}
+__device__ __forceinline__ void StoreValue(void* p, std::int64_t i, int type, float v) {
+  if (type == kF32) {
+    static_cast<float*>(p)[i] = v;
+  } else if (type == kBF16) {
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  } else {
+    static_cast<__half*>(p)[i] = __float2half_rn(v);
+  }
+}
+
+// The pieces of x, in bf16 bits: truncations, so each remainder is exact and none overflows.
+template <int kPieces>
+__device__ __forceinline__ void Split(float x, std::uint32_t (&bits)[kPieces]) {
+  float rest = x;
+#pragma unroll
+  for (int s = 0; s < kPieces; ++s) {
+    const std::uint32_t b = __float_as_uint(rest);
+    bits[s] = b >> 16;
+    rest -= __uint_as_float(b & 0xffff0000u);
+  }
+  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) {  // inf - inf: the first piece says it all
+    if ((__float_as_uint(x) & 0x007fffffu) != 0) bits[0] |= 0x0040u;  // a NaN stays one
+#pragma unroll
+    for (int s = 1; s < kPieces; ++s) bits[s] = 0;
+  }
+}
+
+// Eight consecutive values (zero from `valid` on) times Down as pieces, a 16-byte quad a piece.
+template <int kType, bool kDown = true>
+__device__ __forceinline__ void LoadSplit8(const void* row, std::int64_t at, int valid, bool vec,
+                                           uint4 (&quads)[Pieces(kType)]) {
+  constexpr int kPieces = Pieces(kType);
+  if constexpr (kType == kBF16) {
+    if (vec && valid >= 8) {
+      uint4 q = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
+      if constexpr (kDown) {
+        auto* pairs = reinterpret_cast<__nv_bfloat162*>(&q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pairs[i] = __hmul2(pairs[i], __float2bfloat162_rn(Down(kType)));
+      }
+      quads[0] = q;
+      return;
+    }
+  }
+  float v[8];
+  if (vec && valid >= 8) {
+    if constexpr (kType == kF32) {
+      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
+      const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
+      const std::uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = HalfBitsToFloat(w[i] & 0xffffu);
+        v[(2 * i) + 1] = HalfBitsToFloat(w[i] >> 16);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? LoadValue(row, at + i, kType) : 0.0f;
+  }
+  if constexpr (kDown && kType != kF16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= Down(kType);
+  }
+  std::uint32_t packed[kPieces][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    std::uint32_t lo[kPieces], hi[kPieces];
+    Split<kPieces>(v[2 * i], lo);
+    Split<kPieces>(v[(2 * i) + 1], hi);
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) packed[s][i] = lo[s] | (hi[s] << 16);
+  }
+#pragma unroll
+  for (int s = 0; s < kPieces; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
+}
+
+// Columns a token takes, tokens an MMA's 8 columns hold.
+__host__ __device__ constexpr int Cols(int pieces) { return pieces == 3 ? 4 : pieces; }
+__host__ __device__ constexpr int TokensATile(int pieces) { return 8 / Cols(pieces); }
+
+__device__ __forceinline__ void Mma(float (&c)[4], std::uint32_t a0, std::uint32_t a1, std::uint32_t a2,
+                                    std::uint32_t a3, std::uint32_t b0, std::uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two codes at bits 0 and 16 of w >> 4 j as bf16 values less (128 + zero) twice.
+__device__ __forceinline__ std::uint32_t Pair(std::uint32_t w, int j, std::uint32_t zero2) {
+  const std::uint32_t biased = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased),
+                                   *reinterpret_cast<const __nv_bfloat162*>(&zero2));
+  return *reinterpret_cast<const std::uint32_t*>(&v);
+}
+__device__ __forceinline__ std::uint32_t Zero2(std::uint32_t word) { return __byte_perm(word, 0, 0x3232); }
+__device__ __forceinline__ float Scale(std::uint32_t word, bool bf16) {
+  return bf16 ? __uint_as_float(word << 16) : HalfBitsToFloat(word & 0xffffu);
+}
+
+// A step of a tile as a lane holds it.
+template <int kGroups>
+struct StepWeights {
+  uint4 a, b;                                // rows g and g + 8
+  std::uint32_t word_a[kGroups], word_b[kGroups];
+  __device__ __forceinline__ void Load(const std::uint8_t* block, int lane) {
+    a = LoadStream16(block + (lane * 16));
+    b = LoadStream16(block + 512 + (lane * 16));
+    const std::uint8_t* words = block + 1024 + ((lane >> 2) * (kGroups * 4));
+    if constexpr (kGroups == 1) {
+      word_a[0] = LoadStream4(words);
+      word_b[0] = LoadStream4(words + 32);
+    } else if constexpr (kGroups == 2) {
+      const uint2 wa = LoadStream8(words), wb = LoadStream8(words + 64);
+      word_a[0] = wa.x, word_a[1] = wa.y, word_b[0] = wb.x, word_b[1] = wb.y;
+    } else {
+      const uint4 wa = LoadStream16(words), wb = LoadStream16(words + 128);
+      word_a[0] = wa.x, word_a[1] = wa.y, word_a[2] = wa.z, word_a[3] = wa.w;
+      word_b[0] = wb.x, word_b[1] = wb.y, word_b[2] = wb.z, word_b[3] = wb.w;
+    }
+  }
+};
+
+// total += the step's products: column quads come from column(nt, i), the 16 bytes that hold
+// values 32 i + 8 t .. + 7 of the step for column lane / 4 of column tile nt.
+template <int kGroups, int kTiles, typename Column>
+__device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool bf16_scales, int tiles,
+                                             float (&total)[kTiles][4], Column column) {
+  const std::uint32_t wa[4] = {w.a.x, w.a.y, w.a.z, w.a.w}, wb[4] = {w.b.x, w.b.y, w.b.z, w.b.w};
+  constexpr int kBlocks = 4 / kGroups;  // 32-value blocks a group
+#pragma unroll
+  for (int group = 0; group < kGroups; ++group) {
+    const std::uint32_t za = Zero2(w.word_a[group]), zb = Zero2(w.word_b[group]);
+    float sum[kTiles][4];
+#pragma unroll
+    for (int nt = 0; nt < kTiles; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const int i = (group * kBlocks) + b;
+      std::uint32_t pa[4], pb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pa[j] = Pair(wa[i], j, za);
+        pb[j] = Pair(wb[i], j, zb);
+      }
+#pragma unroll
+      for (int nt = 0; nt < kTiles; ++nt) {
+        if (nt == 0 || nt < tiles) {
+          const uint4 x = column(nt, i);
+          Mma(sum[nt], pa[0], pb[0], pa[1], pb[1], x.x, x.y);
+          Mma(sum[nt], pa[2], pb[2], pa[3], pb[3], x.z, x.w);
+        }
+      }
+    }
+    const float sa = Scale(w.word_a[group], bf16_scales), sb = Scale(w.word_b[group], bf16_scales);
+#pragma unroll
+    for (int nt = 0; nt < kTiles; ++nt) {
+      total[nt][0] = fmaf(sa, sum[nt][0], total[nt][0]);
+      total[nt][1] = fmaf(sa, sum[nt][1], total[nt][1]);
+      total[nt][2] = fmaf(sb, sum[nt][2], total[nt][2]);
+      total[nt][3] = fmaf(sb, sum[nt][3], total[nt][3]);
+    }
+  }
+}
+
+// A lane's sums of one column tile with a token's columns added up: values[r][j] is row g + 8 r,
+// token TokenOf(j); with 2 or 3 pieces only j = 0 counts.
+template <int kPieces>
+__device__ __forceinline__ void FoldColumns(const float (&total)[4], float (&values)[2][2]) {
+  if constexpr (kPieces == 1) {
+    values[0][0] = total[0], values[0][1] = total[1], values[1][0] = total[2], values[1][1] = total[3];
+  } else {
+    values[0][0] = total[0] + total[1];
+    values[1][0] = total[2] + total[3];
+    values[0][1] = values[1][1] = 0.0f;
+    if constexpr (kPieces == 3) {  // columns 0, 1 in an even lane, 2 (and a zero) in the next
+#pragma unroll
+      for (int r = 0; r < 2; ++r) values[r][0] += __shfl_xor_sync(0xffffffffu, values[r][0], 1);
+    }
+  }
+}
+// The token (within a column tile) of values[.][j] in lane t = lane % 4; every value is valid in
+// some lanes more than once with 3 pieces (t and t ^ 1 hold the same).
+template <int kPieces>
+__device__ __forceinline__ int TokenOf(int t, int j) {
+  return kPieces == 1 ? (2 * t) + j : kPieces == 2 ? t : t >> 1;
+}
+#endif  // __CUDACC__
+
+}  // namespace w4
+}  // namespace llmp_b200
+
+#endif  // LLMP_B200_CSRC_W4_CUH_

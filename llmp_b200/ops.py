@@ -8,12 +8,13 @@ B200 the calls raise.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
 from . import _native as N
-from ._native import (GLU_GEGLU, GLU_NONE, GLU_SWIGLU, GLU_SWIGLU_CLAMP, TYPE_Q4_K, TYPE_Q8_0,
-                      LaunchFailed, Rejected)
+from ._native import (GLU_GEGLU, GLU_NONE, GLU_SWIGLU, GLU_SWIGLU_CLAMP, SCORE_SIGMOID, SCORE_SOFTMAX,
+                      TYPE_Q4_K, TYPE_Q8_0, LaunchFailed, Rejected)
 
 __all__ = ["available", "sm_count", "device_faults", "device_faults_clear", "block_bytes", "block_elems", "q8_1_row_blocks",
            "quantize_q8", "vecq", "vecq_ranks", "mmvq", "vecq_f32", "vecq_q8", "vecq_q8_scratch", "vecq_variants", "vecq_block_sums", "mxfp8_padded_rows",
@@ -21,6 +22,8 @@ __all__ = ["available", "sm_count", "device_faults", "device_faults_clear", "blo
            "DECODER_MXFP8_ATOMS", "DECODER_BF16", "DECODER_F16", "DECODER_NVFP4_SPLIT", "DECODER_NVFP4_ATOMS",
            "DECODER_MXFP4_SPLIT", "DECODER_MXFP4_ATOMS", "mmq_quantize", "mmq_quantize_slots", "mmq", "mmq_scratch", "mmq_block_sums", "q4k_relayout", "moe_route", "grouped_gemm",
            "moe_glu_quantize", "moe_combine", "moe_ep_pack", "moe_ffn", "moe_decode", "moe_decode_fits",
+           "W4Matrix", "w4_relayout", "w4_vector", "moe_layer", "block_norm", "Logprobs", "logprobs",
+           "SCORE_SOFTMAX", "SCORE_SIGMOID",
            "mmq_glu", "grouped_gemm_glu", "TYPE_Q8_0", "TYPE_Q4_K",
            "TYPE_Q4_0", "TYPE_Q5_0", "TYPE_Q5_K", "TYPE_Q6_K", "TYPE_IQ4_NL",
            "GLU_NONE", "GLU_SWIGLU", "GLU_SWIGLU_CLAMP", "GLU_GEGLU", "Rejected", "LaunchFailed"]
@@ -877,3 +880,227 @@ def decode_grouped(decoder: int, data: torch.Tensor, x: torch.Tensor, k: int, ou
     N.check(N.lib().llmp_b200_decode_grouped(C.byref(g), _stream()), "llmp_b200_decode_grouped")
     torch.cuda.current_stream().synchronize()     # the operand table lives until here
     return out
+
+
+# ----------------------------------------------------------------------- 4-bit weights, group scales
+_FLOAT = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16}
+
+
+def _rows(t: torch.Tensor, what: str) -> int:
+    """The element type of a float [rows, values] tensor of the current device whose rows are contiguous."""
+    kind = _FLOAT.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if kind is None or t.dim() != 2 or not t.is_cuda:
+        raise Rejected(f"{what}: a CUDA F32, F16 or BF16 tensor of rows")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise Rejected(f"{what}: contiguous rows")
+    if t.get_device() != torch.cuda.current_device():
+        raise Rejected(f"{what}: on the current device")
+    return kind
+
+
+def _out(out: torch.Tensor | None, rows: int, width: int, dtype, like: torch.Tensor, what: str):
+    if out is None:
+        return torch.empty((rows, width), dtype=dtype, device=like.device)
+    _rows(out, what)
+    if tuple(out.shape) != (rows, width) or (rows > 1 and out.stride(0) < width):
+        raise Rejected(f"{what}: [{rows}, {width}]")
+    return out
+
+
+class W4Matrix:
+    """4-bit weights as the products read them (llmp_b200_w4_matrix over a slab of w4_relayout):
+    n outputs of k values, or with `glu` n gate rows and n up rows; experts of them."""
+    __slots__ = ("slab", "desc", "n", "k", "experts", "glu", "device")
+
+    def __init__(self, slab: torch.Tensor, n: int, k: int, group: int, experts: int, scale_dtype, glu: bool):
+        self.slab, self.n, self.k, self.experts, self.glu = slab, n // 2 if glu else n, k, experts, bool(glu)
+        self.device = slab.get_device()
+        self.desc = N.W4MatrixDesc(slab.data_ptr(), n, k, group, experts, _FLOAT[scale_dtype], int(glu))
+
+
+def w4_relayout(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+                glu: bool = False) -> W4Matrix:
+    """4-bit weights, once at load time, into the slab that w4_vector and moe_layer read.  codes uint8
+    [n, k / 2] or [experts, n, k / 2] (value 2 i in byte i's low nibble), scales F16 or BF16 [.., n,
+    k / group], zeros uint8 [.., n, (k / group + 1) / 2] (group 2 i in the low nibble) or None (8): a
+    weight is scale * (code - zero).  glu: the rows are n / 2 gate rows, then as many up rows.  The
+    arrays are not needed afterwards."""
+    _need(codes, torch.uint8, "w4_relayout codes")
+    if codes.get_device() != torch.cuda.current_device():
+        raise Rejected("w4_relayout: on the current device")
+    lead = tuple(codes.shape[:-2])
+    if codes.dim() not in (2, 3) or codes.stride(-1) != 1 or codes.numel() == 0:
+        raise Rejected("w4_relayout: codes uint8 [n, k / 2] or [experts, n, k / 2], rows contiguous")
+    experts = lead[0] if lead else 1
+    n, k = codes.shape[-2], 2 * codes.shape[-1]
+    if not isinstance(scales, torch.Tensor) or scales.dtype not in (torch.float16, torch.bfloat16) or \
+            scales.get_device() != codes.get_device() or scales.dim() != codes.dim() or \
+            tuple(scales.shape[:-1]) != lead + (n,) or scales.shape[-1] == 0 or \
+            (scales.stride(-1) != 1 and scales.shape[-1] > 1):
+        raise Rejected("w4_relayout: scales F16 or BF16 [.., n, k / group] on the codes' device, rows contiguous")
+    groups = scales.shape[-1]
+    if k % groups != 0 or k // groups not in (32, 64, 128):
+        raise Rejected("w4_relayout: groups of 32, 64 or 128 values")
+    if zeros is not None:
+        _need(zeros, torch.uint8, "w4_relayout zeros")
+        if zeros.get_device() != codes.get_device() or tuple(zeros.shape) != lead + (n, (groups + 1) // 2) or \
+                (zeros.stride(-1) != 1 and zeros.shape[-1] > 1):
+            raise Rejected("w4_relayout: zeros uint8 [.., n, (k / group + 1) / 2] on the codes' device, rows contiguous")
+    if glu and n % 2 != 0:
+        raise Rejected("w4_relayout: as many gate as up rows")
+    nbytes = int(N.lib().llmp_b200_w4_slab_bytes(n, k, k // groups, experts, int(glu)))
+    slab = torch.empty((nbytes,), dtype=torch.uint8, device=codes.device)
+    matrix = W4Matrix(slab, n, k, k // groups, experts, scales.dtype, glu)
+
+    def strides(t):   # (between rows, between experts); a size of one has none
+        return (t.stride(-2) if n > 1 else t.shape[-1]), (t.stride(0) if experts > 1 and lead else 0)
+    s = N.W4Source()
+    s.codes, (s.code_row, s.code_expert) = codes.data_ptr(), strides(codes)
+    s.scales, (s.scale_row, s.scale_expert) = scales.data_ptr(), strides(scales)
+    if zeros is not None:
+        s.zeros, (s.zero_row, s.zero_expert) = zeros.data_ptr(), strides(zeros)
+    N.check(N.lib().llmp_b200_w4_relayout(C.byref(s), C.byref(matrix.desc), _stream()), "llmp_b200_w4_relayout")
+    return matrix
+
+
+def w4_vector(w: W4Matrix, x: torch.Tensor, *, glu: int = GLU_NONE, limit: float = 0.0,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """x F32, F16 or BF16 [rows <= 16, k] times 4-bit weights -> [rows, n] (glu: of gate and up
+    products), in x's type or `out`'s."""
+    kind = _rows(x, "w4_vector x")
+    rows = x.shape[0]
+    if x.shape[1] != w.k or w.device != x.get_device():
+        raise Rejected("w4_vector: x [rows, k] on the weights' device")
+    out = _out(out, rows, w.n, x.dtype, x, "w4_vector output")
+    p = N.W4Product(w.desc, x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), rows, kind,
+                    _FLOAT[out.dtype], glu, limit)
+    N.check(N.lib().llmp_b200_w4_vector(C.byref(p), _stream()), "llmp_b200_w4_vector")
+    return out
+
+
+def moe_layer(x: torch.Tensor, router: torch.Tensor, gate_up: W4Matrix, down: W4Matrix, used: int, *,
+              bias: torch.Tensor | None = None, score: int = SCORE_SOFTMAX, renormalize: bool = True,
+              scale: float = 1.0, glu: int = GLU_SWIGLU, limit: float = 0.0, out: torch.Tensor | None = None):
+    """A whole mixture-of-experts layer for 1 to 16 tokens (llmp_b200_moe_layer): router's product, choice
+    of `used` experts a token, their products over 4-bit weights, weighted sum.  x [tokens, hidden],
+    router [experts, hidden] in F32, F16 or BF16, bias F32 [experts]; gate_up of [experts, 2 inter, hidden]
+    (w4_relayout glu=True), down of [experts, hidden, inter].  Returns (y [tokens, hidden] in x's type or
+    `out`'s, ids I32 [tokens, used], weights F32 [tokens, used])."""
+    kind, router_kind = _rows(x, "moe_layer x"), _rows(router, "moe_layer router")
+    tokens, hidden = x.shape
+    device = x.get_device()
+    if hidden != gate_up.k or tuple(router.shape) != (gate_up.experts, hidden) or gate_up.device != device or \
+            down.device != device:
+        raise Rejected("moe_layer: x [tokens, hidden], router [experts, hidden] and experts on one device")
+    if bias is not None:
+        _need(bias, torch.float32, "moe_layer bias")
+        if tuple(bias.shape) != (gate_up.experts,) or not bias.is_contiguous() or bias.get_device() != device:
+            raise Rejected("moe_layer: bias F32 [experts]")
+    if not 1 <= used <= min(16, gate_up.experts) or tokens > 16:
+        raise Rejected("moe_layer: 1 to 16 experts a token, no more than there are, 1 to 16 tokens")
+    out = _out(out, tokens, hidden, x.dtype, x, "moe_layer output")
+    ids = torch.empty((tokens, used), dtype=torch.int32, device=x.device)
+    weights = torch.empty((tokens, used), dtype=torch.float32, device=x.device)
+    L = N.lib()
+    scratch = torch.empty((int(L.llmp_b200_moe_layer_scratch(used, tokens, gate_up.n)),), dtype=torch.uint8, device=x.device)
+    d = N.MoeLayerDesc(x.data_ptr(), x.stride(0), router.data_ptr(), router.stride(0),
+                       bias.data_ptr() if bias is not None else None, gate_up.desc, down.desc, out.data_ptr(),
+                       out.stride(0), ids.data_ptr(), weights.data_ptr(), scratch.data_ptr(), kind, router_kind,
+                       _FLOAT[out.dtype], tokens, used, score, int(renormalize), scale, glu, limit)
+    N.check(L.llmp_b200_moe_layer(C.byref(d), _stream()), "llmp_b200_moe_layer")
+    return out, ids, weights
+
+
+# ----------------------------------------------------------------------- between the products
+def block_norm(block: torch.Tensor, residual: torch.Tensor | None = None, *, pre: torch.Tensor | None = None,
+               post: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float = 1.0,
+               offset: float = 0.0, eps: float = 1e-6, out_residual: torch.Tensor | None = None,
+               out: torch.Tensor | None = None, q8: bool = False):
+    """r = residual + scale * gate * rms_norm(block, offset + post), h = rms_norm(r, offset + pre) in one kernel
+    (llmp_b200_block_norm).  block and residual [rows, width] of one type, gate of that type [width] or
+    [rows, width], post and pre [width] of that type or F32; each but block may be None.  Returns (r, h), h
+    None without pre; with q8 (F32 rows) (r, h, h's Q8_1 rows as quantize_q8 makes them).  out_residual
+    may be residual."""
+    kind = _rows(block, "block_norm block")
+    rows, width = block.shape
+    device = block.get_device()
+    d = N.BlockNormDesc()
+    d.block, d.block_stride, d.rows, d.width, d.type = block.data_ptr(), block.stride(0), rows, width, kind
+    if residual is not None:
+        if _rows(residual, "block_norm residual") != kind or residual.shape != block.shape:
+            raise Rejected("block_norm: a residual like the block's output")
+        d.residual, d.residual_stride = residual.data_ptr(), residual.stride(0)
+    if gate is not None:
+        if gate.dim() == 1:
+            gate = gate.unsqueeze(0)
+        if _rows(gate, "block_norm gate") != kind or tuple(gate.shape) not in ((1, width), (rows, width)):
+            raise Rejected("block_norm: a gate [width] or [rows, width] of the rows' type")
+        d.gate, d.gate_stride = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else 0
+    d.weight_type = kind
+    for name, weight in (("post", post), ("pre", pre)):
+        if weight is None:
+            continue
+        if not isinstance(weight, torch.Tensor) or weight.get_device() != device or tuple(weight.shape) != (width,) or \
+                (weight.stride(0) != 1 and width > 1) or weight.dtype not in (block.dtype, torch.float32):
+            raise Rejected(f"block_norm: {name} [width] of the rows' type or F32")
+        setattr(d, name, weight.data_ptr())
+        d.weight_type = _FLOAT[weight.dtype]
+    if post is not None and pre is not None and post.dtype != pre.dtype:
+        raise Rejected("block_norm: post and pre of one type")
+    if pre is None and (out is not None or q8):
+        raise Rejected("block_norm: a second norm's weight")
+    for t in (out_residual, out):
+        if t is not None and t.dtype != block.dtype:
+            raise Rejected("block_norm: outputs of the rows' type")
+    out_residual = _out(out_residual, rows, width, block.dtype, block, "block_norm out_residual")
+    d.out_residual, d.out_residual_stride = out_residual.data_ptr(), out_residual.stride(0)
+    blocks = None
+    if pre is not None:
+        out = _out(out, rows, width, block.dtype, block, "block_norm output")
+        d.out, d.out_stride = out.data_ptr(), out.stride(0)
+        if q8:
+            if kind != N.TYPE_F32:
+                raise Rejected("block_norm: Q8_1 rows of F32 ones")
+            blocks = torch.empty((rows, q8_1_row_blocks(width) * 36), dtype=torch.uint8, device=block.device)
+            d.q8 = blocks.data_ptr()
+    d.scale, d.offset, d.eps = scale, offset, eps
+    N.check(N.lib().llmp_b200_block_norm(C.byref(d), _stream()), "llmp_b200_block_norm")
+    return (out_residual, out, blocks) if q8 else (out_residual, out)
+
+
+class Logprobs(NamedTuple):
+    """What logprobs returns."""
+    logprobs: torch.Tensor      # F32 [rows, given]
+    ranks: torch.Tensor         # I32 [rows, given], 1 for the largest logit
+    entropy: torch.Tensor       # F32 [rows]
+    top_ids: torch.Tensor       # I32 [rows, top]
+    top_logprobs: torch.Tensor  # F32 [rows, top]
+
+
+def logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: int = 0,
+             temperature: float = 1.0) -> Logprobs:
+    """Log probabilities and ranks of given tokens (I32 [rows, given <= 16] or None), the entropy and the
+    `top` <= 32 largest of logits F32, F16 or BF16 [rows, vocab] (llmp_b200_logprobs).  Masked logits are
+    -inf."""
+    kind = _rows(logits, "logprobs logits")
+    rows, vocab = logits.shape
+    given = 0
+    if tokens is not None:
+        _need(tokens, torch.int32, "logprobs tokens")
+        if tokens.dim() != 2 or tokens.shape[0] != rows or not tokens.is_contiguous() or \
+                tokens.get_device() != logits.get_device():
+            raise Rejected("logprobs: packed tokens I32 [rows, given] on the logits' device")
+        given = tokens.shape[1]
+    if not 0 <= given <= 16 or not 0 <= top <= min(32, vocab):
+        raise Rejected("logprobs: up to 16 given tokens a row and 32 alternatives, no more than there are logits")
+    device = logits.device
+    r = Logprobs(torch.empty((rows, given), dtype=torch.float32, device=device),
+                 torch.empty((rows, given), dtype=torch.int32, device=device),
+                 torch.empty((rows,), dtype=torch.float32, device=device),
+                 torch.empty((rows, top), dtype=torch.int32, device=device),
+                 torch.empty((rows, top), dtype=torch.float32, device=device))
+    d = N.LogprobsDesc(logits.data_ptr(), logits.stride(0), tokens.data_ptr() if given else None,
+                       r.logprobs.data_ptr(), r.ranks.data_ptr(), r.entropy.data_ptr(), r.top_ids.data_ptr(),
+                       r.top_logprobs.data_ptr(), rows, kind, vocab, given, top, temperature)
+    N.check(N.lib().llmp_b200_logprobs(C.byref(d), _stream()), "llmp_b200_logprobs")
+    return r
