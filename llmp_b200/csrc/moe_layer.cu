@@ -90,7 +90,7 @@ struct FirstShared {
 template <int kType, int kRouter, int kTiles>
 __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_t* staged, int first_expert, int tokens,
                                            int warp, int lane, double (&partial)[kTileRows][kMaxTokens]) {
-  constexpr int kPieces = Pieces(kType), kRouterPieces = Pieces(kRouter);
+  constexpr int kPieces = Pieces(kType, true), kRouterPieces = Pieces(kRouter, true);
   const int g = lane >> 2, t = lane & 3;
   const int piece = g % Cols(kPieces);
   const int tiles = (tokens + TokensATile(kPieces) - 1) / TokensATile(kPieces);
@@ -104,8 +104,8 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
   for (int b = warp * blocks / kWarps; b < (warp + 1) * blocks / kWarps; ++b) {
     uint4 qa[kRouterPieces], qb[kRouterPieces];
     const int at = (32 * b) + (8 * t);
-    LoadSplit8<kRouter, false>(base + (row_a * row_bytes), at, row_a < a.experts ? 8 : 0, a.router_vec, qa);
-    LoadSplit8<kRouter, false>(base + (row_b * row_bytes), at, row_b < a.experts ? 8 : 0, a.router_vec, qb);
+    LoadSplit8<kRouter, false, true>(base + (row_a * row_bytes), at, row_a < a.experts ? 8 : 0, a.router_vec, qa);
+    LoadSplit8<kRouter, false, true>(base + (row_b * row_bytes), at, row_b < a.experts ? 8 : 0, a.router_vec, qb);
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       if (nt >= tiles) break;
@@ -117,8 +117,8 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
 #pragma unroll
       for (int r = 0; r < kRouterPieces; ++r) {
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        Mma(sum, qa[r].x, qb[r].x, qa[r].y, qb[r].y, x.x, x.y);
-        Mma(sum, qa[r].z, qb[r].z, qa[r].w, qb[r].w, x.z, x.w);
+        Mma<false, true>(sum, qa[r].x, qb[r].x, qa[r].y, qb[r].y, x.x, x.y);
+        Mma<false, false>(sum, qa[r].z, qb[r].z, qa[r].w, qb[r].w, x.z, x.w);
 #pragma unroll
         for (int c = 0; c < 4; ++c) total[nt][c] += sum[c];
       }
@@ -152,13 +152,13 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
 // Tokens token_of(0 .. count - 1) of x as pieces in shared memory.
 template <int kType, typename Token>
 __device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* staged, int count, Token token_of) {
-  constexpr int kPieces = Pieces(kType);
+  constexpr int kPieces = Pieces(kType, true);
   const int padded = a.steps_up * kStep;
   for (int i = static_cast<int>(threadIdx.x); i < count * (padded / 8); i += kThreads) {
     const int c = i / (padded / 8), at = (i % (padded / 8)) * 8;
     uint4 quads[kPieces];
     const auto* row = static_cast<const std::uint8_t*>(a.x) + (token_of(c) * a.x_stride * TypeBytes(kType));
-    LoadSplit8<kType>(row, at, a.hidden - at, a.x_vec, quads);
+    LoadSplit8<kType, true, true>(row, at, a.hidden - at, a.x_vec, quads);
 #pragma unroll
     for (int s = 0; s < kPieces; ++s) {
       *reinterpret_cast<uint4*>(staged + (((c * kPieces) + s) * a.x_pitch) + (at * 2)) = quads[s];
@@ -225,7 +225,7 @@ __device__ __forceinline__ void Choose(const LayerArgs& a, float* logits, int t,
 template <int kType, int kGroups>
 __global__ void __launch_bounds__(kThreads)
 FirstKernel(const LayerArgs a) {
-  constexpr int kPieces = Pieces(kType);
+  constexpr int kPieces = Pieces(kType, true);
   constexpr int kTiles = kMaxTokens / TokensATile(kPieces);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
@@ -366,7 +366,7 @@ FirstKernel(const LayerArgs a) {
     for (int step = step0; step < step1; ++step, block += kBlock) {
       StepWeights<kGroups> w;
       w.Load(block, lane);
-      MultiplyStep<kGroups, kTiles>(w, a.bf16_up, tiles, total, [&](int nt, int i) {
+      MultiplyStep<false, kGroups, kTiles>(w, a.bf16_up, tiles, total, [&](int nt, int i) {
         if (column_at[nt] == 0xffffffffu) return make_uint4(0, 0, 0, 0);
         return *reinterpret_cast<const uint4*>(staged + column_at[nt] + (step * 256) + (i * 64));
       });
@@ -449,7 +449,7 @@ SecondKernel(const LayerArgs a) {
     for (int step = step0; step < step1; ++step, block += kBlock) {
       StepWeights<kGroups> w;
       w.Load(block, lane);
-      MultiplyStep<kGroups, kTiles>(w, a.bf16_down, tiles, total, [&](int nt, int b) {
+      MultiplyStep<false, kGroups, kTiles>(w, a.bf16_down, tiles, total, [&](int nt, int b) {
         const int at = (step * kStep) + (32 * b);  // inter is whole 32-value blocks
         if (column[nt] == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
         return __ldcg(reinterpret_cast<const uint4*>(column[nt] + at));
@@ -499,7 +499,7 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   if (const cudaError_t e = Configure(FirstKernel<kType, kGroups>, configured_device, kFirstSmemLimit); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  const int smem = (a.cap * Pieces(kType) * a.x_pitch) + (a.tokens * a.experts * 4);
+  const int smem = (a.cap * Pieces(kType, true) * a.x_pitch) + (a.tokens * a.experts * 4);
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
   const std::int64_t units = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) * a.tiles_up;
   const std::int64_t most = std::max<std::int64_t>(1, static_cast<std::int64_t>(SmCount()) * 2 / kCluster);
@@ -604,7 +604,7 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.choice = static_cast<Choice*>(d.scratch);
   a.h = reinterpret_cast<unsigned short*>(static_cast<std::uint8_t*>(d.scratch) + ChoiceBytes());
   a.x_pitch = (a.steps_up * kStep * 2) + 64;
-  a.cap = std::max(1, std::min(d.tokens, kXBudget / (Pieces(d.x_type) * a.x_pitch)));
+  a.cap = std::max(1, std::min(d.tokens, kXBudget / (Pieces(d.x_type, true) * a.x_pitch)));
   const auto s = static_cast<cudaStream_t>(stream);
   if (d.x_type == kF32) return LaunchLayer<kF32>(d.gate_up.group, d.down.group, a, s);
   if (d.x_type == kF16) return LaunchLayer<kF16>(d.gate_up.group, d.down.group, a, s);

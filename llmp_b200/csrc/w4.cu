@@ -2,9 +2,11 @@
 // matrix-vector products of 1 to 16 activation rows, plain or as the GLU of a gate and an up
 // product.  No counterpart in the reference's templates (its affine decoders,
 // src/kernels/decode, are the nearest); stands beside decode_vector.cu and mxfp8_gemv.cu.
-#include "w4.cuh"
+#include <cooperative_groups.h>
 
 #include <algorithm>
+
+#include "w4.cuh"
 
 namespace llmp_b200 {
 namespace w4 {
@@ -23,8 +25,8 @@ int CheckMatrix(const llmp_b200_w4_matrix& m, const char* what) {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+namespace cg = cooperative_groups;
+
 
 struct Source {
   llmp_b200_w4_source s;
@@ -105,6 +107,9 @@ RelayoutKernel(const Source a, std::uint8_t* __restrict__ slab) {
 struct VectorArgs {
   const std::uint8_t* slab;
   int tiles, steps, k, outputs, rows;
+  int warps, parts;   // warps a CTA; of them `parts` divide a tile's steps
+  int rounds;         // of warps / parts tiles
+  int meet_floats;    // one buffer of partial sums
   const void* x;
   std::int64_t x_stride;
   bool x_vec;
@@ -116,103 +121,193 @@ struct VectorArgs {
   float limit;
 };
 
-// Staged activations: kChunk values a column at a pitch of 64 more bytes, so the two columns that a
-// quarter warp reads (64 bytes each) lie in different halves of the banks.
-constexpr int kChunk = 1024;
-constexpr int kPitch = (kChunk * 2) + 64;
+// Staged activations: a column's values at a pitch of 64 more bytes than whole steps, so the two
+// columns that a quarter warp reads (64 bytes each) lie in different halves of the banks.
+__host__ __device__ constexpr int Pitch(int steps) { return (steps * kStep * 2) + 64; }
 
-// A warp a tile of 16 rows over all of k; the activations staged a chunk at a time.
+// Persistent CTAs.  A round is a few tiles of 16 weight rows, each tile's steps divided among `parts`
+// warps, whose sums meet in shared memory: with one token a matrix of 4096 x 4096 is 8.7 MB in 256 tiles,
+// too few for a warp each.  The activations are staged (and split) once a CTA.  Weights come
+// through a ring of kSlots steps a warp (cp.async, its own lanes' copies: no CTA barrier, any depth of
+// requests without registers) that runs on from one round's tile to the next.  Where the activations
+// of all of k do not fit, the CTAs of a cluster divide k as well and read each other's sums.
+constexpr int kSlots = 4;
+constexpr int kMaxWarps = 16;
+
 template <int kTiles, int kType, int kGroups>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kMaxWarps * 32, 1)
 VectorKernel(const VectorArgs a) {
   constexpr int kPieces = Pieces(kType);
+  constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int clusters = static_cast<int>(gridDim.x) / ranks, first_round = static_cast<int>(blockIdx.x) / ranks;
+  const int threads = a.warps * 32;
   const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int step0 = a.steps * rank / ranks, steps = (a.steps * (rank + 1) / ranks) - step0;  // this CTA's
+  const int tiles_a_round = a.warps / a.parts;
+  const int my_tile = warp / a.parts, part = warp % a.parts;
+  const int begin = steps * part / a.parts, count = (steps * (part + 1) / a.parts) - begin;  // this warp's
+  const int pitch = Pitch(steps), columns = a.rows * kPieces;
+  std::uint8_t* ring = smem + (warp * kSlots * kBlock);
+  float* meet = reinterpret_cast<float*>(smem + (a.warps * kSlots * kBlock));  // [2][warps][rows][16]
+  std::uint8_t* staged = reinterpret_cast<std::uint8_t*>(meet + (2 * a.meet_floats));  // and a column of zeros
+
+  // the requests' place in this warp's sequence of steps: round after round
+  int load_round = first_round, load_step = 0;
+  auto request = [&](int slot) {  // one commit a call, so that the waits can count
+    const int tile = (load_round * tiles_a_round) + my_tile;
+    if (load_round < a.rounds && tile < a.tiles && count > 0) {
+      const std::uint8_t* src =
+          a.slab + ((static_cast<std::size_t>(tile) * a.steps) + step0 + begin + load_step) * kBlock + (lane * 16);
+      std::uint8_t* dst = ring + (slot * kBlock) + (lane * 16);
+      CopyAsync16(dst, src);
+      CopyAsync16(dst + 512, src + 512);
+      if (lane < 4 * kGroups) CopyAsync16(dst + 1024, src + 1024);
+    }
+    CopyAsyncCommit();
+    if (++load_step >= count) load_step = 0, load_round += clusters;
+  };
   GridLaunchDependents();
   GridDependencyWait();
-  const int tile = (static_cast<int>(blockIdx.x) * kWarps) + warp;
-  const bool live = tile < a.tiles;
-  constexpr int kBlock = BlockBytes(kStep / kGroups);
-  const std::uint8_t* block = a.slab + (static_cast<std::size_t>(live ? tile : 0) * a.steps * kBlock);
-  float total[kTiles][4];
 #pragma unroll
-  for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
-  // this lane's column of each column tile: the token and piece it stands for
+  for (int i = 0; i < kSlots - 1; ++i) request(i);
+
+  const int octets = steps * (kStep / 8);
+  for (int token = 0; token < a.rows; ++token) {
+    const auto* row = static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType));
+    for (int i = static_cast<int>(threadIdx.x); i < octets; i += threads) {
+      uint4 quads[kPieces];
+      const int at = (step0 * kStep) + (i * 8);
+      LoadSplit8<kType>(row, at, a.k - at, a.x_vec, quads);
+#pragma unroll
+      for (int s = 0; s < kPieces; ++s) {
+        *reinterpret_cast<uint4*>(staged + (((token * kPieces) + s) * pitch) + (i * 16)) = quads[s];
+      }
+    }
+  }
+  for (int i = static_cast<int>(threadIdx.x); i < octets; i += threads) {
+    *reinterpret_cast<uint4*>(staged + (columns * pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
+  }
+  // this lane's column of each column tile: the token and piece it stands for, or the zeros
   const int piece = g % Cols(kPieces);
-  std::uint32_t column_at[kTiles];
+  const std::uint8_t* column[kTiles];
 #pragma unroll
   for (int nt = 0; nt < kTiles; ++nt) {
     const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-    const bool real = token < a.rows && piece < kPieces;
-    column_at[nt] = real ? static_cast<std::uint32_t>(((token * kPieces) + piece) * kPitch + (t * 16)) : 0xffffffffu;
+    const int c = token < a.rows && piece < kPieces ? (token * kPieces) + piece : columns;
+    column[nt] = staged + (c * pitch) + (t * 16) + (begin * 256);
   }
-  for (int first = 0; first < a.k; first += kChunk) {
-    __syncthreads();
-    const int values = min(kChunk, a.k - first);
-    const int padded = (values + kStep - 1) / kStep * kStep;
-    for (int i = static_cast<int>(threadIdx.x); i < a.rows * (padded / 8); i += kThreads) {
-      const int token = i / (padded / 8), at = (i % (padded / 8)) * 8;
-      uint4 quads[kPieces];
-      const auto* row = static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType));
-      LoadSplit8<kType>(row, first + at, values - at, a.x_vec, quads);
+  __syncthreads();
+
+  int slot = 0, buffer = 0;
+  for (int round = first_round; round < a.rounds; round += clusters, buffer ^= 1) {
+    const bool live = (round * tiles_a_round) + my_tile < a.tiles;
+    float total[kTiles][4];
 #pragma unroll
-      for (int s = 0; s < kPieces; ++s) {
-        *reinterpret_cast<uint4*>(smem + (((token * kPieces) + s) * kPitch) + (at * 2)) = quads[s];
+    for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
+    for (int step = 0; step < count; ++step) {
+      CopyAsyncWait<kSlots - 2>();
+      __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
+      request(slot == 0 ? kSlots - 1 : slot - 1);
+      if (live) {
+        StepWeights<kGroups> w;
+        w.LoadShared(ring + (slot * kBlock), lane);
+        MultiplyStep<kType == kF16, kGroups, kTiles>(w, a.bf16_scales, kTiles, total, [&](int nt, int i) {
+          return *reinterpret_cast<const uint4*>(column[nt] + (step * 256) + (i * 64));
+        });
       }
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
     }
-    __syncthreads();
-    if (!live) continue;
-    for (int step = 0; step < padded / kStep; ++step, block += kBlock) {
-      StepWeights<kGroups> w;
-      w.Load(block, lane);
-      MultiplyStep<kGroups, kTiles>(w, a.bf16_scales, kTiles, total, [&](int nt, int i) {
-        if (column_at[nt] == 0xffffffffu) return make_uint4(0, 0, 0, 0);
-        return *reinterpret_cast<const uint4*>(smem + column_at[nt] + (step * 256) + (i * 64));
-      });
-    }
-  }
-  if (!live) return;
+    float* mine = meet + (buffer * a.meet_floats) + (warp * kTileRows * a.rows);
 #pragma unroll
-  for (int nt = 0; nt < kTiles; ++nt) {
-    float v[2][2];
-    FoldColumns<kPieces>(total[nt], v);
+    for (int nt = 0; nt < kTiles; ++nt) {
+      float v[2][2];
+      FoldColumns<kPieces>(total[nt], v);
 #pragma unroll
-    for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
-      const int token = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t, j);
-      if (token >= a.rows) continue;
-      if (a.glu != LLMP_B200_GLU_NONE) {
-        const int row = (tile * 8) + g;
-        if (row < a.outputs) {
-          StoreValue(a.y, (token * a.y_stride) + row, a.y_type,
-                     Glu(a.glu, v[0][j] * Up(kType), v[1][j] * Up(kType), a.limit));
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = (tile * 16) + g + (8 * r);
-          if (row < a.outputs) StoreValue(a.y, (token * a.y_stride) + row, a.y_type, v[r][j] * Up(kType));
+      for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
+        const int token = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t, j);
+        if (token < a.rows && (kPieces != 3 || (t & 1) == 0)) {
+          mine[(token * kTileRows) + g] = v[0][j];
+          mine[(token * kTileRows) + g + 8] = v[1][j];
         }
       }
     }
+    // two buffers: who writes one again has passed the barrier behind its last readers
+    if (ranks > 1) cluster.sync(); else __syncthreads();
+    const int height = a.glu != LLMP_B200_GLU_NONE ? 8 : 16;
+    const int outputs = tiles_a_round * a.rows * height;
+    for (int i = (rank * threads) + static_cast<int>(threadIdx.x); i < outputs; i += threads * ranks) {
+      const int r = i % height, token = (i / height) % a.rows, o = (i / height) / a.rows;
+      const int tile = (round * tiles_a_round) + o, row = (tile * height) + r;
+      if (tile >= a.tiles || row >= a.outputs) continue;
+      const int at = (buffer * a.meet_floats) + (((o * a.parts * a.rows) + token) * kTileRows) + r;
+      float first = 0.0f, second = 0.0f;
+      for (int q = 0; q < ranks; ++q) {
+        const float* p = (ranks > 1 ? cluster.map_shared_rank(meet, q) : meet) + at;
+        for (int s = 0; s < a.parts; ++s) {
+          first += p[s * kTileRows * a.rows];
+          if (height == 8) second += p[(s * kTileRows * a.rows) + 8];
+        }
+      }
+      const float v = height == 8 ? Glu(a.glu, first * Up(kType), second * Up(kType), a.limit) : first * Up(kType);
+      StoreValue(a.y, (token * a.y_stride) + row, a.y_type, v);
+    }
   }
+  if (ranks > 1) cluster.sync();  // nobody leaves while another reads its sums
+}
+
+constexpr int kSmemLimit = 224 * 1024;
+constexpr int kMaxRanks = 8;
+// Shared memory of a CTA: rings, two buffers of sums, the staged activations.
+std::int64_t SmemBytes(int warps, int ranks, int rows, int steps, int type, int block_bytes) {
+  return (static_cast<std::int64_t>(warps) * kSlots * block_bytes) + (2 * warps * kTileRows * rows * 4) +
+         (((rows * Pieces(type)) + 1) * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
 }
 
 template <int kTiles, int kType, int kGroups>
-int LaunchVector(const VectorArgs& a, cudaStream_t stream) {
-  const int smem = a.rows * Pieces(kType) * kPitch;
+int LaunchVector(VectorArgs a, cudaStream_t stream) {
   static thread_local int configured_device = -1;
   int device = -1;
   cudaGetDevice(&device);
   if (configured_device != device) {
-    const cudaError_t set = cudaFuncSetAttribute(VectorKernel<kTiles, kType, kGroups>,
-                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, 16 * Pieces(kType) * kPitch);
+    const cudaError_t set = cudaFuncSetAttribute(VectorKernel<kTiles, kType, kGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 kSmemLimit);
     if (set != cudaSuccess) return Failed(set, "w4_vector attribute");
     configured_device = device;
   }
-  const dim3 grid(static_cast<unsigned>((a.tiles + kWarps - 1) / kWarps));
-  const cudaError_t e = LaunchPdl(VectorKernel<kTiles, kType, kGroups>, grid, dim3(kThreads),
-                                  static_cast<std::size_t>(smem), stream, a);
+  auto bytes = [&](int warps, int ranks) {
+    return SmemBytes(warps, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
+  };
+  // two CTAs of eight warps an SM where the staged activations allow it, else one of sixteen, else as few ranks as
+  // their memory needs
+  int ranks = 1, per_sm = 2;
+  a.warps = 8;
+  if (bytes(8, 1) > 112 * 1024) {
+    a.warps = 16, per_sm = 1;
+    while (ranks < kMaxRanks && bytes(16, ranks) > kSmemLimit) ranks *= 2;
+  }
+  const int ctas = std::max(1, SmCount() * per_sm / ranks);
+  a.parts = a.warps;
+  while (a.parts > 1 && (a.parts > a.steps / ranks || a.tiles >= 4 * ctas * (2 * a.warps / a.parts))) a.parts /= 2;
+  a.rounds = (a.tiles + (a.warps / a.parts) - 1) / (a.warps / a.parts);
+  a.meet_floats = a.warps * kTileRows * a.rows;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(std::min(a.rounds, ctas) * ranks));
+  config.blockDim = dim3(static_cast<unsigned>(a.warps * 32));
+  config.dynamicSmemBytes = static_cast<std::size_t>(bytes(a.warps, ranks));
+  config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  attribute[1].id = cudaLaunchAttributeClusterDimension;
+  attribute[1].val.clusterDim.x = static_cast<unsigned>(ranks);
+  attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
+  config.attrs = attribute;
+  config.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&config, VectorKernel<kTiles, kType, kGroups>, a);
   return e == cudaSuccess ? 0 : Failed(e, "w4_vector launch");
 }
 
@@ -282,6 +377,7 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream) {
   const llmp_b200_w4_product& p = *product;
   if (const int status = w4::CheckMatrix(p.w, "w4_vector"); status != 0) return status;
   if (p.w.experts != 1) return Reject("w4_vector: one matrix");
+  if (p.w.k > 131072) return Reject("w4_vector: k up to 131072");
   if (p.rows == 0) return 0;
   if (p.x == nullptr || p.y == nullptr) return Reject("w4_vector: activations and an output");
   if (p.rows < 1 || p.rows > 16) return Reject("w4_vector: 1 to 16 rows");
@@ -306,9 +402,20 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream) {
   a.bf16_scales = p.w.scale_type == w4::kBF16;
   a.glu = p.glu, a.limit = p.limit;
   const auto s = static_cast<cudaStream_t>(stream);
-  if (p.x_type == w4::kF32) return w4::LaunchTiles<w4::kF32>(p.w.group, a, s);
-  if (p.x_type == w4::kF16) return w4::LaunchTiles<w4::kF16>(p.w.group, a, s);
-  return w4::LaunchTiles<w4::kBF16>(p.w.group, a, s);
+  // as many rows a launch as a cluster's shared memory takes: all of them but for very long ones
+  const int block_bytes = w4::BlockBytes(p.w.group);
+  int most = p.rows;
+  while (most > 1 && w4::SmemBytes(16, w4::kMaxRanks, most, a.steps, p.x_type, block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
+  for (int first = 0; first < p.rows; first += most) {
+    a.rows = std::min(most, p.rows - first);
+    a.x = static_cast<const std::uint8_t*>(p.x) + (first * p.x_stride * xb);
+    a.y = static_cast<std::uint8_t*>(p.y) + (first * p.y_stride * w4::TypeBytes(p.y_type));
+    const int status = p.x_type == w4::kF32   ? w4::LaunchTiles<w4::kF32>(p.w.group, a, s)
+                       : p.x_type == w4::kF16 ? w4::LaunchTiles<w4::kF16>(p.w.group, a, s)
+                                              : w4::LaunchTiles<w4::kBF16>(p.w.group, a, s);
+    if (status != 0) return status;
+  }
+  return 0;
 }
 
 }  // extern "C"

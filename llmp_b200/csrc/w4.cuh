@@ -20,10 +20,10 @@
 // that nothing overflows that the scaled product would not.
 //
 // The tokens are the MMA's 8 columns.  A product is exact (code - zero has 5 bits, a bf16 column
-// 8), sums are F32, and the scale multiplies a group's F32 sum, so nothing is rounded to fewer
-// bits.  F16 and F32 activations are split into 2 and 3 bf16 columns whose sum they are, exactly
-// (11 and 24 significant bits in pieces of 8); a token takes kCols = 1, 2 or 4 columns (one of
-// the 4 is zero).
+// 8, an f16 one 11), sums are F32, and the scale multiplies a group's F32 sum, so nothing is
+// rounded to fewer bits.  BF16 and F16 activations are columns as they are, with the codes in the same
+// type (0x6400 is 1024 in f16); an F32 one is split into 3 bf16 columns whose sum it is, exactly
+// (24 significant bits in pieces of 8).  A token takes 1, 2 or 4 columns (one of the 4 is zero).
 #ifndef LLMP_B200_CSRC_W4_CUH_
 #define LLMP_B200_CSRC_W4_CUH_
 
@@ -48,8 +48,10 @@ __host__ __device__ constexpr int Tiles(int n, int glu) {
 constexpr int kF32 = LLMP_B200_TYPE_F32, kF16 = LLMP_B200_TYPE_F16, kBF16 = LLMP_B200_TYPE_BF16;
 inline bool FloatType(int t) { return t == kF32 || t == kF16 || t == kBF16; }
 __host__ __device__ constexpr int TypeBytes(int t) { return t == kF32 ? 4 : 2; }
-// bf16 pieces that a value of the type is the sum of.
-__host__ __device__ constexpr int Pieces(int t) { return t == kF32 ? 3 : t == kF16 ? 2 : 1; }
+// The columns that a value of the type is the sum of: itself, or bf16 pieces (bf16_only: f16 in pieces too).
+__host__ __device__ constexpr int Pieces(int t, bool bf16_only = false) {
+  return t == kF32 ? 3 : t == kF16 && bf16_only ? 2 : 1;
+}
 
 // Activations enter this much smaller, results leave this much larger.
 __host__ __device__ constexpr float Down(int t) { return t == kF16 ? 1.0f : 0x1p-11f; }
@@ -92,79 +94,126 @@ __device__ __forceinline__ void Split(float x, std::uint32_t (&bits)[kPieces]) {
 }
 
 // Eight consecutive values (zero from `valid` on) times Down as pieces, a 16-byte quad a piece.
-template <int kType, bool kDown = true>
+template <int kType, bool kDown = true, bool kBf16Only = false>
 __device__ __forceinline__ void LoadSplit8(const void* row, std::int64_t at, int valid, bool vec,
-                                           uint4 (&quads)[Pieces(kType)]) {
-  constexpr int kPieces = Pieces(kType);
-  if constexpr (kType == kBF16) {
+                                           uint4 (&quads)[Pieces(kType, kBf16Only)]) {
+  constexpr int kPieces = Pieces(kType, kBf16Only);
+  if constexpr (kPieces > 1) {
+    float v[8];
     if (vec && valid >= 8) {
-      uint4 q = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
-      if constexpr (kDown) {
-        auto* pairs = reinterpret_cast<__nv_bfloat162*>(&q);
+      if constexpr (kType == kF32) {
+        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
+        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
+        const std::uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pairs[i] = __hmul2(pairs[i], __float2bfloat162_rn(Down(kType)));
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = HalfBitsToFloat(w[i] & 0xffffu);
+          v[(2 * i) + 1] = HalfBitsToFloat(w[i] >> 16);
+        }
       }
-      quads[0] = q;
-      return;
-    }
-  }
-  float v[8];
-  if (vec && valid >= 8) {
-    if constexpr (kType == kF32) {
-      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
-      const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
-      const std::uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < valid ? LoadValue(row, at + i, kType) : 0.0f;
+    }
+    std::uint32_t packed[kPieces][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      std::uint32_t lo[kPieces], hi[kPieces];
+      Split<kPieces>(kDown && kType == kF32 ? v[2 * i] * Down(kType) : v[2 * i], lo);
+      Split<kPieces>(kDown && kType == kF32 ? v[(2 * i) + 1] * Down(kType) : v[(2 * i) + 1], hi);
+#pragma unroll
+      for (int s = 0; s < kPieces; ++s) packed[s][i] = lo[s] | (hi[s] << 16);
+    }
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
+  } else {
+    uint4 q;
+    if (vec && valid >= 8) {
+      q = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
+    } else {
+      std::uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v[2 * i] = HalfBitsToFloat(w[i] & 0xffffu);
-        v[(2 * i) + 1] = HalfBitsToFloat(w[i] >> 16);
+        const auto* p = static_cast<const unsigned short*>(row) + at + (2 * i);
+        w[i] = (2 * i) < valid ? p[0] : 0u;
+        if ((2 * i) + 1 < valid) w[i] |= static_cast<std::uint32_t>(p[1]) << 16;
       }
+      q = make_uint4(w[0], w[1], w[2], w[3]);
     }
-  } else {
+    if constexpr (kDown && kType == kBF16) {
+      auto* pairs = reinterpret_cast<__nv_bfloat162*>(&q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < valid ? LoadValue(row, at + i, kType) : 0.0f;
+      for (int i = 0; i < 4; ++i) pairs[i] = __hmul2(pairs[i], __float2bfloat162_rn(Down(kType)));
+    }
+    quads[0] = q;
   }
-  if constexpr (kDown && kType != kF16) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= Down(kType);
-  }
-  std::uint32_t packed[kPieces][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    std::uint32_t lo[kPieces], hi[kPieces];
-    Split<kPieces>(v[2 * i], lo);
-    Split<kPieces>(v[(2 * i) + 1], hi);
-#pragma unroll
-    for (int s = 0; s < kPieces; ++s) packed[s][i] = lo[s] | (hi[s] << 16);
-  }
-#pragma unroll
-  for (int s = 0; s < kPieces; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
 }
 
 // Columns a token takes, tokens an MMA's 8 columns hold.
 __host__ __device__ constexpr int Cols(int pieces) { return pieces == 3 ? 4 : pieces; }
 __host__ __device__ constexpr int TokensATile(int pieces) { return 8 / Cols(pieces); }
 
+// c += A B, or c = A B (kFirst: no registers to clear); kHalf: f16 operands, else bf16.
+template <bool kHalf, bool kFirst>
 __device__ __forceinline__ void Mma(float (&c)[4], std::uint32_t a0, std::uint32_t a1, std::uint32_t a2,
                                     std::uint32_t a3, std::uint32_t b0, std::uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (kFirst && kHalf) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  } else if constexpr (kFirst) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+  } else if constexpr (kHalf) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
 }
 
-// Two codes at bits 0 and 16 of w >> 4 j as bf16 values less (128 + zero) twice.
+// Two codes at bits 0 and 16 of w >> 4 j as values of the MMA's type, less 128 (f16: 1024) + zero twice.
+template <bool kHalf>
 __device__ __forceinline__ std::uint32_t Pair(std::uint32_t w, int j, std::uint32_t zero2) {
-  const std::uint32_t biased = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
-  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased),
-                                   *reinterpret_cast<const __nv_bfloat162*>(&zero2));
-  return *reinterpret_cast<const std::uint32_t*>(&v);
+  const std::uint32_t biased = ((w >> (4 * j)) & 0x000f000fu) | (kHalf ? 0x64006400u : 0x43004300u);
+  if constexpr (kHalf) {
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&zero2));
+    return *reinterpret_cast<const std::uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&zero2));
+    return *reinterpret_cast<const std::uint32_t*>(&v);
+  }
 }
-__device__ __forceinline__ std::uint32_t Zero2(std::uint32_t word) { return __byte_perm(word, 0, 0x3232); }
+// A word's 128 + zero twice; the same last bits after 1024's exponent are 1024 + zero in f16.
+template <bool kHalf>
+__device__ __forceinline__ std::uint32_t Zero2(std::uint32_t word) {
+  return __byte_perm(word, 0, 0x3232) + (kHalf ? 0x21002100u : 0u);
+}
+// total += scale * sum, two sums an instruction.
+__device__ __forceinline__ void AddScaled2(float& t0, float& t1, float scale, float s0, float s1) {
+  asm("{\n"
+      ".reg .b64 t, f, s;\n"
+      "mov.b64 t, {%0, %1};\n"
+      "mov.b64 f, {%2, %2};\n"
+      "mov.b64 s, {%3, %4};\n"
+      "fma.rn.f32x2 t, f, s, t;\n"
+      "mov.b64 {%0, %1}, t;\n"
+      "}\n"
+      : "+f"(t0), "+f"(t1)
+      : "f"(scale), "f"(s0), "f"(s1));
+}
 __device__ __forceinline__ float Scale(std::uint32_t word, bool bf16) {
   return bf16 ? __uint_as_float(word << 16) : HalfBitsToFloat(word & 0xffffu);
 }
@@ -174,6 +223,13 @@ template <int kGroups>
 struct StepWeights {
   uint4 a, b;                                // rows g and g + 8
   std::uint32_t word_a[kGroups], word_b[kGroups];
+  __device__ __forceinline__ void LoadShared(const std::uint8_t* block, int lane) {
+    a = *reinterpret_cast<const uint4*>(block + (lane * 16));
+    b = *reinterpret_cast<const uint4*>(block + 512 + (lane * 16));
+    const auto* words = reinterpret_cast<const std::uint32_t*>(block + 1024) + ((lane >> 2) * kGroups);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) word_a[i] = words[i], word_b[i] = words[(8 * kGroups) + i];
+  }
   __device__ __forceinline__ void Load(const std::uint8_t* block, int lane) {
     a = LoadStream16(block + (lane * 16));
     b = LoadStream16(block + 512 + (lane * 16));
@@ -192,44 +248,58 @@ struct StepWeights {
   }
 };
 
+// Copies that complete behind the thread's back, counted in groups.
+__device__ __forceinline__ void CopyAsync16(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<std::uint32_t>(__cvta_generic_to_shared(shared))), "l"(global)
+               : "memory");
+}
+__device__ __forceinline__ void CopyAsyncCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void CopyAsyncWait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
 // total += the step's products: column quads come from column(nt, i), the 16 bytes that hold
 // values 32 i + 8 t .. + 7 of the step for column lane / 4 of column tile nt.
-template <int kGroups, int kTiles, typename Column>
+template <bool kHalf, int kGroups, int kTiles, typename Column>
 __device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool bf16_scales, int tiles,
                                              float (&total)[kTiles][4], Column column) {
   const std::uint32_t wa[4] = {w.a.x, w.a.y, w.a.z, w.a.w}, wb[4] = {w.b.x, w.b.y, w.b.z, w.b.w};
   constexpr int kBlocks = 4 / kGroups;  // 32-value blocks a group
 #pragma unroll
   for (int group = 0; group < kGroups; ++group) {
-    const std::uint32_t za = Zero2(w.word_a[group]), zb = Zero2(w.word_b[group]);
+    const std::uint32_t za = Zero2<kHalf>(w.word_a[group]), zb = Zero2<kHalf>(w.word_b[group]);
     float sum[kTiles][4];
-#pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) sum[nt][0] = sum[nt][1] = sum[nt][2] = sum[nt][3] = 0.0f;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const int i = (group * kBlocks) + b;
       std::uint32_t pa[4], pb[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        pa[j] = Pair(wa[i], j, za);
-        pb[j] = Pair(wb[i], j, zb);
+        pa[j] = Pair<kHalf>(wa[i], j, za);
+        pb[j] = Pair<kHalf>(wb[i], j, zb);
       }
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
         if (nt == 0 || nt < tiles) {
           const uint4 x = column(nt, i);
-          Mma(sum[nt], pa[0], pb[0], pa[1], pb[1], x.x, x.y);
-          Mma(sum[nt], pa[2], pb[2], pa[3], pb[3], x.z, x.w);
+          if (b == 0) {
+            Mma<kHalf, true>(sum[nt], pa[0], pb[0], pa[1], pb[1], x.x, x.y);
+          } else {
+            Mma<kHalf, false>(sum[nt], pa[0], pb[0], pa[1], pb[1], x.x, x.y);
+          }
+          Mma<kHalf, false>(sum[nt], pa[2], pb[2], pa[3], pb[3], x.z, x.w);
         }
       }
     }
     const float sa = Scale(w.word_a[group], bf16_scales), sb = Scale(w.word_b[group], bf16_scales);
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
-      total[nt][0] = fmaf(sa, sum[nt][0], total[nt][0]);
-      total[nt][1] = fmaf(sa, sum[nt][1], total[nt][1]);
-      total[nt][2] = fmaf(sb, sum[nt][2], total[nt][2]);
-      total[nt][3] = fmaf(sb, sum[nt][3], total[nt][3]);
+      if (nt == 0 || nt < tiles) {
+        AddScaled2(total[nt][0], total[nt][1], sa, sum[nt][0], sum[nt][1]);
+        AddScaled2(total[nt][2], total[nt][3], sb, sum[nt][2], sum[nt][3]);
+      }
     }
   }
 }
