@@ -90,7 +90,7 @@ struct FirstShared {
 template <int kType, int kRouter, int kTiles>
 __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_t* staged, int first_expert, int tokens,
                                            int warp, int lane, double (&partial)[kTileRows][kMaxTokens]) {
-  constexpr int kPieces = Pieces(kType, true), kRouterPieces = Pieces(kRouter, true);
+  constexpr int kPieces = BfloatPieces(kType), kRouterPieces = BfloatPieces(kRouter);
   const int g = lane >> 2, t = lane & 3;
   const int piece = g % Cols(kPieces);
   const int tiles = (tokens + TokensATile(kPieces) - 1) / TokensATile(kPieces);
@@ -104,8 +104,8 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
   for (int b = warp * blocks / kWarps; b < (warp + 1) * blocks / kWarps; ++b) {
     uint4 qa[kRouterPieces], qb[kRouterPieces];
     const int at = (32 * b) + (8 * t);
-    LoadSplit8<kRouter, false, true>(base + (row_a * row_bytes), at, row_a < a.experts ? 8 : 0, a.router_vec, qa);
-    LoadSplit8<kRouter, false, true>(base + (row_b * row_bytes), at, row_b < a.experts ? 8 : 0, a.router_vec, qb);
+    LoadBfloat8<kRouter>(base + (row_a * row_bytes), at, row_a < a.experts ? 8 : 0, a.router_vec, qa);
+    LoadBfloat8<kRouter>(base + (row_b * row_bytes), at, row_b < a.experts ? 8 : 0, a.router_vec, qb);
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       if (nt >= tiles) break;
@@ -152,13 +152,13 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
 // Tokens token_of(0 .. count - 1) of x as pieces in shared memory.
 template <int kType, typename Token>
 __device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* staged, int count, Token token_of) {
-  constexpr int kPieces = Pieces(kType, true);
+  constexpr int kPieces = BfloatPieces(kType);
   const int padded = a.steps_up * kStep;
   for (int i = static_cast<int>(threadIdx.x); i < count * (padded / 8); i += kThreads) {
     const int c = i / (padded / 8), at = (i % (padded / 8)) * 8;
     uint4 quads[kPieces];
     const auto* row = static_cast<const std::uint8_t*>(a.x) + (token_of(c) * a.x_stride * TypeBytes(kType));
-    LoadSplit8<kType, true, true>(row, at, a.hidden - at, a.x_vec, quads);
+    LoadBfloat8<kType>(row, at, a.hidden - at, a.x_vec, quads);
 #pragma unroll
     for (int s = 0; s < kPieces; ++s) {
       *reinterpret_cast<uint4*>(staged + (((c * kPieces) + s) * a.x_pitch) + (at * 2)) = quads[s];
@@ -225,7 +225,7 @@ __device__ __forceinline__ void Choose(const LayerArgs& a, float* logits, int t,
 template <int kType, int kGroups>
 __global__ void __launch_bounds__(kThreads)
 FirstKernel(const LayerArgs a) {
-  constexpr int kPieces = Pieces(kType, true);
+  constexpr int kPieces = BfloatPieces(kType);
   constexpr int kTiles = kMaxTokens / TokensATile(kPieces);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
@@ -263,7 +263,7 @@ FirstKernel(const LayerArgs a) {
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += s.partial[w][row][c];
         for (int r = 0; r < kCluster; ++r) {
-          cluster.map_shared_rank(logits, r)[((first + c) * a.experts) + e] = static_cast<float>(sum * Up(kType));
+          cluster.map_shared_rank(logits, r)[((first + c) * a.experts) + e] = static_cast<float>(sum);
         }
       }
       __syncthreads();
@@ -376,7 +376,7 @@ FirstKernel(const LayerArgs a) {
     for (int nt = 0; nt < kTiles; ++nt) {
       if (nt >= tiles) break;
       float v[2][2];
-      FoldColumns<kPieces>(total[nt], v);
+      FoldColumns<false, kPieces>(total[nt], v);
 #pragma unroll
       for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
         const int c = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t4, j);
@@ -399,7 +399,7 @@ FirstKernel(const LayerArgs a) {
       }
       constexpr int kGlu = GluPieces(kType);
       std::uint32_t bits[kGlu];
-      Split<kGlu>(Glu(a.glu, gate * Up(kType), up * Up(kType), a.limit) * Down(kF32), bits);
+      Split<kGlu>(Glu(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
       unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[begin + c]) * kGlu * a.inter) + at;
 #pragma unroll
       for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);
@@ -459,7 +459,7 @@ SecondKernel(const LayerArgs a) {
     for (int nt = 0; nt < kTiles; ++nt) {
       if (nt >= tiles) break;
       float v[2][2];
-      FoldColumns<kGlu>(total[nt], v);
+      FoldColumns<false, kGlu>(total[nt], v);
       const int c = (nt * TokensATile(kGlu)) + TokenOf<kGlu>(t4, 0);
       if (c < count) {
         float* out = sums + (((__ldcg(&a.choice->pairs[begin + c]) * kParts) + part) * kTileRows);
@@ -475,7 +475,7 @@ SecondKernel(const LayerArgs a) {
     float y = 0.0f;
     for (int j = 0; j < a.used; ++j) {
       const float* p = sums + (((t * a.used) + j) * kParts * kTileRows) + r;
-      y = fmaf(__ldcg(&a.weights[(t * a.used) + j]), (p[0] + p[kTileRows]) * Up(kF32), y);
+      y = fmaf(__ldcg(&a.weights[(t * a.used) + j]), (p[0] + p[kTileRows]) * Up(false), y);
     }
     StoreValue(a.y, (t * a.y_stride) + row, a.y_type, y);
   }
@@ -499,7 +499,7 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   if (const cudaError_t e = Configure(FirstKernel<kType, kGroups>, configured_device, kFirstSmemLimit); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  const int smem = (a.cap * Pieces(kType, true) * a.x_pitch) + (a.tokens * a.experts * 4);
+  const int smem = (a.cap * BfloatPieces(kType) * a.x_pitch) + (a.tokens * a.experts * 4);
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
   const std::int64_t units = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) * a.tiles_up;
   const std::int64_t most = std::max<std::int64_t>(1, static_cast<std::int64_t>(SmCount()) * 2 / kCluster);
@@ -604,7 +604,7 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.choice = static_cast<Choice*>(d.scratch);
   a.h = reinterpret_cast<unsigned short*>(static_cast<std::uint8_t*>(d.scratch) + ChoiceBytes());
   a.x_pitch = (a.steps_up * kStep * 2) + 64;
-  a.cap = std::max(1, std::min(d.tokens, kXBudget / (Pieces(d.x_type, true) * a.x_pitch)));
+  a.cap = std::max(1, std::min(d.tokens, kXBudget / (BfloatPieces(d.x_type) * a.x_pitch)));
   const auto s = static_cast<cudaStream_t>(stream);
   if (d.x_type == kF32) return LaunchLayer<kF32>(d.gate_up.group, d.down.group, a, s);
   if (d.x_type == kF16) return LaunchLayer<kF16>(d.gate_up.group, d.down.group, a, s);

@@ -88,7 +88,7 @@ RelayoutKernel(const Source a, std::uint8_t* __restrict__ slab) {
       const int r = (tid - 64) / groups, gi = (tid - 64) % groups;
       const std::int64_t row = source_row(r);
       const int group = (step * groups) + gi;
-      std::uint32_t word = 0x43000000u;  // scale 0, zero 0
+      std::uint32_t word = 0xe4000000u;  // scale 0, zero 0
       if (row >= 0 && group < a.k / a.group) {
         const std::uint32_t scale = static_cast<const unsigned short*>(
             a.s.scales)[(expert * a.s.scale_expert) + (row * a.s.scale_row) + group];
@@ -97,7 +97,7 @@ RelayoutKernel(const Source a, std::uint8_t* __restrict__ slab) {
           zero = a.s.zeros[(expert * a.s.zero_expert) + (row * a.s.zero_row) + (group / 2)];
           zero = (group & 1) != 0 ? zero >> 4 : zero & 15u;
         }
-        word = scale | ((0x4300u + zero) << 16);  // 128 + zero, exact in bf16
+        word = scale | ((0xe400u + zero) << 16);  // -(1024 + zero), exact in f16
       }
       *reinterpret_cast<std::uint32_t*>(out + 1024 + ((tid - 64) * 4)) = word;
     }
@@ -127,144 +127,217 @@ __host__ __device__ constexpr int Pitch(int steps) { return (steps * kStep * 2) 
 
 // Persistent CTAs.  A round is a few tiles of 16 weight rows, each tile's steps divided among `parts`
 // warps, whose sums meet in shared memory: with one token a matrix of 4096 x 4096 is 8.7 MB in 256 tiles,
-// too few for a warp each.  The activations are staged (and split) once a CTA.  Weights come
+// too few for a warp each.  The activations are staged (scaled, split) once a CTA.  Weights come
 // through a ring of kSlots steps a warp (cp.async, its own lanes' copies: no CTA barrier, any depth of
-// requests without registers) that runs on from one round's tile to the next.  Where the activations
-// of all of k do not fit, the CTAs of a cluster divide k as well and read each other's sums.
+// requests without registers) that runs on from one round's tile to the next.  Warps of their own
+// add the parts up and store the results: those that multiply only arrive at the barrier and go on to the
+// next round's other buffer of sums.  Where the activations of all of k do not fit, the CTAs of a
+// cluster divide k as well and read each other's sums.
 constexpr int kSlots = 4;
 constexpr int kMaxWarps = 16;
+constexpr int kMaxRows = 16;
+__host__ __device__ constexpr int Reducers(int warps) { return warps > 8 ? 2 : 1; }
+
+__device__ __forceinline__ void BarrierSync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void BarrierArrive(int id, int threads) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
 
 template <int kTiles, int kType, int kGroups>
-__global__ void __launch_bounds__(kMaxWarps * 32, 1)
+__global__ void __launch_bounds__((kMaxWarps + 2) * 32, 1)  // 112 registers: two CTAs of nine warps an SM
 VectorKernel(const VectorArgs a) {
-  constexpr int kPieces = Pieces(kType);
+  constexpr int kPieces = HalfPieces(kType);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
+  __shared__ std::uint32_t magnitude[kMaxRows];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int clusters = static_cast<int>(gridDim.x) / ranks, first_round = static_cast<int>(blockIdx.x) / ranks;
-  const int threads = a.warps * 32;
-  const int lane = static_cast<int>(threadIdx.x) & 31, warp = static_cast<int>(threadIdx.x) >> 5;
+  const int threads = (a.warps + Reducers(a.warps)) * 32;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int step0 = a.steps * rank / ranks, steps = (a.steps * (rank + 1) / ranks) - step0;  // this CTA's
   const int tiles_a_round = a.warps / a.parts;
   const int my_tile = warp / a.parts, part = warp % a.parts;
   const int begin = steps * part / a.parts, count = (steps * (part + 1) / a.parts) - begin;  // this warp's
   const int pitch = Pitch(steps), columns = a.rows * kPieces;
+  const bool multiplies = warp < a.warps;
   std::uint8_t* ring = smem + (warp * kSlots * kBlock);
   float* meet = reinterpret_cast<float*>(smem + (a.warps * kSlots * kBlock));  // [2][warps][rows][16]
   std::uint8_t* staged = reinterpret_cast<std::uint8_t*>(meet + (2 * a.meet_floats));  // and a column of zeros
 
-  // the requests' place in this warp's sequence of steps: round after round
-  int load_round = first_round, load_step = 0;
+  // this warp's steps, round after round: where the next request reads
+  const int first_tile = (first_round * tiles_a_round) + my_tile;
+  const std::uint8_t* src =
+      a.slab + ((static_cast<std::size_t>(first_tile) * a.steps) + step0 + begin) * kBlock + (lane * 16);
+  const std::size_t to_next_round = ((static_cast<std::size_t>(clusters) * tiles_a_round * a.steps) - count) * kBlock;
+  const int rounds_mine = first_tile < a.tiles && multiplies
+                              ? ((a.tiles - 1 - first_tile) / (clusters * tiles_a_round)) + 1 : 0;
+  int left = rounds_mine * count, left_of_round = count;
   auto request = [&](int slot) {  // one commit a call, so that the waits can count
-    const int tile = (load_round * tiles_a_round) + my_tile;
-    if (load_round < a.rounds && tile < a.tiles && count > 0) {
-      const std::uint8_t* src =
-          a.slab + ((static_cast<std::size_t>(tile) * a.steps) + step0 + begin + load_step) * kBlock + (lane * 16);
+    if (left > 0) {
       std::uint8_t* dst = ring + (slot * kBlock) + (lane * 16);
       CopyAsync16(dst, src);
       CopyAsync16(dst + 512, src + 512);
       if (lane < 4 * kGroups) CopyAsync16(dst + 1024, src + 1024);
+      --left;
+      src += kBlock;
+      if (--left_of_round == 0) src += to_next_round, left_of_round = count;
     }
     CopyAsyncCommit();
-    if (++load_step >= count) load_step = 0, load_round += clusters;
   };
   GridLaunchDependents();
+  if (rounds_mine > 0) {  // into L2 only: what a kernel before may still write is not read yet
+    const std::size_t bytes = static_cast<std::size_t>(count) * kBlock;
+    for (std::size_t at = 0; at < bytes; at += 32 * 128) {
+      if (at + (lane * 128) < bytes) asm volatile("prefetch.global.L2 [%0];" ::"l"(src + at + (lane * 112)));
+    }
+  }
   GridDependencyWait();
 #pragma unroll
   for (int i = 0; i < kSlots - 1; ++i) request(i);
 
-  const int octets = steps * (kStep / 8);
-  for (int token = 0; token < a.rows; ++token) {
-    const auto* row = static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType));
-    for (int i = static_cast<int>(threadIdx.x); i < octets; i += threads) {
-      uint4 quads[kPieces];
-      const int at = (step0 * kStep) + (i * 8);
-      LoadSplit8<kType>(row, at, a.k - at, a.x_vec, quads);
-#pragma unroll
-      for (int s = 0; s < kPieces; ++s) {
-        *reinterpret_cast<uint4*>(staged + (((token * kPieces) + s) * pitch) + (i * 16)) = quads[s];
-      }
-    }
-  }
-  for (int i = static_cast<int>(threadIdx.x); i < octets; i += threads) {
+  const int octets = steps * (kStep / 8), x0 = step0 * kStep;
+  auto row_of = [&](int token) { return static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType)); };
+  for (int i = tid; i < octets; i += threads) {
     *reinterpret_cast<uint4*>(staged + (columns * pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
   }
-  // this lane's column of each column tile: the token and piece it stands for, or the zeros
-  const int piece = g % Cols(kPieces);
-  const std::uint8_t* column[kTiles];
-#pragma unroll
-  for (int nt = 0; nt < kTiles; ++nt) {
-    const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-    const int c = token < a.rows && piece < kPieces ? (token * kPieces) + piece : columns;
-    column[nt] = staged + (c * pitch) + (t * 16) + (begin * 256);
+  if constexpr (kType == kF32) {
+    if (tid < kMaxRows) magnitude[tid] = 0;
+    __syncthreads();
+    for (int token = 0; token < a.rows; ++token) {
+      std::uint32_t most = 0;
+      for (int i = tid; i < octets; i += threads) {
+        most = max(most, Magnitude8(row_of(token), x0 + (i * 8), a.k - x0 - (i * 8), a.x_vec));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0) atomicMax(&magnitude[token], most);
+    }
+    __syncthreads();
+    for (int token = 0; token < a.rows; ++token) {
+      const float scale = PowerOfTwo(ScaleExponent(magnitude[token]));
+      for (int i = tid; i < octets; i += threads) {
+        uint4 quads[2];
+        LoadHalf8(row_of(token), x0 + (i * 8), a.k - x0 - (i * 8), a.x_vec, scale, quads);
+        *reinterpret_cast<uint4*>(staged + ((token * 2) * pitch) + (i * 16)) = quads[0];
+        *reinterpret_cast<uint4*>(staged + (((token * 2) + 1) * pitch) + (i * 16)) = quads[1];
+      }
+    }
+  } else {
+    for (int token = 0; token < a.rows; ++token) {
+      for (int i = tid; i < octets; i += threads) {
+        Stage8(staged + (token * pitch) + (i * 16), row_of(token), x0 + (i * 8), a.k - x0 - (i * 8), a.x_vec);
+      }
+    }
+    CopyAsyncCommit();
+    CopyAsyncWait<0>();
   }
   __syncthreads();
 
-  int slot = 0, buffer = 0;
-  for (int round = first_round; round < a.rounds; round += clusters, buffer ^= 1) {
-    const bool live = (round * tiles_a_round) + my_tile < a.tiles;
-    float total[kTiles][4];
-#pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
-    for (int step = 0; step < count; ++step) {
-      CopyAsyncWait<kSlots - 2>();
-      __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
-      request(slot == 0 ? kSlots - 1 : slot - 1);
-      if (live) {
-        StepWeights<kGroups> w;
-        w.LoadShared(ring + (slot * kBlock), lane);
-        MultiplyStep<kType == kF16, kGroups, kTiles>(w, a.bf16_scales, kTiles, total, [&](int nt, int i) {
-          return *reinterpret_cast<const uint4*>(column[nt] + (step * 256) + (i * 64));
-        });
-      }
-      slot = slot == kSlots - 1 ? 0 : slot + 1;
-    }
-    float* mine = meet + (buffer * a.meet_floats) + (warp * kTileRows * a.rows);
+  // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
+  if (multiplies) {
+    // this lane's column of each column tile: the token and piece it stands for, or the zeros
+    const int piece = g % Cols(kPieces);
+    const std::uint8_t* column[kTiles];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
-      float v[2][2];
-      FoldColumns<kPieces>(total[nt], v);
-#pragma unroll
-      for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
-        const int token = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t, j);
-        if (token < a.rows && (kPieces != 3 || (t & 1) == 0)) {
-          mine[(token * kTileRows) + g] = v[0][j];
-          mine[(token * kTileRows) + g + 8] = v[1][j];
-        }
-      }
+      const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
+      column[nt] = staged + ((token < a.rows ? (token * kPieces) + piece : columns) * pitch) + (t * 16) + (begin * 256);
     }
-    // two buffers: who writes one again has passed the barrier behind its last readers
-    if (ranks > 1) cluster.sync(); else __syncthreads();
-    const int height = a.glu != LLMP_B200_GLU_NONE ? 8 : 16;
-    const int outputs = tiles_a_round * a.rows * height;
-    for (int i = (rank * threads) + static_cast<int>(threadIdx.x); i < outputs; i += threads * ranks) {
-      const int r = i % height, token = (i / height) % a.rows, o = (i / height) / a.rows;
-      const int tile = (round * tiles_a_round) + o, row = (tile * height) + r;
-      if (tile >= a.tiles || row >= a.outputs) continue;
-      const int at = (buffer * a.meet_floats) + (((o * a.parts * a.rows) + token) * kTileRows) + r;
-      float first = 0.0f, second = 0.0f;
-      for (int q = 0; q < ranks; ++q) {
-        const float* p = (ranks > 1 ? cluster.map_shared_rank(meet, q) : meet) + at;
-        for (int s = 0; s < a.parts; ++s) {
-          first += p[s * kTileRows * a.rows];
-          if (height == 8) second += p[(s * kTileRows * a.rows) + 8];
+    int slot = 0, buffer = 0;
+    for (int round = first_round, n = 0; round < a.rounds; round += clusters, buffer ^= 1, ++n) {
+      float total[kTiles][4];
+#pragma unroll
+      for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
+      if (n < rounds_mine) {
+        for (int step = 0; step < count; ++step) {
+          CopyAsyncWait<kSlots - 2>();
+          __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
+          request(slot == 0 ? kSlots - 1 : slot - 1);
+          StepWeights<kGroups> w;
+          w.LoadShared(ring + (slot * kBlock), lane);
+          MultiplyStep<kType != kBF16, kGroups, kTiles>(w, a.bf16_scales, kTiles, total, [&](int nt, int i) {
+            return *reinterpret_cast<const uint4*>(column[nt] + (step * 256) + (i * 64));
+          });
+          slot = slot == kSlots - 1 ? 0 : slot + 1;
         }
       }
-      const float v = height == 8 ? Glu(a.glu, first * Up(kType), second * Up(kType), a.limit) : first * Up(kType);
-      StoreValue(a.y, (token * a.y_stride) + row, a.y_type, v);
+      if (ranks == 1 && n >= 2) BarrierSync(3 + buffer, threads);
+      float* mine = meet + (buffer * a.meet_floats) + (warp * kTileRows * a.rows);
+#pragma unroll
+      for (int nt = 0; nt < kTiles; ++nt) {
+        float v[2][2];
+        FoldColumns<kType != kBF16, kPieces>(total[nt], v);
+#pragma unroll
+        for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
+          const int token = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t, j);
+          if (token < a.rows) {
+            mine[(token * kTileRows) + g] = v[0][j];
+            mine[(token * kTileRows) + g + 8] = v[1][j];
+          }
+        }
+      }
+      // of a cluster all threads meet: no buffer is written again before every rank has met once more
+      if (ranks > 1) cluster.sync(); else BarrierArrive(1 + buffer, threads);
+    }
+  } else {
+    // a lane adds up four rows (with a GLU: of gate and of up) of a token, a tile's tokens side by side
+    const bool glu = a.glu != LLMP_B200_GLU_NONE;
+    const int quad = glu ? (lane & 1) * 4 : (lane & 3) * 4;
+    const int lane_token = glu ? lane >> 1 : lane >> 2, tokens_a_pass = glu ? 16 : 8;
+    int buffer = 0;
+    for (int round = first_round; round < a.rounds; round += clusters, buffer ^= 1) {
+      if (ranks > 1) cluster.sync(); else BarrierSync(1 + buffer, threads);
+      for (int o = rank; o < tiles_a_round; o += ranks) {
+        const int tile = (round * tiles_a_round) + o;
+        if (tile >= a.tiles) break;
+        for (int token = ((warp - a.warps) * tokens_a_pass) + lane_token; token < a.rows;
+             token += Reducers(a.warps) * tokens_a_pass) {
+          float first[4] = {0.0f, 0.0f, 0.0f, 0.0f}, second[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int q = 0; q < ranks; ++q) {
+            const float* p = (ranks > 1 ? cluster.map_shared_rank(meet, q) : meet) + (buffer * a.meet_floats) +
+                             (((o * a.parts * a.rows) + token) * kTileRows) + quad;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f), sum2 = sum;
+#pragma unroll 4
+            for (int s = 0; s < a.parts; ++s, p += kTileRows * a.rows) {
+              const float4 v = *reinterpret_cast<const float4*>(p);
+              sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+              if (glu) {
+                const float4 u = *reinterpret_cast<const float4*>(p + 8);
+                sum2.x += u.x, sum2.y += u.y, sum2.z += u.z, sum2.w += u.w;
+              }
+            }
+            float up = Up(kType != kBF16);  // (each rank's F32 activations have their own scale)
+            if constexpr (kType == kF32) {
+              up = PowerOfTwo(-ScaleExponent(ranks > 1 ? *cluster.map_shared_rank(&magnitude[token], q) : magnitude[token]));
+            }
+            first[0] = fmaf(sum.x, up, first[0]), first[1] = fmaf(sum.y, up, first[1]);
+            first[2] = fmaf(sum.z, up, first[2]), first[3] = fmaf(sum.w, up, first[3]);
+            second[0] = fmaf(sum2.x, up, second[0]), second[1] = fmaf(sum2.y, up, second[1]);
+            second[2] = fmaf(sum2.z, up, second[2]), second[3] = fmaf(sum2.w, up, second[3]);
+          }
+          const int row = (tile * (glu ? 8 : 16)) + quad;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (row + r >= a.outputs) break;
+            StoreValue(a.y, (token * a.y_stride) + row + r, a.y_type, glu ? Glu(a.glu, first[r], second[r], a.limit) : first[r]);
+          }
+        }
+      }
+      if (ranks == 1) BarrierArrive(3 + buffer, threads);
     }
   }
   if (ranks > 1) cluster.sync();  // nobody leaves while another reads its sums
 }
 
-constexpr int kSmemLimit = 224 * 1024;
+constexpr int kSmemLimit = 226 * 1024;
 constexpr int kMaxRanks = 8;
 // Shared memory of a CTA: rings, two buffers of sums, the staged activations.
 std::int64_t SmemBytes(int warps, int ranks, int rows, int steps, int type, int block_bytes) {
   return (static_cast<std::int64_t>(warps) * kSlots * block_bytes) + (2 * warps * kTileRows * rows * 4) +
-         (((rows * Pieces(type)) + 1) * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
+         (((rows * HalfPieces(type)) + 1) * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
 }
 
 template <int kTiles, int kType, int kGroups>
@@ -281,13 +354,15 @@ int LaunchVector(VectorArgs a, cudaStream_t stream) {
   auto bytes = [&](int warps, int ranks) {
     return SmemBytes(warps, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
   };
-  // two CTAs of eight warps an SM where the staged activations allow it, else one of sixteen, else as few ranks as
-  // their memory needs
-  int ranks = 1, per_sm = 2;
-  a.warps = 8;
-  if (bytes(8, 1) > 112 * 1024) {
-    a.warps = 16, per_sm = 1;
-    while (ranks < kMaxRanks && bytes(16, ranks) > kSmemLimit) ranks *= 2;
+  // two CTAs of eight warps an SM where the staged activations allow it, else one of sixteen, of eight, else as few
+  // ranks as their memory needs
+  int ranks = 1, per_sm = 1;
+  if (a.warps = 8; bytes(8, 1) <= 112 * 1024) {
+    per_sm = 2;
+  } else if (a.warps = 16; bytes(16, 1) > kSmemLimit) {
+    a.warps = 8;
+    while (ranks < kMaxRanks && bytes(8, ranks) > kSmemLimit) ranks *= 2;
+    if (bytes(16, ranks) <= kSmemLimit) a.warps = 16;
   }
   const int ctas = std::max(1, SmCount() * per_sm / ranks);
   a.parts = a.warps;
@@ -296,7 +371,7 @@ int LaunchVector(VectorArgs a, cudaStream_t stream) {
   a.meet_floats = a.warps * kTileRows * a.rows;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(std::min(a.rounds, ctas) * ranks));
-  config.blockDim = dim3(static_cast<unsigned>(a.warps * 32));
+  config.blockDim = dim3(static_cast<unsigned>((a.warps + Reducers(a.warps)) * 32));
   config.dynamicSmemBytes = static_cast<std::size_t>(bytes(a.warps, ranks));
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
@@ -320,13 +395,10 @@ int LaunchGroups(int group, const VectorArgs& a, cudaStream_t stream) {
 
 template <int kType>
 int LaunchTiles(int group, const VectorArgs& a, cudaStream_t stream) {
-  constexpr int kTokens = TokensATile(Pieces(kType));
+  constexpr int kTokens = TokensATile(HalfPieces(kType));
   if (a.rows <= kTokens) return LaunchGroups<1, kType>(group, a, stream);
   if (a.rows <= 2 * kTokens) return LaunchGroups<2, kType>(group, a, stream);
-  if constexpr (kTokens <= 4) {
-    if (a.rows <= 4 * kTokens) return LaunchGroups<4, kType>(group, a, stream);
-  }
-  if constexpr (kTokens <= 2) return LaunchGroups<8, kType>(group, a, stream);
+  if constexpr (kTokens <= 4) return LaunchGroups<4, kType>(group, a, stream);
   return Reject("w4_vector: too many rows");
 }
 
@@ -405,7 +477,7 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream) {
   // as many rows a launch as a cluster's shared memory takes: all of them but for very long ones
   const int block_bytes = w4::BlockBytes(p.w.group);
   int most = p.rows;
-  while (most > 1 && w4::SmemBytes(16, w4::kMaxRanks, most, a.steps, p.x_type, block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
+  while (most > 1 && w4::SmemBytes(8, w4::kMaxRanks, most, a.steps, p.x_type, block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
   for (int first = 0; first < p.rows; first += most) {
     a.rows = std::min(most, p.rows - first);
     a.x = static_cast<const std::uint8_t*>(p.x) + (first * p.x_stride * xb);

@@ -7,23 +7,23 @@
 //   [2][32 lanes][16 bytes]  codes: lane (g, t) = (lane / 4, lane % 4) holds row g's and row g + 8's
 //                            values 32 i + 8 t .. + 7 of the step in word i = 0..3, the even values'
 //                            nibbles in the low half and the odd ones' in the high half
-//   [16 rows][128 / group]   words: the scale's 16 bits, and above them 128 + zero as a bf16
+//   [16 rows][128 / group]   words: the scale's 16 bits, and above them -(1024 + zero) as an f16
 //
-// so a warp reads a step with two 16-byte loads a lane and one load of its rows' words, and word
-// i >> 4 j & 0x000f000f is a pair of neighbouring codes.  Or'ed with 0x4300 (128 in bf16, whose
-// last four mantissa bits then are the code) and less 128 + zero they are two exact bf16 values:
+// so a warp reads a step with two 16-byte copies a lane and a few of its rows' words.  Codes multiply
+// as exact small integers: word & 0x000f000f, or'ed with 0x6400 (1024 in f16, whose last four mantissa
+// bits then are the code), plus -(1024 + zero), is a pair of neighbouring values in one addition;
+// & 0x00f000f0 the same way is 1024 + 16 code, a pair in one multiply-add; a shift by 8 serves the other
+// two.  In bf16, 0x4300 is 128, every pair needs its shift, and the multiply-add takes 2^-11 into the pair.  They are
 // the A fragment of mma.sync.m16n8k16, whose k order is free as long as B's is the same.  With a
 // GLU a tile's rows 0..7 are gate rows and 8..15 the same rows of up, so a lane's sums hold both.
 //
-// A group's sum comes before its scale: up to 15 * 128 times the activations, which enter 2^-11
-// smaller where their type reaches F32's range (exact down to 2^-98) and whose results leave 2^11 larger, so
-// that nothing overflows that the scaled product would not.
-//
-// The tokens are the MMA's 8 columns.  A product is exact (code - zero has 5 bits, a bf16 column
-// 8, an f16 one 11), sums are F32, and the scale multiplies a group's F32 sum, so nothing is
-// rounded to fewer bits.  BF16 and F16 activations are columns as they are, with the codes in the same
-// type (0x6400 is 1024 in f16); an F32 one is split into 3 bf16 columns whose sum it is, exactly
-// (24 significant bits in pieces of 8).  A token takes 1, 2 or 4 columns (one of the 4 is zero).
+// The tokens are the MMA's 8 columns.  Sums are F32 and the scale multiplies a group's F32 sum: nothing of
+// the weights is rounded.  BF16 and F16 activations multiply as they are, in their own type; a group's sum
+// comes before its scale and may be 15 * 128 times an activation, hence bf16's 2^-11 (taken back in
+// the result): it overflows only where the scaled product would.  F32 activations are two f16
+// pieces of the value times a power of two a row, which brings the row's largest finite value to 2^14..2^15: the second
+// piece 2^11 larger, the two within a unit of the value's last bit, and exact bf16 pieces (3, without
+// a scale) where values must not lose that.
 #ifndef LLMP_B200_CSRC_W4_CUH_
 #define LLMP_B200_CSRC_W4_CUH_
 
@@ -48,14 +48,12 @@ __host__ __device__ constexpr int Tiles(int n, int glu) {
 constexpr int kF32 = LLMP_B200_TYPE_F32, kF16 = LLMP_B200_TYPE_F16, kBF16 = LLMP_B200_TYPE_BF16;
 inline bool FloatType(int t) { return t == kF32 || t == kF16 || t == kBF16; }
 __host__ __device__ constexpr int TypeBytes(int t) { return t == kF32 ? 4 : 2; }
-// The columns that a value of the type is the sum of: itself, or bf16 pieces (bf16_only: f16 in pieces too).
-__host__ __device__ constexpr int Pieces(int t, bool bf16_only = false) {
-  return t == kF32 ? 3 : t == kF16 && bf16_only ? 2 : 1;
-}
+// The f16 pieces, and the bf16 pieces, that a value of the type is the sum of.
+__host__ __device__ constexpr int HalfPieces(int t) { return t == kF32 ? 2 : 1; }
+__host__ __device__ constexpr int BfloatPieces(int t) { return t == kF32 ? 3 : t == kF16 ? 2 : 1; }
 
-// Activations enter this much smaller, results leave this much larger.
-__host__ __device__ constexpr float Down(int t) { return t == kF16 ? 1.0f : 0x1p-11f; }
-__host__ __device__ constexpr float Up(int t) { return t == kF16 ? 1.0f : 0x1p+11f; }
+// A product in bf16 leaves this much larger.
+__host__ __device__ constexpr float Up(bool half) { return half ? 1.0f : 0x1p+11f; }
 
 // Shape and alignment of a matrix whose slab a product reads: 0 or a refusal.
 int CheckMatrix(const llmp_b200_w4_matrix& m, const char* what);
@@ -93,64 +91,85 @@ __device__ __forceinline__ void Split(float x, std::uint32_t (&bits)[kPieces]) {
   }
 }
 
-// Eight consecutive values (zero from `valid` on) times Down as pieces, a 16-byte quad a piece.
-template <int kType, bool kDown = true, bool kBf16Only = false>
-__device__ __forceinline__ void LoadSplit8(const void* row, std::int64_t at, int valid, bool vec,
-                                           uint4 (&quads)[Pieces(kType, kBf16Only)]) {
-  constexpr int kPieces = Pieces(kType, kBf16Only);
-  if constexpr (kPieces > 1) {
-    float v[8];
-    if (vec && valid >= 8) {
-      if constexpr (kType == kF32) {
-        const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
-        const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
-        const std::uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = HalfBitsToFloat(w[i] & 0xffffu);
-          v[(2 * i) + 1] = HalfBitsToFloat(w[i] >> 16);
-        }
-      }
+// Eight consecutive values (zero from `valid` on).
+template <int kType>
+__device__ __forceinline__ void Load8(const void* row, std::int64_t at, int valid, bool vec, float (&v)[8]) {
+  if (vec && valid >= 8) {
+    if constexpr (kType == kF32) {
+      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at);
+      const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(row) + at + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < valid ? LoadValue(row, at + i, kType) : 0.0f;
-    }
-    std::uint32_t packed[kPieces][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      std::uint32_t lo[kPieces], hi[kPieces];
-      Split<kPieces>(kDown && kType == kF32 ? v[2 * i] * Down(kType) : v[2 * i], lo);
-      Split<kPieces>(kDown && kType == kF32 ? v[(2 * i) + 1] * Down(kType) : v[(2 * i) + 1], hi);
-#pragma unroll
-      for (int s = 0; s < kPieces; ++s) packed[s][i] = lo[s] | (hi[s] << 16);
-    }
-#pragma unroll
-    for (int s = 0; s < kPieces; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
-  } else {
-    uint4 q;
-    if (vec && valid >= 8) {
-      q = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
-    } else {
-      std::uint32_t w[4];
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const unsigned short*>(row) + at);
+      const std::uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const auto* p = static_cast<const unsigned short*>(row) + at + (2 * i);
-        w[i] = (2 * i) < valid ? p[0] : 0u;
-        if ((2 * i) + 1 < valid) w[i] |= static_cast<std::uint32_t>(p[1]) << 16;
+        if constexpr (kType == kF16) {
+          v[2 * i] = HalfBitsToFloat(w[i] & 0xffffu);
+          v[(2 * i) + 1] = HalfBitsToFloat(w[i] >> 16);
+        } else {
+          v[2 * i] = __uint_as_float(w[i] << 16);
+          v[(2 * i) + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
       }
-      q = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    if constexpr (kDown && kType == kBF16) {
-      auto* pairs = reinterpret_cast<__nv_bfloat162*>(&q);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pairs[i] = __hmul2(pairs[i], __float2bfloat162_rn(Down(kType)));
-    }
-    quads[0] = q;
+    for (int i = 0; i < 8; ++i) v[i] = i < valid ? LoadValue(row, at + i, kType) : 0.0f;
   }
 }
+// ... as bf16 pieces, a 16-byte quad a piece.
+template <int kType>
+__device__ __forceinline__ void LoadBfloat8(const void* row, std::int64_t at, int valid, bool vec,
+                                            uint4 (&quads)[BfloatPieces(kType)]) {
+  constexpr int kPieces = BfloatPieces(kType);
+  float v[8];
+  Load8<kType>(row, at, valid, vec, v);
+  std::uint32_t packed[kPieces][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    std::uint32_t lo[kPieces], hi[kPieces];
+    Split<kPieces>(v[2 * i], lo);
+    Split<kPieces>(v[(2 * i) + 1], hi);
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) packed[s][i] = lo[s] | (hi[s] << 16);
+  }
+#pragma unroll
+  for (int s = 0; s < kPieces; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
+}
+// Eight F32 values times `scale` as two f16 pieces.
+__device__ __forceinline__ void LoadHalf8(const void* row, std::int64_t at, int valid, bool vec, float scale, uint4 (&quads)[2]) {
+  float v[8];
+  Load8<kF32>(row, at, valid, vec, v);
+  std::uint32_t packed[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = v[2 * i] * scale, b = v[(2 * i) + 1] * scale;
+    const __half2 first = __floats2half2_rn(a, b);
+    packed[0][i] = *reinterpret_cast<const std::uint32_t*>(&first);
+    const float2 f = __half22float2(first);  // the remainders are exact; of an infinity there is none
+    const __half2 second = __floats2half2_rn(isinf(f.x) ? 0.0f : (a - f.x) * 2048.0f, isinf(f.y) ? 0.0f : (b - f.y) * 2048.0f);
+    packed[1][i] = *reinterpret_cast<const std::uint32_t*>(&second);
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
+}
+// The largest finite magnitude's bits among eight F32 values, and the power of two that brings it to 2^14..2^15.
+__device__ __forceinline__ std::uint32_t Magnitude8(const void* row, std::int64_t at, int valid, bool vec) {
+  float v[8];
+  Load8<kF32>(row, at, valid, vec, v);
+  std::uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const std::uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    if (b < 0x7f800000u) most = max(most, b);
+  }
+  return most;
+}
+__device__ __forceinline__ int ScaleExponent(std::uint32_t magnitude) {
+  return min(126, 141 - static_cast<int>(magnitude >> 23));  // 14 - (exponent - 127); at least 14 - 127
+}
+__device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<std::uint32_t>(e + 127) << 23); }
 
 // Columns a token takes, tokens an MMA's 8 columns hold.
 __host__ __device__ constexpr int Cols(int pieces) { return pieces == 3 ? 4 : pieces; }
@@ -183,24 +202,74 @@ __device__ __forceinline__ void Mma(float (&c)[4], std::uint32_t a0, std::uint32
   }
 }
 
-// Two codes at bits 0 and 16 of w >> 4 j as values of the MMA's type, less 128 (f16: 1024) + zero twice.
+// The zero points of a row's group as the pairs take them.
 template <bool kHalf>
-__device__ __forceinline__ std::uint32_t Pair(std::uint32_t w, int j, std::uint32_t zero2) {
-  const std::uint32_t biased = ((w >> (4 * j)) & 0x000f000fu) | (kHalf ? 0x64006400u : 0x43004300u);
+struct Zeros {
+  std::uint32_t near, far;  // f16: -(1024 + zero), -(64 + zero); bf16: -2^-11 (128 + zero), unused
+  __device__ __forceinline__ explicit Zeros(std::uint32_t word) {
+    near = __byte_perm(word, 0, 0x3232);
+    if constexpr (kHalf) {
+      const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&near), __floats2half2_rn(960.0f, 960.0f));
+      far = *reinterpret_cast<const std::uint32_t*>(&v);
+    } else {
+      near -= 0x26802680u;  // 0xe400 + zero to 0xbd80 + zero
+      far = 0;
+    }
+  }
+};
+// A word's codes less the zero point: pairs[j] holds values 2 j and 2 j + 1.
+template <bool kHalf>
+__device__ __forceinline__ void Pairs(std::uint32_t w, const Zeros<kHalf>& z, std::uint32_t (&pairs)[4]) {
   if constexpr (kHalf) {
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&zero2));
-    return *reinterpret_cast<const std::uint32_t*>(&v);
+    const __half2 near = *reinterpret_cast<const __half2*>(&z.near), far = *reinterpret_cast<const __half2*>(&z.far);
+    const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+#pragma unroll
+    for (int j = 0; j < 4; j += 2, w >>= 8) {
+      const std::uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
+      const __half2 va = __hadd2(*reinterpret_cast<const __half2*>(&a), near);
+      const __half2 vb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, far);
+      pairs[j] = *reinterpret_cast<const std::uint32_t*>(&va);
+      pairs[j + 1] = *reinterpret_cast<const std::uint32_t*>(&vb);
+    }
   } else {
-    const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&zero2));
-    return *reinterpret_cast<const std::uint32_t*>(&v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const std::uint32_t a = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+      const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), __float2bfloat162_rn(0x1p-11f),
+                                       *reinterpret_cast<const __nv_bfloat162*>(&z.near));
+      pairs[j] = *reinterpret_cast<const std::uint32_t*>(&v);
+    }
   }
 }
-// A word's 128 + zero twice; the same last bits after 1024's exponent are 1024 + zero in f16.
-template <bool kHalf>
-__device__ __forceinline__ std::uint32_t Zero2(std::uint32_t word) {
-  return __byte_perm(word, 0, 0x3232) + (kHalf ? 0x21002100u : 0u);
+// Copies that complete behind the thread's back, counted in groups.
+__device__ __forceinline__ void CopyAsync16(void* shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<std::uint32_t>(__cvta_generic_to_shared(shared))), "l"(global)
+               : "memory");
 }
+__device__ __forceinline__ void CopyAsyncCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void CopyAsyncWait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// Eight 16-bit values as they are (zero from `valid` on) into shared memory: in the thread's open group of copies
+// where they may be copied 16 bytes at a time.
+__device__ __forceinline__ void Stage8(void* shared, const void* row, std::int64_t at, int valid, bool vec) {
+  const auto* p = static_cast<const unsigned short*>(row) + at;
+  if (vec && valid >= 8) {
+    CopyAsync16(shared, p);
+    return;
+  }
+  std::uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = (2 * i) < valid ? p[2 * i] : 0u;
+    if ((2 * i) + 1 < valid) w[i] |= static_cast<std::uint32_t>(p[(2 * i) + 1]) << 16;
+  }
+  *reinterpret_cast<uint4*>(shared) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // total += scale * sum, two sums an instruction.
 __device__ __forceinline__ void AddScaled2(float& t0, float& t1, float scale, float s0, float s1) {
   asm("{\n"
@@ -248,18 +317,6 @@ struct StepWeights {
   }
 };
 
-// Copies that complete behind the thread's back, counted in groups.
-__device__ __forceinline__ void CopyAsync16(void* shared, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                   static_cast<std::uint32_t>(__cvta_generic_to_shared(shared))), "l"(global)
-               : "memory");
-}
-__device__ __forceinline__ void CopyAsyncCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void CopyAsyncWait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
-}
-
 // total += the step's products: column quads come from column(nt, i), the 16 bytes that hold
 // values 32 i + 8 t .. + 7 of the step for column lane / 4 of column tile nt.
 template <bool kHalf, int kGroups, int kTiles, typename Column>
@@ -269,17 +326,14 @@ __device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool
   constexpr int kBlocks = 4 / kGroups;  // 32-value blocks a group
 #pragma unroll
   for (int group = 0; group < kGroups; ++group) {
-    const std::uint32_t za = Zero2<kHalf>(w.word_a[group]), zb = Zero2<kHalf>(w.word_b[group]);
+    const Zeros<kHalf> za(w.word_a[group]), zb(w.word_b[group]);
     float sum[kTiles][4];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
       const int i = (group * kBlocks) + b;
       std::uint32_t pa[4], pb[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        pa[j] = Pair<kHalf>(wa[i], j, za);
-        pb[j] = Pair<kHalf>(wb[i], j, zb);
-      }
+      Pairs<kHalf>(wa[i], za, pa);
+      Pairs<kHalf>(wb[i], zb, pb);
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
         if (nt == 0 || nt < tiles) {
@@ -305,14 +359,15 @@ __device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool
 }
 
 // A lane's sums of one column tile with a token's columns added up: values[r][j] is row g + 8 r,
-// token TokenOf(j); with 2 or 3 pieces only j = 0 counts.
-template <int kPieces>
+// token TokenOf(j); with 2 or 3 pieces only j = 0 counts.  An f16 value's second piece is 2^11 larger.
+template <bool kHalf, int kPieces>
 __device__ __forceinline__ void FoldColumns(const float (&total)[4], float (&values)[2][2]) {
   if constexpr (kPieces == 1) {
     values[0][0] = total[0], values[0][1] = total[1], values[1][0] = total[2], values[1][1] = total[3];
   } else {
-    values[0][0] = total[0] + total[1];
-    values[1][0] = total[2] + total[3];
+    constexpr float kSecond = kHalf ? 0x1p-11f : 1.0f;
+    values[0][0] = fmaf(total[1], kSecond, total[0]);
+    values[1][0] = fmaf(total[3], kSecond, total[2]);
     values[0][1] = values[1][1] = 0.0f;
     if constexpr (kPieces == 3) {  // columns 0, 1 in an even lane, 2 (and a zero) in the next
 #pragma unroll
