@@ -49,7 +49,6 @@ struct LayerArgs {
   const std::uint8_t* down;
   int experts, used, tokens, hidden, inter;
   int tiles_up, steps_up, tiles_down, steps_down;
-  bool bf16_up, bf16_down;
   int glu;
   float limit;
   void* y;
@@ -358,15 +357,13 @@ FirstKernel(const LayerArgs a) {
       }
     }
     const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
-    float total[kTiles][4];
-#pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
+    Sums total[kTiles];
     const std::uint8_t* block =
         a.gate_up + ((((static_cast<std::size_t>(e) * a.tiles_up) + tile) * a.steps_up) + step0) * kBlock;
     for (int step = step0; step < step1; ++step, block += kBlock) {
       StepWeights<kGroups> w;
       w.Load(block, lane);
-      MultiplyStep<false, kGroups, kTiles>(w, a.bf16_up, tiles, total, [&](int nt, int i) {
+      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int i) {
         if (column_at[nt] == 0xffffffffu) return make_uint4(0, 0, 0, 0);
         return *reinterpret_cast<const uint4*>(staged + column_at[nt] + (step * 256) + (i * 64));
       });
@@ -441,15 +438,13 @@ SecondKernel(const LayerArgs a) {
       }
     }
     const int tiles = (count + TokensATile(kGlu) - 1) / TokensATile(kGlu);
-    float total[kTiles][4];
-#pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
+    Sums total[kTiles];
     const std::uint8_t* block =
         a.down + ((((static_cast<std::size_t>(e) * a.tiles_down) + tile) * a.steps_down) + step0) * kBlock;
     for (int step = step0; step < step1; ++step, block += kBlock) {
       StepWeights<kGroups> w;
       w.Load(block, lane);
-      MultiplyStep<false, kGroups, kTiles>(w, a.bf16_down, tiles, total, [&](int nt, int b) {
+      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int b) {
         const int at = (step * kStep) + (32 * b);  // inter is whole 32-value blocks
         if (column[nt] == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
         return __ldcg(reinterpret_cast<const uint4*>(column[nt] + at));
@@ -597,7 +592,6 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.experts = experts, a.used = d.used, a.tokens = d.tokens, a.hidden = hidden, a.inter = inter;
   a.tiles_up = Tiles(d.gate_up.n, 1), a.steps_up = Steps(hidden);
   a.tiles_down = Tiles(d.down.n, 0), a.steps_down = Steps(inter);
-  a.bf16_up = d.gate_up.scale_type == kBF16, a.bf16_down = d.down.scale_type == kBF16;
   a.glu = d.glu, a.limit = d.limit;
   a.y = d.y, a.y_stride = d.y_stride, a.y_type = d.y_type;
   a.ids = d.ids, a.weights = d.weights;

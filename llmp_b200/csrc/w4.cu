@@ -31,6 +31,7 @@ namespace cg = cooperative_groups;
 struct Source {
   llmp_b200_w4_source s;
   int n, k, group, glu, tiles, steps, block_bytes;
+  bool bf16;   // the scales' type
   bool words;  // codes may be read as 32-bit words
   std::int64_t blocks;
 };
@@ -88,7 +89,7 @@ RelayoutKernel(const Source a, std::uint8_t* __restrict__ slab) {
       const int r = (tid - 64) / groups, gi = (tid - 64) % groups;
       const std::int64_t row = source_row(r);
       const int group = (step * groups) + gi;
-      std::uint32_t word = 0xe4000000u;  // scale 0, zero 0
+      std::uint32_t word = 0;
       if (row >= 0 && group < a.k / a.group) {
         const std::uint32_t scale = static_cast<const unsigned short*>(
             a.s.scales)[(expert * a.s.scale_expert) + (row * a.s.scale_row) + group];
@@ -97,7 +98,9 @@ RelayoutKernel(const Source a, std::uint8_t* __restrict__ slab) {
           zero = a.s.zeros[(expert * a.s.zero_expert) + (row * a.s.zero_row) + (group / 2)];
           zero = (group & 1) != 0 ? zero >> 4 : zero & 15u;
         }
-        word = scale | ((0xe400u + zero) << 16);  // -(1024 + zero), exact in f16
+        // exact in F32, with at least 13 last bits of zero (but for a NaN's)
+        word = a.bf16 ? scale << 16 : __float_as_uint(HalfBitsToFloat(scale));
+        word = (word & 0xffffff00u) | zero;
       }
       *reinterpret_cast<std::uint32_t*>(out + 1024 + ((tid - 64) * 4)) = word;
     }
@@ -107,16 +110,16 @@ RelayoutKernel(const Source a, std::uint8_t* __restrict__ slab) {
 struct VectorArgs {
   const std::uint8_t* slab;
   int tiles, steps, k, outputs, rows;
-  int warps, parts;   // warps a CTA; of them `parts` divide a tile's steps
-  int rounds;         // of warps / parts tiles
+  int parts;          // warps that divide a tile's steps
+  int rounds;         // of warps / parts tiles each
   int meet_floats;    // one buffer of partial sums
+  bool zero_column;
   const void* x;
   std::int64_t x_stride;
   bool x_vec;
   void* y;
   std::int64_t y_stride;
   int y_type;
-  bool bf16_scales;
   int glu;
   float limit;
 };
@@ -133,10 +136,12 @@ __host__ __device__ constexpr int Pitch(int steps) { return (steps * kStep * 2) 
 // add the parts up and store the results: those that multiply only arrive at the barrier and go on to the
 // next round's other buffer of sums.  Where the activations of all of k do not fit, the CTAs of a
 // cluster divide k as well and read each other's sums.
-constexpr int kSlots = 4;
-constexpr int kMaxWarps = 16;
 constexpr int kMaxRows = 16;
-__host__ __device__ constexpr int Reducers(int warps) { return warps > 8 ? 2 : 1; }
+// Two CTAs of eight warps an SM, or one of sixteen where the activations take the shared memory of both; rings of what fits.
+__host__ __device__ constexpr int Warps(bool wide) { return wide ? 16 : 8; }
+__host__ __device__ constexpr int Reducers(bool wide) { return wide ? 2 : 1; }
+__host__ __device__ constexpr int Slots(bool wide) { return wide ? 3 : 5; }
+__host__ __device__ constexpr int Threads(bool wide) { return (Warps(wide) + Reducers(wide)) * 32; }
 
 __device__ __forceinline__ void BarrierSync(int id, int threads) {
   asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -145,9 +150,10 @@ __device__ __forceinline__ void BarrierArrive(int id, int threads) {
   asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-template <int kTiles, int kType, int kGroups>
-__global__ void __launch_bounds__((kMaxWarps + 2) * 32, 1)  // 112 registers: two CTAs of nine warps an SM
+template <int kTiles, int kType, int kGroups, bool kWide>
+__global__ void __launch_bounds__(Threads(kWide), kWide ? 1 : 2)
 VectorKernel(const VectorArgs a) {
+  constexpr int kWarps = Warps(kWide), kSlots = Slots(kWide), threads = Threads(kWide);
   constexpr int kPieces = HalfPieces(kType);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
@@ -155,18 +161,18 @@ VectorKernel(const VectorArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int clusters = static_cast<int>(gridDim.x) / ranks, first_round = static_cast<int>(blockIdx.x) / ranks;
-  const int threads = (a.warps + Reducers(a.warps)) * 32;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int step0 = a.steps * rank / ranks, steps = (a.steps * (rank + 1) / ranks) - step0;  // this CTA's
-  const int tiles_a_round = a.warps / a.parts;
+  const int tiles_a_round = kWarps / a.parts;
   const int my_tile = warp / a.parts, part = warp % a.parts;
   const int begin = steps * part / a.parts, count = (steps * (part + 1) / a.parts) - begin;  // this warp's
   const int pitch = Pitch(steps), columns = a.rows * kPieces;
-  const bool multiplies = warp < a.warps;
-  std::uint8_t* ring = smem + (warp * kSlots * kBlock);
-  float* meet = reinterpret_cast<float*>(smem + (a.warps * kSlots * kBlock));  // [2][warps][rows][16]
-  std::uint8_t* staged = reinterpret_cast<std::uint8_t*>(meet + (2 * a.meet_floats));  // and a column of zeros
+  const bool multiplies = warp < kWarps;
+  const std::uint32_t ring = SharedAddress(smem) + (warp * kSlots * kBlock) + (lane * 16);  // + this lane's piece
+  float* meet = reinterpret_cast<float*>(smem + (kWarps * kSlots * kBlock));  // [2][warps][rows][16]
+  const std::uint32_t staged_at = (kWarps * kSlots * kBlock) + (2 * a.meet_floats * 4);
+  std::uint8_t* staged = smem + staged_at;  // and a column of zeros
 
   // this warp's steps, round after round: where the next request reads
   const int first_tile = (first_round * tiles_a_round) + my_tile;
@@ -178,10 +184,10 @@ VectorKernel(const VectorArgs a) {
   int left = rounds_mine * count, left_of_round = count;
   auto request = [&](int slot) {  // one commit a call, so that the waits can count
     if (left > 0) {
-      std::uint8_t* dst = ring + (slot * kBlock) + (lane * 16);
-      CopyAsync16(dst, src);
-      CopyAsync16(dst + 512, src + 512);
-      if (lane < 4 * kGroups) CopyAsync16(dst + 1024, src + 1024);
+      const std::uint32_t dst = ring + (slot * kBlock);
+      CopyAsync16<0>(dst, src);
+      CopyAsync16<512>(dst, src);
+      if (lane < 4 * kGroups) CopyAsync16<1024>(dst, src);
       --left;
       src += kBlock;
       if (--left_of_round == 0) src += to_next_round, left_of_round = count;
@@ -201,8 +207,10 @@ VectorKernel(const VectorArgs a) {
 
   const int octets = steps * (kStep / 8), x0 = step0 * kStep;
   auto row_of = [&](int token) { return static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType)); };
-  for (int i = tid; i < octets; i += threads) {
-    *reinterpret_cast<uint4*>(staged + (columns * pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
+  if (a.zero_column) {
+    for (int i = tid; i < octets; i += threads) {
+      *reinterpret_cast<uint4*>(staged + (columns * pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
+    }
   }
   if constexpr (kType == kF32) {
     if (tid < kMaxRows) magnitude[tid] = 0;
@@ -240,26 +248,24 @@ VectorKernel(const VectorArgs a) {
   if (multiplies) {
     // this lane's column of each column tile: the token and piece it stands for, or the zeros
     const int piece = g % Cols(kPieces);
-    const std::uint8_t* column[kTiles];
+    std::uint32_t column[kTiles];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-      column[nt] = staged + ((token < a.rows ? (token * kPieces) + piece : columns) * pitch) + (t * 16) + (begin * 256);
+      column[nt] = staged_at + ((token < a.rows ? (token * kPieces) + piece : columns) * pitch) + (t * 16) + (begin * 256);
     }
     int slot = 0, buffer = 0;
     for (int round = first_round, n = 0; round < a.rounds; round += clusters, buffer ^= 1, ++n) {
-      float total[kTiles][4];
-#pragma unroll
-      for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0f;
+      Sums total[kTiles];
       if (n < rounds_mine) {
         for (int step = 0; step < count; ++step) {
           CopyAsyncWait<kSlots - 2>();
           __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
           request(slot == 0 ? kSlots - 1 : slot - 1);
           StepWeights<kGroups> w;
-          w.LoadShared(ring + (slot * kBlock), lane);
-          MultiplyStep<kType != kBF16, kGroups, kTiles>(w, a.bf16_scales, kTiles, total, [&](int nt, int i) {
-            return *reinterpret_cast<const uint4*>(column[nt] + (step * 256) + (i * 64));
+          w.LoadShared(smem + (((warp * kSlots) + slot) * kBlock), lane);
+          MultiplyStep<kType != kBF16, kGroups, kTiles>(w, kTiles, total, [&](int nt, int i) {
+            return *reinterpret_cast<const uint4*>(smem + column[nt] + (step * 256) + (i * 64));
           });
           slot = slot == kSlots - 1 ? 0 : slot + 1;
         }
@@ -293,8 +299,8 @@ VectorKernel(const VectorArgs a) {
       for (int o = rank; o < tiles_a_round; o += ranks) {
         const int tile = (round * tiles_a_round) + o;
         if (tile >= a.tiles) break;
-        for (int token = ((warp - a.warps) * tokens_a_pass) + lane_token; token < a.rows;
-             token += Reducers(a.warps) * tokens_a_pass) {
+        for (int token = ((warp - kWarps) * tokens_a_pass) + lane_token; token < a.rows;
+             token += Reducers(kWide) * tokens_a_pass) {
           float first[4] = {0.0f, 0.0f, 0.0f, 0.0f}, second[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           for (int q = 0; q < ranks; ++q) {
             const float* p = (ranks > 1 ? cluster.map_shared_rank(meet, q) : meet) + (buffer * a.meet_floats) +
@@ -332,47 +338,38 @@ VectorKernel(const VectorArgs a) {
   if (ranks > 1) cluster.sync();  // nobody leaves while another reads its sums
 }
 
-constexpr int kSmemLimit = 226 * 1024;
+constexpr int kSmemLimit = 226 * 1024, kSmemOfTwo = 112 * 1024;
 constexpr int kMaxRanks = 8;
-// Shared memory of a CTA: rings, two buffers of sums, the staged activations.
-std::int64_t SmemBytes(int warps, int ranks, int rows, int steps, int type, int block_bytes) {
-  return (static_cast<std::int64_t>(warps) * kSlots * block_bytes) + (2 * warps * kTileRows * rows * 4) +
-         (((rows * HalfPieces(type)) + 1) * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
+// Shared memory of a CTA: rings, two buffers of sums, the staged activations (and a column of zeros, unless
+// they fill every column tile).
+bool ZeroColumn(int rows, int type) { return type == kF32 ? rows % 4 != 0 : rows % 8 != 0; }
+std::int64_t SmemBytes(bool wide, int ranks, int rows, int steps, int type, int block_bytes) {
+  const int columns = (rows * HalfPieces(type)) + (ZeroColumn(rows, type) ? 1 : 0);
+  return (static_cast<std::int64_t>(Warps(wide)) * Slots(wide) * block_bytes) + (2 * Warps(wide) * kTileRows * rows * 4) +
+         (columns * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
 }
 
-template <int kTiles, int kType, int kGroups>
-int LaunchVector(VectorArgs a, cudaStream_t stream) {
+template <int kTiles, int kType, int kGroups, bool kWide>
+int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream) {
+  constexpr int kWarps = Warps(kWide);
   static thread_local int configured_device = -1;
   int device = -1;
   cudaGetDevice(&device);
   if (configured_device != device) {
-    const cudaError_t set = cudaFuncSetAttribute(VectorKernel<kTiles, kType, kGroups>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 kSmemLimit);
+    const cudaError_t set = cudaFuncSetAttribute(VectorKernel<kTiles, kType, kGroups, kWide>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (set != cudaSuccess) return Failed(set, "w4_vector attribute");
     configured_device = device;
   }
-  auto bytes = [&](int warps, int ranks) {
-    return SmemBytes(warps, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
-  };
-  // two CTAs of eight warps an SM where the staged activations allow it, else one of sixteen, of eight, else as few
-  // ranks as their memory needs
-  int ranks = 1, per_sm = 1;
-  if (a.warps = 8; bytes(8, 1) <= 112 * 1024) {
-    per_sm = 2;
-  } else if (a.warps = 16; bytes(16, 1) > kSmemLimit) {
-    a.warps = 8;
-    while (ranks < kMaxRanks && bytes(8, ranks) > kSmemLimit) ranks *= 2;
-    if (bytes(16, ranks) <= kSmemLimit) a.warps = 16;
-  }
-  const int ctas = std::max(1, SmCount() * per_sm / ranks);
-  a.parts = a.warps;
-  while (a.parts > 1 && (a.parts > a.steps / ranks || a.tiles >= 4 * ctas * (2 * a.warps / a.parts))) a.parts /= 2;
-  a.rounds = (a.tiles + (a.warps / a.parts) - 1) / (a.warps / a.parts);
-  a.meet_floats = a.warps * kTileRows * a.rows;
+  const int ctas = std::max(1, SmCount() * (smem <= kSmemOfTwo ? 2 : 1) / ranks);
+  a.parts = kWarps;
+  while (a.parts > 1 && (a.parts > a.steps / ranks || a.tiles >= 4 * ctas * (2 * kWarps / a.parts))) a.parts /= 2;
+  a.rounds = (a.tiles + (kWarps / a.parts) - 1) / (kWarps / a.parts);
+  a.meet_floats = kWarps * kTileRows * a.rows;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(std::min(a.rounds, ctas) * ranks));
-  config.blockDim = dim3(static_cast<unsigned>((a.warps + Reducers(a.warps)) * 32));
-  config.dynamicSmemBytes = static_cast<std::size_t>(bytes(a.warps, ranks));
+  config.blockDim = dim3(static_cast<unsigned>(Threads(kWide)));
+  config.dynamicSmemBytes = static_cast<std::size_t>(smem);
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -382,15 +379,32 @@ int LaunchVector(VectorArgs a, cudaStream_t stream) {
   attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&config, VectorKernel<kTiles, kType, kGroups>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&config, VectorKernel<kTiles, kType, kGroups, kWide>, a);
   return e == cudaSuccess ? 0 : Failed(e, "w4_vector launch");
+}
+
+template <int kTiles, int kType, int kGroups>
+int LaunchPlanned(VectorArgs a, cudaStream_t stream) {
+  auto bytes = [&](bool wide, int ranks) {
+    return SmemBytes(wide, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
+  };
+  a.zero_column = ZeroColumn(a.rows, kType);
+  if (const std::int64_t smem = bytes(false, 1); smem <= kSmemOfTwo) {
+    return LaunchVector<kTiles, kType, kGroups, false>(a, 1, smem, stream);
+  }
+  int ranks = 1;
+  while (ranks < kMaxRanks && bytes(false, ranks) > kSmemLimit) ranks *= 2;
+  if (const std::int64_t smem = bytes(true, ranks); smem <= kSmemLimit) {
+    return LaunchVector<kTiles, kType, kGroups, true>(a, ranks, smem, stream);
+  }
+  return LaunchVector<kTiles, kType, kGroups, false>(a, ranks, bytes(false, ranks), stream);
 }
 
 template <int kTiles, int kType>
 int LaunchGroups(int group, const VectorArgs& a, cudaStream_t stream) {
-  if (group == 128) return LaunchVector<kTiles, kType, 1>(a, stream);
-  if (group == 64) return LaunchVector<kTiles, kType, 2>(a, stream);
-  return LaunchVector<kTiles, kType, 4>(a, stream);
+  if (group == 128) return LaunchPlanned<kTiles, kType, 1>(a, stream);
+  if (group == 64) return LaunchPlanned<kTiles, kType, 2>(a, stream);
+  return LaunchPlanned<kTiles, kType, 4>(a, stream);
 }
 
 template <int kType>
@@ -434,6 +448,7 @@ int llmp_b200_w4_relayout(const llmp_b200_w4_source* source, const llmp_b200_w4_
   a.s = s;
   a.n = matrix->n, a.k = matrix->k, a.group = matrix->group, a.glu = matrix->glu;
   a.tiles = w4::Tiles(a.n, a.glu), a.steps = w4::Steps(a.k), a.block_bytes = w4::BlockBytes(a.group);
+  a.bf16 = matrix->scale_type == w4::kBF16;
   a.words = Aligned(s.codes, 4) && s.code_row % 4 == 0 && s.code_expert % 4 == 0;
   a.blocks = static_cast<std::int64_t>(matrix->experts) * a.tiles * a.steps;
   const unsigned grid = static_cast<unsigned>(std::min<std::int64_t>(a.blocks, 1 << 20));
@@ -471,13 +486,12 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream) {
   a.x = p.x, a.x_stride = p.x_stride;
   a.x_vec = Aligned(p.x, 16) && (p.rows == 1 || (p.x_stride * xb) % 16 == 0);
   a.y = p.y, a.y_stride = p.y_stride, a.y_type = p.y_type;
-  a.bf16_scales = p.w.scale_type == w4::kBF16;
   a.glu = p.glu, a.limit = p.limit;
   const auto s = static_cast<cudaStream_t>(stream);
   // as many rows a launch as a cluster's shared memory takes: all of them but for very long ones
   const int block_bytes = w4::BlockBytes(p.w.group);
   int most = p.rows;
-  while (most > 1 && w4::SmemBytes(8, w4::kMaxRanks, most, a.steps, p.x_type, block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
+  while (most > 1 && w4::SmemBytes(false, w4::kMaxRanks, most, a.steps, p.x_type, block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
   for (int first = 0; first < p.rows; first += most) {
     a.rows = std::min(most, p.rows - first);
     a.x = static_cast<const std::uint8_t*>(p.x) + (first * p.x_stride * xb);

@@ -7,12 +7,12 @@
 //   [2][32 lanes][16 bytes]  codes: lane (g, t) = (lane / 4, lane % 4) holds row g's and row g + 8's
 //                            values 32 i + 8 t .. + 7 of the step in word i = 0..3, the even values'
 //                            nibbles in the low half and the odd ones' in the high half
-//   [16 rows][128 / group]   words: the scale's 16 bits, and above them -(1024 + zero) as an f16
+//   [16 rows][128 / group]   words: the scale in F32, whose last byte the 16-bit types leave free for the zero
 //
 // so a warp reads a step with two 16-byte copies a lane and a few of its rows' words.  Codes multiply
 // as exact small integers: word & 0x000f000f, or'ed with 0x6400 (1024 in f16, whose last four mantissa
-// bits then are the code), plus -(1024 + zero), is a pair of neighbouring values in one addition;
-// & 0x00f000f0 the same way is 1024 + 16 code, a pair in one multiply-add; a shift by 8 serves the other
+// bits then are the code), plus -(1024 + zero), whose two bytes are 0xe4 and the zero, is a pair of neighbouring
+// values in one addition; & 0x00f000f0 the same way is 1024 + 16 code, a pair in one multiply-add; a shift by 8 serves the other
 // two.  In bf16, 0x4300 is 128, every pair needs its shift, and the multiply-add takes 2^-11 into the pair.  They are
 // the A fragment of mma.sync.m16n8k16, whose k order is free as long as B's is the same.  With a
 // GLU a tile's rows 0..7 are gate rows and 8..15 the same rows of up, so a lane's sums hold both.
@@ -180,34 +180,37 @@ template <bool kHalf, bool kFirst>
 __device__ __forceinline__ void Mma(float (&c)[4], std::uint32_t a0, std::uint32_t a1, std::uint32_t a2,
                                     std::uint32_t a3, std::uint32_t b0, std::uint32_t b1) {
   if constexpr (kFirst && kHalf) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   } else if constexpr (kFirst) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
   } else if constexpr (kHalf) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   } else {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 }
 
+__device__ __forceinline__ std::uint32_t SharedAddress(const void* p) {
+  return static_cast<std::uint32_t>(__cvta_generic_to_shared(p));
+}
 // The zero points of a row's group as the pairs take them.
 template <bool kHalf>
 struct Zeros {
   std::uint32_t near, far;  // f16: -(1024 + zero), -(64 + zero); bf16: -2^-11 (128 + zero), unused
   __device__ __forceinline__ explicit Zeros(std::uint32_t word) {
-    near = __byte_perm(word, 0, 0x3232);
+    near = __byte_perm(word, 0xe4e4e4e4u, 0x4040);
     if constexpr (kHalf) {
       const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&near), __floats2half2_rn(960.0f, 960.0f));
       far = *reinterpret_cast<const std::uint32_t*>(&v);
@@ -242,10 +245,9 @@ __device__ __forceinline__ void Pairs(std::uint32_t w, const Zeros<kHalf>& z, st
   }
 }
 // Copies that complete behind the thread's back, counted in groups.
-__device__ __forceinline__ void CopyAsync16(void* shared, const void* global) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                   static_cast<std::uint32_t>(__cvta_generic_to_shared(shared))), "l"(global)
-               : "memory");
+template <int kOffset = 0>
+__device__ __forceinline__ void CopyAsync16(std::uint32_t shared, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%2], 16;" ::"r"(shared), "l"(global), "n"(kOffset) : "memory");
 }
 __device__ __forceinline__ void CopyAsyncCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
@@ -258,7 +260,7 @@ __device__ __forceinline__ void CopyAsyncWait() {
 __device__ __forceinline__ void Stage8(void* shared, const void* row, std::int64_t at, int valid, bool vec) {
   const auto* p = static_cast<const unsigned short*>(row) + at;
   if (vec && valid >= 8) {
-    CopyAsync16(shared, p);
+    CopyAsync16(SharedAddress(shared), p);
     return;
   }
   std::uint32_t w[4];
@@ -270,58 +272,67 @@ __device__ __forceinline__ void Stage8(void* shared, const void* row, std::int64
   *reinterpret_cast<uint4*>(shared) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// total += scale * sum, two sums an instruction.
-__device__ __forceinline__ void AddScaled2(float& t0, float& t1, float scale, float s0, float s1) {
-  asm("{\n"
-      ".reg .b64 t, f, s;\n"
-      "mov.b64 t, {%0, %1};\n"
-      "mov.b64 f, {%2, %2};\n"
-      "mov.b64 s, {%3, %4};\n"
-      "fma.rn.f32x2 t, f, s, t;\n"
-      "mov.b64 {%0, %1}, t;\n"
-      "}\n"
-      : "+f"(t0), "+f"(t1)
-      : "f"(scale), "f"(s0), "f"(s1));
-}
-__device__ __forceinline__ float Scale(std::uint32_t word, bool bf16) {
-  return bf16 ? __uint_as_float(word << 16) : HalfBitsToFloat(word & 0xffffu);
-}
+__device__ __forceinline__ float Scale(std::uint32_t word) { return __uint_as_float(word & 0xffffff00u); }
 
 // A step of a tile as a lane holds it.
 template <int kGroups>
 struct StepWeights {
   uint4 a, b;                                // rows g and g + 8
   std::uint32_t word_a[kGroups], word_b[kGroups];
-  __device__ __forceinline__ void LoadShared(const std::uint8_t* block, int lane) {
-    a = *reinterpret_cast<const uint4*>(block + (lane * 16));
-    b = *reinterpret_cast<const uint4*>(block + 512 + (lane * 16));
-    const auto* words = reinterpret_cast<const std::uint32_t*>(block + 1024) + ((lane >> 2) * kGroups);
-#pragma unroll
-    for (int i = 0; i < kGroups; ++i) word_a[i] = words[i], word_b[i] = words[(8 * kGroups) + i];
-  }
-  __device__ __forceinline__ void Load(const std::uint8_t* block, int lane) {
-    a = LoadStream16(block + (lane * 16));
-    b = LoadStream16(block + 512 + (lane * 16));
+  template <typename Load16, typename Load8, typename Load4>
+  __device__ __forceinline__ void From(const std::uint8_t* block, int lane, Load16 load16, Load8 load8, Load4 load4) {
+    a = load16(block + (lane * 16));
+    b = load16(block + 512 + (lane * 16));
     const std::uint8_t* words = block + 1024 + ((lane >> 2) * (kGroups * 4));
     if constexpr (kGroups == 1) {
-      word_a[0] = LoadStream4(words);
-      word_b[0] = LoadStream4(words + 32);
+      word_a[0] = load4(words);
+      word_b[0] = load4(words + 32);
     } else if constexpr (kGroups == 2) {
-      const uint2 wa = LoadStream8(words), wb = LoadStream8(words + 64);
+      const uint2 wa = load8(words), wb = load8(words + 64);
       word_a[0] = wa.x, word_a[1] = wa.y, word_b[0] = wb.x, word_b[1] = wb.y;
     } else {
-      const uint4 wa = LoadStream16(words), wb = LoadStream16(words + 128);
+      const uint4 wa = load16(words), wb = load16(words + 128);
       word_a[0] = wa.x, word_a[1] = wa.y, word_a[2] = wa.z, word_a[3] = wa.w;
       word_b[0] = wb.x, word_b[1] = wb.y, word_b[2] = wb.z, word_b[3] = wb.w;
     }
   }
+  __device__ __forceinline__ void LoadShared(const std::uint8_t* block, int lane) {
+    From(block, lane, [](const void* p) { return *static_cast<const uint4*>(p); },
+         [](const void* p) { return *static_cast<const uint2*>(p); },
+         [](const void* p) { return *static_cast<const std::uint32_t*>(p); });
+  }
+  __device__ __forceinline__ void Load(const std::uint8_t* block, int lane) {
+    From(block, lane, [](const void* p) { return LoadStream16(p); }, [](const void* p) { return LoadStream8(p); },
+         [](const void* p) { return LoadStream4(p); });
+  }
+};
+
+// Two floats in a register pair: multiply-adds take both at once.
+using Float2 = unsigned long long;
+__device__ __forceinline__ Float2 Pack(float a, float b) {
+  Float2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void Unpack(Float2 v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ Float2 Fma2(Float2 a, Float2 b, Float2 c) {
+  Float2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+// A column tile's sums of a lane: row g's two columns, row g + 8's.
+struct Sums {
+  Float2 a, b;
+  __device__ __forceinline__ Sums() : a(0), b(0) {}
 };
 
 // total += the step's products: column quads come from column(nt, i), the 16 bytes that hold
 // values 32 i + 8 t .. + 7 of the step for column lane / 4 of column tile nt.
 template <bool kHalf, int kGroups, int kTiles, typename Column>
-__device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool bf16_scales, int tiles,
-                                             float (&total)[kTiles][4], Column column) {
+__device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, int tiles, Sums (&total)[kTiles],
+                                             Column column) {
   const std::uint32_t wa[4] = {w.a.x, w.a.y, w.a.z, w.a.w}, wb[4] = {w.b.x, w.b.y, w.b.z, w.b.w};
   constexpr int kBlocks = 4 / kGroups;  // 32-value blocks a group
 #pragma unroll
@@ -347,12 +358,13 @@ __device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool
         }
       }
     }
-    const float sa = Scale(w.word_a[group], bf16_scales), sb = Scale(w.word_b[group], bf16_scales);
+    const float sa = Scale(w.word_a[group]), sb = Scale(w.word_b[group]);
+    const Float2 sa2 = Pack(sa, sa), sb2 = Pack(sb, sb);
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       if (nt == 0 || nt < tiles) {
-        AddScaled2(total[nt][0], total[nt][1], sa, sum[nt][0], sum[nt][1]);
-        AddScaled2(total[nt][2], total[nt][3], sb, sum[nt][2], sum[nt][3]);
+        total[nt].a = Fma2(sa2, Pack(sum[nt][0], sum[nt][1]), total[nt].a);
+        total[nt].b = Fma2(sb2, Pack(sum[nt][2], sum[nt][3]), total[nt].b);
       }
     }
   }
@@ -361,7 +373,10 @@ __device__ __forceinline__ void MultiplyStep(const StepWeights<kGroups>& w, bool
 // A lane's sums of one column tile with a token's columns added up: values[r][j] is row g + 8 r,
 // token TokenOf(j); with 2 or 3 pieces only j = 0 counts.  An f16 value's second piece is 2^11 larger.
 template <bool kHalf, int kPieces>
-__device__ __forceinline__ void FoldColumns(const float (&total)[4], float (&values)[2][2]) {
+__device__ __forceinline__ void FoldColumns(const Sums& sums, float (&values)[2][2]) {
+  float total[4];
+  Unpack(sums.a, total[0], total[1]);
+  Unpack(sums.b, total[2], total[3]);
   if constexpr (kPieces == 1) {
     values[0][0] = total[0], values[0][1] = total[1], values[1][0] = total[2], values[1][1] = total[3];
   } else {
