@@ -220,6 +220,12 @@ struct Zeros {
     }
   }
 };
+// (w & mask) | bits, one instruction (two constants in an expression become two).
+__device__ __forceinline__ std::uint32_t AndOr(std::uint32_t w, std::uint32_t mask, std::uint32_t bits) {
+  std::uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(mask), "r"(bits));
+  return v;
+}
 // A word's codes less the zero point: pairs[j] holds values 2 j and 2 j + 1.
 template <bool kHalf>
 __device__ __forceinline__ void Pairs(std::uint32_t w, const Zeros<kHalf>& z, std::uint32_t (&pairs)[4]) {
@@ -228,7 +234,7 @@ __device__ __forceinline__ void Pairs(std::uint32_t w, const Zeros<kHalf>& z, st
     const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
 #pragma unroll
     for (int j = 0; j < 4; j += 2, w >>= 8) {
-      const std::uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
+      const std::uint32_t a = AndOr(w, 0x000f000fu, 0x64006400u), b = AndOr(w, 0x00f000f0u, 0x64006400u);
       const __half2 va = __hadd2(*reinterpret_cast<const __half2*>(&a), near);
       const __half2 vb = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, far);
       pairs[j] = *reinterpret_cast<const std::uint32_t*>(&va);
@@ -237,7 +243,7 @@ __device__ __forceinline__ void Pairs(std::uint32_t w, const Zeros<kHalf>& z, st
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const std::uint32_t a = ((w >> (4 * j)) & 0x000f000fu) | 0x43004300u;
+      const std::uint32_t a = AndOr(w >> (4 * j), 0x000f000fu, 0x43004300u);
       const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a), __float2bfloat162_rn(0x1p-11f),
                                        *reinterpret_cast<const __nv_bfloat162*>(&z.near));
       pairs[j] = *reinterpret_cast<const std::uint32_t*>(&v);
