@@ -213,24 +213,37 @@ VectorKernel(const VectorArgs a) {
     }
   }
   if constexpr (kType == kF32) {
+    // twice over the rows, four octets of a thread in flight at once: the largest magnitudes, then the pieces
     if (tid < kMaxRows) magnitude[tid] = 0;
     __syncthreads();
-    for (int token = 0; token < a.rows; ++token) {
-      std::uint32_t most = 0;
-      for (int i = tid; i < octets; i += threads) {
-        most = max(most, Magnitude8(row_of(token), x0 + (i * 8), a.k - x0 - (i * 8), a.x_vec));
+    constexpr int kBatch = 4;
+    const int all = a.rows * octets;  // octets are whole half warps
+    for (int first = tid; first - tid < all; first += kBatch * threads) {
+      std::uint32_t most[kBatch];
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const int i = first + (q * threads), token = i / octets, at = x0 + ((i - (token * octets)) * 8);
+        most[q] = i < all ? Magnitude8(row_of(token), at, a.k - at, a.x_vec) : 0;
       }
-      most = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0) atomicMax(&magnitude[token], most);
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const int i = first + (q * threads);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) most[q] = max(most[q], __shfl_xor_sync(0xffffffffu, most[q], o));
+        if ((lane & 15) == 0 && i < all) atomicMax(&magnitude[i / octets], most[q]);
+      }
     }
     __syncthreads();
-    for (int token = 0; token < a.rows; ++token) {
-      const float scale = PowerOfTwo(ScaleExponent(magnitude[token]));
-      for (int i = tid; i < octets; i += threads) {
+    for (int first = tid; first < all; first += kBatch * threads) {
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) {
+        const int i = first + (q * threads), token = i / octets, octet = i - (token * octets), at = x0 + (octet * 8);
+        if (i >= all) break;
         uint4 quads[2];
-        LoadHalf8(row_of(token), x0 + (i * 8), a.k - x0 - (i * 8), a.x_vec, scale, quads);
-        *reinterpret_cast<uint4*>(staged + ((token * 2) * pitch) + (i * 16)) = quads[0];
-        *reinterpret_cast<uint4*>(staged + (((token * 2) + 1) * pitch) + (i * 16)) = quads[1];
+        LoadHalf8(row_of(token), at, a.k - at, a.x_vec, PowerOfTwo(ScaleExponent(magnitude[token])), quads);
+        std::uint8_t* out = staged + ((token * 2) * pitch) + (octet * 16);
+        *reinterpret_cast<uint4*>(out) = quads[0];
+        *reinterpret_cast<uint4*>(out + pitch) = quads[1];
       }
     }
   } else {
@@ -289,46 +302,40 @@ VectorKernel(const VectorArgs a) {
       if (ranks > 1) cluster.sync(); else BarrierArrive(1 + buffer, threads);
     }
   } else {
-    // a lane adds up four rows (with a GLU: of gate and of up) of a token, a tile's tokens side by side
+    // a lane adds up four rows of a token (with a GLU two, of gate and of up), a tile's tokens side by side
     const bool glu = a.glu != LLMP_B200_GLU_NONE;
-    const int quad = glu ? (lane & 1) * 4 : (lane & 3) * 4;
-    const int lane_token = glu ? lane >> 1 : lane >> 2, tokens_a_pass = glu ? 16 : 8;
+    const int lane_row = glu ? (lane & 3) * 2 : (lane & 3) * 4;
     int buffer = 0;
     for (int round = first_round; round < a.rounds; round += clusters, buffer ^= 1) {
       if (ranks > 1) cluster.sync(); else BarrierSync(1 + buffer, threads);
       for (int o = rank; o < tiles_a_round; o += ranks) {
         const int tile = (round * tiles_a_round) + o;
         if (tile >= a.tiles) break;
-        for (int token = ((warp - kWarps) * tokens_a_pass) + lane_token; token < a.rows;
-             token += Reducers(kWide) * tokens_a_pass) {
-          float first[4] = {0.0f, 0.0f, 0.0f, 0.0f}, second[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int token = ((warp - kWarps) * 8) + (lane >> 2); token < a.rows; token += Reducers(kWide) * 8) {
+          float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // four rows, or two gate rows and two up rows
           for (int q = 0; q < ranks; ++q) {
             const float* p = (ranks > 1 ? cluster.map_shared_rank(meet, q) : meet) + (buffer * a.meet_floats) +
-                             (((o * a.parts * a.rows) + token) * kTileRows) + quad;
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f), sum2 = sum;
+                             (((o * a.parts * a.rows) + token) * kTileRows) + lane_row;
+            const int far = glu ? 8 : 2;
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
             for (int s = 0; s < a.parts; ++s, p += kTileRows * a.rows) {
-              const float4 v = *reinterpret_cast<const float4*>(p);
-              sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-              if (glu) {
-                const float4 u = *reinterpret_cast<const float4*>(p + 8);
-                sum2.x += u.x, sum2.y += u.y, sum2.z += u.z, sum2.w += u.w;
-              }
+              const float2 v = *reinterpret_cast<const float2*>(p), u = *reinterpret_cast<const float2*>(p + far);
+              part[0] += v.x, part[1] += v.y, part[2] += u.x, part[3] += u.y;
             }
             float up = Up(kType != kBF16);  // (each rank's F32 activations have their own scale)
             if constexpr (kType == kF32) {
               up = PowerOfTwo(-ScaleExponent(ranks > 1 ? *cluster.map_shared_rank(&magnitude[token], q) : magnitude[token]));
             }
-            first[0] = fmaf(sum.x, up, first[0]), first[1] = fmaf(sum.y, up, first[1]);
-            first[2] = fmaf(sum.z, up, first[2]), first[3] = fmaf(sum.w, up, first[3]);
-            second[0] = fmaf(sum2.x, up, second[0]), second[1] = fmaf(sum2.y, up, second[1]);
-            second[2] = fmaf(sum2.z, up, second[2]), second[3] = fmaf(sum2.w, up, second[3]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[r] = fmaf(part[r], up, sums[r]);
           }
-          const int row = (tile * (glu ? 8 : 16)) + quad;
+          if (glu) sums[0] = Glu(a.glu, sums[0], sums[2], a.limit), sums[1] = Glu(a.glu, sums[1], sums[3], a.limit);
+          const int row = (tile * (glu ? 8 : 16)) + lane_row;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            if (row + r >= a.outputs) break;
-            StoreValue(a.y, (token * a.y_stride) + row + r, a.y_type, glu ? Glu(a.glu, first[r], second[r], a.limit) : first[r]);
+            if (row + r >= a.outputs || (glu && r >= 2)) break;
+            StoreValue(a.y, (token * a.y_stride) + row + r, a.y_type, sums[r]);
           }
         }
       }
