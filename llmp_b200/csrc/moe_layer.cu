@@ -22,11 +22,14 @@ namespace {
 namespace cg = cooperative_groups;
 using namespace w4;
 
-constexpr int kThreads = 256, kWarps = 8;
+constexpr int kWarps = 16, kReducers = 2;          // of the first kernel: that multiply, that add up
+constexpr int kThreads = (kWarps + kReducers) * 32;
+constexpr int kSlots = 4;                          // steps a warp's ring holds
+constexpr int kTilesARound = 2;                    // each divided among kWarps / 2 warps
 constexpr int kCluster = 8;
 constexpr int kMaxTokens = 16, kMaxUsed = 16, kMaxExperts = 512;
 constexpr int kMaxPairs = kMaxTokens * kMaxUsed;
-constexpr int kXBudget = 100 * 1024;  // staged activations a CTA: two CTAs an SM
+constexpr int kFirstSmemLimit = 196 * 1024;        // dynamic; the choice's lists are static
 
 // The choice as the first kernel leaves it for the second: the named experts in ascending order, expert
 // i's (token, slot) pairs (t * used + j, in token order) being pairs[first[i]] .. pairs[first[i + 1] - 1].
@@ -60,6 +63,9 @@ struct LayerArgs {
   unsigned short* h;  // bf16 pieces of the GLU rows: [pair][piece][inter]
   int cap;            // tokens staged at a time
   int x_pitch;        // bytes of a staged piece of a token
+  int parts;          // warps that divide a tile's steps of hidden
+  int block_down;     // bytes of a step of the down slab
+  bool prefetch_down; // small enough for L2 while the first kernel works
 };
 
 // Pieces of a GLU value: 16-bit activations keep 16 bits of it, F32 ones all 24.
@@ -73,53 +79,81 @@ __device__ __forceinline__ std::uint32_t OrderKey(float v) {
 }
 
 struct FirstShared {
-  double partial[kWarps][kTileRows][kMaxTokens];  // the router's; the units' as floats, twice
   std::int32_t ids[kMaxPairs];
   float weights[kMaxPairs];
   std::uint32_t mask[kMaxExperts];  // tokens that name the expert
   std::int32_t start[kMaxExperts];
   std::int32_t group_expert[kMaxPairs], group_first[kMaxPairs], group_count[kMaxPairs];
+  std::int32_t token[kMaxPairs];    // of choice.pairs
   std::int32_t groups;
   Choice choice;
 };
 
-// kPieces of the router's elements: 16 experts' logits for the staged tokens, this warp's share of
-// hidden.  Products of two bf16 pieces are exact; a 32-value block's sum is F32 and the blocks are
-// added in 64 bits, because the choice compares values that may lie next to each other.
+// Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums and
+// the scores that a bias changes), two buffers of partial sums, the staged tokens and a column of zeros, logits.
+struct FirstLayout {
+  int ring, meet, staged, logits, bytes;
+  __host__ __device__ FirstLayout(int block_bytes, int cap, int pieces, int x_pitch, int tokens, int experts) {
+    ring = kWarps * kSlots * block_bytes;
+    const int before = (kWarps * kTileRows * kMaxTokens * 8) + (tokens * experts * 4);
+    if (ring < before) ring = (before + 255) / 256 * 256;
+    meet = ring;
+    staged = meet + (2 * kWarps * kTileRows * cap * 4);
+    logits = staged + (((cap * pieces) + 1) * x_pitch);
+    bytes = logits + (tokens * experts * 4);
+  }
+};
+
+// 16 experts' logits for the staged tokens over this warp's share of hidden.  Products of two bf16 pieces are
+// exact; a 32-value block's sum is F32 and the blocks are added in 64 bits, because the choice compares
+// values that may lie next to each other.  kBatch blocks' router rows are in flight together.
 template <int kType, int kRouter, int kTiles>
-__device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_t* staged, int first_expert, int tokens,
-                                           int warp, int lane, double (&partial)[kTileRows][kMaxTokens]) {
+__device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_t* smem, int staged, int first_expert,
+                                           int first_tile, int tokens, int warp, int lane,
+                                           double (&partial)[kTileRows][kMaxTokens]) {
   constexpr int kPieces = BfloatPieces(kType), kRouterPieces = BfloatPieces(kRouter);
+  constexpr int kBatch = kRouter == kF32 ? 2 : 4;
   const int g = lane >> 2, t = lane & 3;
   const int piece = g % Cols(kPieces);
-  const int tiles = (tokens + TokensATile(kPieces) - 1) / TokensATile(kPieces);
   double total[kTiles][4];
 #pragma unroll
   for (int nt = 0; nt < kTiles; ++nt) total[nt][0] = total[nt][1] = total[nt][2] = total[nt][3] = 0.0;
-  const int blocks = a.hidden / 32;
+  int column[kTiles];
+#pragma unroll
+  for (int nt = 0; nt < kTiles; ++nt) {
+    const int token = ((first_tile + nt) * TokensATile(kPieces)) + (g / Cols(kPieces));
+    const int c = token < tokens && piece < kPieces ? (token * kPieces) + piece : a.cap * kPieces;
+    column[nt] = staged + (c * a.x_pitch) + (t * 16);
+  }
   const int row_a = first_expert + g, row_b = row_a + 8;
   const auto* base = static_cast<const std::uint8_t*>(a.router);
   const std::int64_t row_bytes = a.router_stride * TypeBytes(kRouter);
-  for (int b = warp * blocks / kWarps; b < (warp + 1) * blocks / kWarps; ++b) {
-    uint4 qa[kRouterPieces], qb[kRouterPieces];
-    const int at = (32 * b) + (8 * t);
-    LoadBfloat8<kRouter>(base + (row_a * row_bytes), at, row_a < a.experts ? 8 : 0, a.router_vec, qa);
-    LoadBfloat8<kRouter>(base + (row_b * row_bytes), at, row_b < a.experts ? 8 : 0, a.router_vec, qb);
+  const int blocks = a.hidden / 32, end = (warp + 1) * blocks / kWarps;
+  for (int first = warp * blocks / kWarps; first < end; first += kBatch) {
+    float va[kBatch][8], vb[kBatch][8];
 #pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) {
-      if (nt >= tiles) break;
-      const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (token < tokens && piece < kPieces) {
-        x = *reinterpret_cast<const uint4*>(staged + (((token * kPieces) + piece) * a.x_pitch) + (at * 2));
-      }
+    for (int q = 0; q < kBatch; ++q) {
+      const int at = (32 * (first + q)) + (8 * t);
+      Load8<kRouter>(base + (row_a * row_bytes), at, first + q < end && row_a < a.experts ? 8 : 0, a.router_vec, va[q]);
+      Load8<kRouter>(base + (row_b * row_bytes), at, first + q < end && row_b < a.experts ? 8 : 0, a.router_vec, vb[q]);
+    }
 #pragma unroll
-      for (int r = 0; r < kRouterPieces; ++r) {
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        Mma<false, true>(sum, qa[r].x, qb[r].x, qa[r].y, qb[r].y, x.x, x.y);
-        Mma<false, false>(sum, qa[r].z, qb[r].z, qa[r].w, qb[r].w, x.z, x.w);
+    for (int q = 0; q < kBatch; ++q) {
+      if (first + q >= end) break;
+      uint4 qa[kRouterPieces], qb[kRouterPieces];
+      PackBfloat8(va[q], qa);
+      PackBfloat8(vb[q], qb);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) total[nt][c] += sum[c];
+      for (int nt = 0; nt < kTiles; ++nt) {
+        const uint4 x = *reinterpret_cast<const uint4*>(smem + column[nt] + ((first + q) * 64));
+#pragma unroll
+        for (int r = 0; r < kRouterPieces; ++r) {
+          float sum[4];
+          Mma<false, true>(sum, qa[r].x, qb[r].x, qa[r].y, qb[r].y, x.x, x.y);
+          Mma<false, false>(sum, qa[r].z, qb[r].z, qa[r].w, qb[r].w, x.z, x.w);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) total[nt][c] += sum[c];
+        }
       }
     }
   }
@@ -139,7 +173,7 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
     }
 #pragma unroll
     for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
-      const int token = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t, j);
+      const int token = ((first_tile + nt) * TokensATile(kPieces)) + TokenOf<kPieces>(t, j);
       if (token < tokens) {
         partial[g][token] = v[0][j];
         partial[g + 8][token] = v[1][j];
@@ -148,163 +182,200 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
   }
 }
 
-// Tokens token_of(0 .. count - 1) of x as pieces in shared memory.
+// Tokens token_of(0 .. count - 1) of x as pieces in shared memory, by threads tid, tid + threads, ...
 template <int kType, typename Token>
-__device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* staged, int count, Token token_of) {
+__device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* staged, int count, int tid, int threads,
+                                            Token token_of) {
   constexpr int kPieces = BfloatPieces(kType);
-  const int padded = a.steps_up * kStep;
-  for (int i = static_cast<int>(threadIdx.x); i < count * (padded / 8); i += kThreads) {
-    const int c = i / (padded / 8), at = (i % (padded / 8)) * 8;
-    uint4 quads[kPieces];
+  const int octets = a.steps_up * (kStep / 8);
+  for (int c = 0; c < count; ++c) {
     const auto* row = static_cast<const std::uint8_t*>(a.x) + (token_of(c) * a.x_stride * TypeBytes(kType));
-    LoadBfloat8<kType>(row, at, a.hidden - at, a.x_vec, quads);
+    for (int i = tid; i < octets; i += threads) {
+      std::uint8_t* out = staged + ((c * kPieces) * a.x_pitch) + (i * 16);
+      if constexpr (kType == kBF16) {
+        Stage8(out, row, i * 8, a.hidden - (i * 8), a.x_vec);
+      } else {
+        uint4 quads[kPieces];
+        LoadBfloat8<kType>(row, i * 8, a.hidden - (i * 8), a.x_vec, quads);
 #pragma unroll
-    for (int s = 0; s < kPieces; ++s) {
-      *reinterpret_cast<uint4*>(staged + (((c * kPieces) + s) * a.x_pitch) + (at * 2)) = quads[s];
+        for (int s = 0; s < kPieces; ++s) *reinterpret_cast<uint4*>(out + (s * a.x_pitch)) = quads[s];
+      }
     }
   }
+  CopyAsyncCommit();
 }
 
-// A warp: token t's experts, best first, and their weights from its logits.
-__device__ __forceinline__ void Choose(const LayerArgs& a, float* logits, int t, int lane, FirstShared& s) {
-  float* row = logits + (t * a.experts);
-  float top = __uint_as_float(0xff800000u);
-  for (int e = lane; e < a.experts; e += 32) top = fmaxf(top, row[e]);
+// A warp: token t's experts, best first, and their weights from its logits; `by`: room for what a bias makes of them.
+__device__ __forceinline__ void Choose(const LayerArgs& a, const float* row, float* by, int t, int lane, FirstShared& s) {
+  const bool softmax = a.score == LLMP_B200_SCORE_SOFTMAX;
+  float top = __uint_as_float(0xff800000u), total = 1.0f;
+  if (softmax) {
+    for (int e = lane; e < a.experts; e += 32) top = fmaxf(top, row[e]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float total = 0.0f;
-  bool bad = false;
-  if (a.score == LLMP_B200_SCORE_SOFTMAX) {
-    for (int e = lane; e < a.experts; e += 32) {
-      bad = bad || row[e] != row[e];
-      total += expf(row[e] - top);
-    }
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    total = 0.0f;
+    for (int e = lane; e < a.experts; e += 32) total += expf(row[e] - top);  // a NaN makes it one
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if (__any_sync(0xffffffffu, bad)) total = __uint_as_float(0x7fc00000u);
   }
-  auto score = [&](float l) {
-    return a.score == LLMP_B200_SCORE_SOFTMAX ? expf(l - top) / total : 1.0f / (1.0f + expf(-l));
-  };
+  auto score = [&](float l) { return softmax ? expf(l - top) / total : 1.0f / (1.0f + expf(-l)); };
+  const float* values = row;
+  if (a.bias != nullptr) {
+    for (int e = lane; e < a.experts; e += 32) by[e] = score(row[e]) + a.bias[e];
+    values = by;
+  }
   // a lane's best of its experts; the one that is taken is struck out and its lane looks again
-  auto key_of = [&](int e) {
-    return OrderKey(a.bias == nullptr ? row[e] : score(row[e]) + a.bias[e]);
-  };
   std::uint32_t taken = 0;  // bit i: expert lane + 32 i
   std::uint32_t best = 0;
   int best_at = 0;
   auto look = [&]() {
     best = 0;
     for (int e = lane, i = 0; e < a.experts; e += 32, ++i) {
-      if ((taken >> i) & 1u) continue;
-      const std::uint32_t k = key_of(e);
+      const std::uint32_t k = ((taken >> i) & 1u) != 0 ? 0u : OrderKey(values[e]);
       if (k > best) best = k, best_at = e;
     }
   };
   look();
-  float sum = 0.0f, mine = 0.0f;
+  int mine = 0;
   for (int j = 0; j < a.used; ++j) {
     const std::uint32_t most = __reduce_max_sync(0xffffffffu, best);
     const int at = static_cast<int>(__reduce_min_sync(0xffffffffu, best == most ? static_cast<unsigned>(best_at) : 0x7fffffffu));
-    const float p = score(row[at]);
-    sum += p;
-    if (lane == j) mine = p;
-    if (lane == 0) s.ids[(t * a.used) + j] = at;
+    if (lane == j) mine = at;
     if ((at & 31) == lane) {
       taken |= 1u << (at >> 5);
       look();
     }
   }
+  const float p = lane < a.used ? score(row[mine]) : 0.0f;
+  float sum = p;
+  if (a.renormalize != 0) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
   if (lane < a.used) {
-    const float w = a.renormalize != 0 ? mine / sum : mine;
-    s.weights[(t * a.used) + lane] = w * a.scale;
+    s.ids[(t * a.used) + lane] = mine;
+    s.weights[(t * a.used) + lane] = (a.renormalize != 0 ? p / sum : p) * a.scale;
   }
 }
 
+__device__ __forceinline__ void BarrierSync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void BarrierArrive(int id, int threads) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 template <int kType, int kGroups>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1)
 FirstKernel(const LayerArgs a) {
   constexpr int kPieces = BfloatPieces(kType);
   constexpr int kTiles = kMaxTokens / TokensATile(kPieces);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ FirstShared s;
-  std::uint8_t* staged = smem;
-  float* logits = reinterpret_cast<float*>(smem + (static_cast<std::size_t>(a.cap) * kPieces * a.x_pitch));
+  const FirstLayout at(kBlock, a.cap, kPieces, a.x_pitch, a.tokens, a.experts);
+  std::uint8_t* staged = smem + at.staged;
+  float* logits = reinterpret_cast<float*>(smem + at.logits);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
   GridLaunchDependents();
+  const int expert_tiles = (a.experts + 15) / 16;
+  {  // this CTA's router rows into L2 while the kernel before ends
+    const std::size_t row_bytes = static_cast<std::size_t>(a.hidden) * TypeBytes(a.router_type);
+    const int lines = static_cast<int>((row_bytes + 127) / 128);
+    for (int m = rank; m < expert_tiles; m += kCluster) {
+      for (int i = tid; i < 16 * lines; i += kThreads) {
+        const int e = (m * 16) + (i / lines);
+        if (e < a.experts) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const std::uint8_t*>(a.router) +
+                                                       (e * a.router_stride * TypeBytes(a.router_type)) + ((i % lines) * 128)));
+        }
+      }
+    }
+  }
+  for (int i = tid; i < a.x_pitch / 16; i += kThreads) {
+    *reinterpret_cast<uint4*>(staged + (a.cap * kPieces * a.x_pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
+  }
+  for (int e = tid; e < a.experts; e += kThreads) s.mask[e] = 0;
   GridDependencyWait();
-  cluster.sync();  // every CTA of the cluster has begun: its shared memory may be written
 
   // ---- the router's product: 16 experts at a time, CTA rank r the tiles r, r + 8, ...
-  const int expert_tiles = (a.experts + 15) / 16;
+  auto* partial = reinterpret_cast<double(*)[kTileRows][kMaxTokens]>(smem);
+  bool met = false;
   for (int first = 0; first < a.tokens; first += a.cap) {
     const int count = min(a.cap, a.tokens - first);
-    __syncthreads();
-    StageTokens<kType>(a, staged, count, [&](int c) { return static_cast<std::int64_t>(first + c); });
+    if (first > 0) __syncthreads();
+    StageTokens<kType>(a, staged, count, tid, kThreads, [&](int c) { return static_cast<std::int64_t>(first + c); });
+    CopyAsyncWait<0>();
     __syncthreads();
     for (int m = rank; m < expert_tiles; m += kCluster) {
-      if (a.router_type == kF32) {
-        RouterTile<kType, kF32, kTiles>(a, staged, m * 16, count, warp, lane, s.partial[warp]);
-      } else if (a.router_type == kF16) {
-        RouterTile<kType, kF16, kTiles>(a, staged, m * 16, count, warp, lane, s.partial[warp]);
-      } else {
-        RouterTile<kType, kBF16, kTiles>(a, staged, m * 16, count, warp, lane, s.partial[warp]);
+      if (warp < kWarps) {
+        constexpr int kAtOnce = kTiles < 2 ? kTiles : 2;
+        const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
+        for (int nt = 0; nt < tiles; nt += kAtOnce) {
+          if (a.router_type == kF32) {
+            RouterTile<kType, kF32, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
+          } else if (a.router_type == kF16) {
+            RouterTile<kType, kF16, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
+          } else {
+            RouterTile<kType, kBF16, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
+          }
+        }
       }
       __syncthreads();
-      for (int i = tid; i < 16 * count; i += kThreads) {
-        const int row = i / count, c = i % count, e = (m * 16) + row;
+      if (!met) cluster.sync();  // every CTA of the cluster has begun: its shared memory may be written
+      met = true;
+      // eight threads a logit, each storing to one rank
+      for (int i = tid; i < 16 * count * kCluster; i += kThreads) {
+        const int r = i % kCluster, row = (i / kCluster) % 16, c = (i / kCluster) / 16, e = (m * 16) + row;
         if (e >= a.experts) continue;
         double sum = 0.0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += s.partial[w][row][c];
-        for (int r = 0; r < kCluster; ++r) {
-          cluster.map_shared_rank(logits, r)[((first + c) * a.experts) + e] = static_cast<float>(sum);
-        }
+        for (int w = 0; w < kWarps; ++w) sum += partial[w][row][c];
+        cluster.map_shared_rank(logits, r)[((first + c) * a.experts) + e] = static_cast<float>(sum);
       }
       __syncthreads();
     }
   }
-  for (int e = tid; e < a.experts; e += kThreads) s.mask[e] = 0;
+  if (!met) cluster.sync();
   cluster.sync();  // the cluster's logits are in every CTA
 
   // ---- the choice, the same in every CTA
-  for (int t = warp; t < a.tokens; t += kWarps) Choose(a, logits, t, lane, s);
+  if (warp < a.tokens) {
+    auto* by = reinterpret_cast<float*>(smem + (kWarps * kTileRows * kMaxTokens * 8));
+    Choose(a, logits + (warp * a.experts), by + (warp * a.experts), warp, lane, s);
+    if (lane < a.used) atomicOr(&s.mask[s.ids[(warp * a.used) + lane]], 1u << warp);
+  }
   __syncthreads();
   const int pairs = a.tokens * a.used;
-  for (int p = tid; p < pairs; p += kThreads) atomicOr(&s.mask[s.ids[p]], 1u << (p / a.used));
-  __syncthreads();
   if (warp == 0) {
     int named = 0, first = 0, groups = 0;
     for (int base = 0; base < a.experts; base += 32) {
       const int e = base + lane;
       const int count = e < a.experts ? __popc(s.mask[e]) : 0;
-      const int pieces = (count + a.cap - 1) / a.cap;
-      int sum_named = count > 0 ? 1 : 0, sum_first = count, sum_groups = pieces;
+      const int pieces = count <= a.cap ? (count > 0 ? 1 : 0) : (count + a.cap - 1) / a.cap;
+      int packed = (count > 0 ? 1 : 0) | (count << 10) | (pieces << 20);  // each at most 256 in all
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int n0 = __shfl_up_sync(0xffffffffu, sum_named, o), n1 = __shfl_up_sync(0xffffffffu, sum_first, o),
-                  n2 = __shfl_up_sync(0xffffffffu, sum_groups, o);
-        if (lane >= o) sum_named += n0, sum_first += n1, sum_groups += n2;
+        const int below = __shfl_up_sync(0xffffffffu, packed, o);
+        if (lane >= o) packed += below;
       }
       if (count > 0) {
-        const int at = named + sum_named - 1, begin = first + sum_first - count;
-        s.choice.expert[at] = e;
-        s.choice.first[at] = begin;
+        const int i = named + (packed & 0x3ff) - 1, begin = first + ((packed >> 10) & 0x3ff) - count;
+        const int group = groups + (packed >> 20) - pieces;
+        s.choice.expert[i] = e;
+        s.choice.first[i] = begin;
         s.start[e] = begin;
         for (int q = 0; q < pieces; ++q) {
-          const int i = groups + sum_groups - pieces + q;
-          s.group_expert[i] = e;
-          s.group_first[i] = begin + (q * a.cap);
-          s.group_count[i] = min(a.cap, count - (q * a.cap));
+          s.group_expert[group + q] = e;
+          s.group_first[group + q] = begin + (q * a.cap);
+          s.group_count[group + q] = min(a.cap, count - (q * a.cap));
         }
       }
-      named += __shfl_sync(0xffffffffu, sum_named, 31);
-      first += __shfl_sync(0xffffffffu, sum_first, 31);
-      groups += __shfl_sync(0xffffffffu, sum_groups, 31);
+      const int all = __shfl_sync(0xffffffffu, packed, 31);
+      named += all & 0x3ff, first += (all >> 10) & 0x3ff, groups += all >> 20;
     }
     if (lane == 0) {
       s.choice.named = named;
@@ -315,140 +386,253 @@ FirstKernel(const LayerArgs a) {
   __syncthreads();
   for (int p = tid; p < pairs; p += kThreads) {
     const int e = s.ids[p], t = p / a.used;
-    s.choice.pairs[s.start[e] + __popc(s.mask[e] & ((1u << t) - 1u))] = p;
+    const int place = s.start[e] + __popc(s.mask[e] & ((1u << t) - 1u));
+    s.choice.pairs[place] = p;
+    s.token[place] = t;
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int p = tid; p < pairs; p += kThreads) {
-      a.ids[p] = s.ids[p];
-      a.weights[p] = s.weights[p];
-      a.choice->pairs[p] = s.choice.pairs[p];
-    }
-    for (int i = tid; i < s.choice.named; i += kThreads) a.choice->expert[i] = s.choice.expert[i];
-    for (int i = tid; i <= s.choice.named; i += kThreads) a.choice->first[i] = s.choice.first[i];
-    if (tid == 0) a.choice->named = s.choice.named;
-  }
 
-  // ---- this CTA's units: (group, tile of 8 gate and 8 up rows), the warps a share of hidden each
-  const std::int64_t units = static_cast<std::int64_t>(s.groups) * a.tiles_up;
-  const int u0 = static_cast<int>(units * blockIdx.x / gridDim.x), u1 = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x);
+  // ---- this CTA's rounds: a group's two neighbouring tiles of 8 gate and 8 up rows, each divided among the warps
+  const int rounds_a_group = (a.tiles_up + kTilesARound - 1) / kTilesARound;
+  const std::int64_t rounds = static_cast<std::int64_t>(s.groups) * rounds_a_group;
+  const int first_round = static_cast<int>(rounds * blockIdx.x / gridDim.x);
+  const int end_round = static_cast<int>(rounds * (blockIdx.x + 1) / gridDim.x);
   const bool all_staged = a.tokens <= a.cap;
-  const int piece = g % Cols(kPieces);
-  const int step0 = warp * a.steps_up / kWarps, step1 = (warp + 1) * a.steps_up / kWarps;
-  auto* sums = reinterpret_cast<float*>(s.partial);  // [2][kWarps][kTileRows][kMaxTokens]
-  int staged_group = -1;
-  for (int u = u0; u < u1; ++u) {
-    const int group = u / a.tiles_up, tile = u % a.tiles_up;
-    const int e = s.group_expert[group], begin = s.group_first[group], count = s.group_count[group];
-    if (!all_staged && staged_group != group) {
-      __syncthreads();
-      StageTokens<kType>(a, staged, count, [&](int c) { return static_cast<std::int64_t>(s.choice.pairs[begin + c] / a.used); });
-      __syncthreads();
-      staged_group = group;
-    }
-    std::uint32_t column_at[kTiles];
+  float* meet = reinterpret_cast<float*>(smem + at.meet);
+  const int meet_floats = kWarps * kTileRows * a.cap;
+  if (warp < kWarps) {
+    const int my_tile = warp / (kWarps / kTilesARound), part = warp % (kWarps / kTilesARound);
+    const int begin = part < a.parts ? a.steps_up * part / a.parts : 0;
+    const int steps = part < a.parts ? (a.steps_up * (part + 1) / a.parts) - begin : 0;
+    std::uint8_t* ring = smem + (warp * kSlots * kBlock);
+    // where the next request reads
+    int load_group = first_round / rounds_a_group, load_pair = first_round % rounds_a_group;
+    int load_rounds = end_round - first_round, load_left = 0;
+    const std::uint8_t* src = nullptr;
+    auto next_load_round = [&]() {  // the next round in which this warp has a tile
+      while (load_left == 0 && load_rounds > 0 && steps > 0) {
+        const int tile = (load_pair * kTilesARound) + my_tile;
+        if (tile < a.tiles_up) {
+          src = a.gate_up + ((((static_cast<std::size_t>(s.group_expert[load_group]) * a.tiles_up) + tile) * a.steps_up) + begin) * kBlock +
+                (lane * 16);
+          load_left = steps;
+        }
+        --load_rounds;
+        if (++load_pair == rounds_a_group) load_pair = 0, ++load_group;
+      }
+    };
+    auto request = [&](int slot) {  // one commit a call, so that the waits can count
+      if (load_left == 0) next_load_round();
+      if (load_left > 0) {
+        const std::uint32_t dst = SharedAddress(ring) + (slot * kBlock) + (lane * 16);
+        CopyAsync16<0>(dst, src);
+        CopyAsync16<512>(dst, src);
+        if (lane < 4 * kGroups) CopyAsync16<1024>(dst, src);
+        --load_left;
+        src += kBlock;
+      }
+      CopyAsyncCommit();
+    };
 #pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) {
-      const int c = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-      column_at[nt] = 0xffffffffu;
-      if (c < count && piece < kPieces) {
-        const int row = all_staged ? s.choice.pairs[begin + c] / a.used : c;
-        column_at[nt] = static_cast<std::uint32_t>((((row * kPieces) + piece) * a.x_pitch) + (t4 * 16));
+    for (int i = 0; i < kSlots - 1; ++i) request(i);
+    if (a.prefetch_down) {  // the named experts' down rows, on their way while this kernel works
+      const std::int64_t lines = static_cast<std::int64_t>(a.tiles_down) * a.steps_down * a.block_down / 128;  // an expert's
+      const std::int64_t all = lines * s.choice.named, stride = static_cast<std::int64_t>(gridDim.x) * kWarps * 32;
+      for (std::int64_t i = (static_cast<std::int64_t>(blockIdx.x) * kWarps * 32) + tid; i < all; i += stride) {
+        const std::int64_t n = i / lines;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.down + ((s.choice.expert[n] * lines) + (i - (n * lines))) * 128));
       }
     }
-    const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
-    Sums total[kTiles];
-    const std::uint8_t* block =
-        a.gate_up + ((((static_cast<std::size_t>(e) * a.tiles_up) + tile) * a.steps_up) + step0) * kBlock;
-    for (int step = step0; step < step1; ++step, block += kBlock) {
-      StepWeights<kGroups> w;
-      w.Load(block, lane);
-      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int i) {
-        if (column_at[nt] == 0xffffffffu) return make_uint4(0, 0, 0, 0);
-        return *reinterpret_cast<const uint4*>(staged + column_at[nt] + (step * 256) + (i * 64));
-      });
-    }
-    float* buffer = sums + ((u & 1) * kWarps * kTileRows * kMaxTokens);
+    const int piece = g % Cols(kPieces);
+    int group = first_round / rounds_a_group, pair = first_round % rounds_a_group;
+    int slot = 0, buffer = 0, staged_group = -1;
+    for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
+      const int first = s.group_first[group], count = s.group_count[group];
+      if (!all_staged && staged_group != group) {
+        if (staged_group >= 0) BarrierSync(5, kWarps * 32);
+        StageTokens<kType>(a, staged, count, tid, kWarps * 32, [&](int c) { return static_cast<std::int64_t>(s.token[first + c]); });
+        CopyAsyncWait<0>();
+        BarrierSync(5, kWarps * 32);
+        staged_group = group;
+      }
+      const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
+      std::uint32_t column[kTiles];
 #pragma unroll
-    for (int nt = 0; nt < kTiles; ++nt) {
-      if (nt >= tiles) break;
-      float v[2][2];
-      FoldColumns<false, kPieces>(total[nt], v);
-#pragma unroll
-      for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
-        const int c = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t4, j);
-        if (c < count) {
-          buffer[(((warp * kTileRows) + g) * kMaxTokens) + c] = v[0][j];
-          buffer[(((warp * kTileRows) + g + 8) * kMaxTokens) + c] = v[1][j];
+      for (int nt = 0; nt < kTiles; ++nt) {
+        const int c = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
+        int row = a.cap * kPieces;
+        if (c < count && piece < kPieces) row = ((all_staged ? s.token[first + c] : c) * kPieces) + piece;
+        column[nt] = at.staged + (row * a.x_pitch) + (t4 * 16) + (begin * 256);
+      }
+      Sums total[kTiles];
+      if ((pair * kTilesARound) + my_tile < a.tiles_up) {
+        for (int step = 0; step < steps; ++step) {
+          CopyAsyncWait<kSlots - 2>();
+          __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
+          request(slot == 0 ? kSlots - 1 : slot - 1);
+          StepWeights<kGroups> w;
+          w.LoadShared(smem + (((warp * kSlots) + slot) * kBlock), lane);
+          MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int i) {
+            return *reinterpret_cast<const uint4*>(smem + column[nt] + (step * 256) + (i * 64));
+          });
+          slot = slot == kSlots - 1 ? 0 : slot + 1;
         }
       }
-    }
-    __syncthreads();
-    // the other buffer's readers are past the barrier before the one that its next writers pass
-    for (int i = tid; i < 8 * count; i += kThreads) {
-      const int row = i % 8, c = i / 8, at = (tile * 8) + row;
-      if (at >= a.inter) continue;
-      float gate = 0.0f, up = 0.0f;
+      // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
+      if (round - first_round >= 2) BarrierSync(3 + buffer, kThreads);
+      float* mine = meet + (buffer * meet_floats) + (warp * kTileRows * a.cap);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        gate += buffer[(((w * kTileRows) + row) * kMaxTokens) + c];
-        up += buffer[(((w * kTileRows) + row + 8) * kMaxTokens) + c];
+      for (int nt = 0; nt < kTiles; ++nt) {
+        if (nt >= tiles) break;
+        float v[2][2];
+        FoldColumns<false, kPieces>(total[nt], v);
+#pragma unroll
+        for (int j = 0; j < (kPieces == 1 ? 2 : 1); ++j) {
+          const int c = (nt * TokensATile(kPieces)) + TokenOf<kPieces>(t4, j);
+          if (c < count) {
+            mine[(c * kTileRows) + g] = v[0][j];
+            mine[(c * kTileRows) + g + 8] = v[1][j];
+          }
+        }
       }
-      constexpr int kGlu = GluPieces(kType);
-      std::uint32_t bits[kGlu];
-      Split<kGlu>(Glu(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
-      unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[begin + c]) * kGlu * a.inter) + at;
+      BarrierArrive(1 + buffer, kThreads);
+      if (++pair == rounds_a_group) pair = 0, ++group;
+    }
+  } else {
+    if (blockIdx.x == 0) {  // the choice for the caller and the second kernel
+      for (int p = tid - (kWarps * 32); p < pairs; p += kReducers * 32) {
+        a.ids[p] = s.ids[p];
+        a.weights[p] = s.weights[p];
+        a.choice->pairs[p] = s.choice.pairs[p];
+      }
+      for (int i = tid - (kWarps * 32); i < s.choice.named; i += kReducers * 32) a.choice->expert[i] = s.choice.expert[i];
+      for (int i = tid - (kWarps * 32); i <= s.choice.named; i += kReducers * 32) a.choice->first[i] = s.choice.first[i];
+      if (tid == kWarps * 32) a.choice->named = s.choice.named;
+    }
+    // a warp a tile of the round; a lane a row of four tokens
+    const int my_tile = warp - kWarps, row = lane & 7;
+    int group = first_round / rounds_a_group, pair = first_round % rounds_a_group, buffer = 0;
+    for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
+      BarrierSync(1 + buffer, kThreads);
+      const int first = s.group_first[group], count = s.group_count[group];
+      const int out = (((pair * kTilesARound) + my_tile) * 8) + row;
+      const float* p = meet + (buffer * meet_floats) + (my_tile * (kWarps / kTilesARound) * kTileRows * a.cap) + row;
+      for (int c = lane >> 3; c < count && out < a.inter; c += 4) {
+        float gate = 0.0f, up = 0.0f;
+#pragma unroll 4
+        for (int q = 0; q < a.parts; ++q) {
+          gate += p[((q * a.cap) + c) * kTileRows];
+          up += p[(((q * a.cap) + c) * kTileRows) + 8];
+        }
+        constexpr int kGlu = GluPieces(kType);
+        std::uint32_t bits[kGlu];
+        Split<kGlu>(Glu(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
+        unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[first + c]) * kGlu * a.inter) + out;
 #pragma unroll
-      for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);
+        for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);
+      }
+      BarrierArrive(3 + buffer, kThreads);
+      if (++pair == rounds_a_group) pair = 0, ++group;
     }
   }
 }
 
-// A CTA's 16 rows of the output: its warps take (expert, half of inter) items in turn, each pair's
-// sums meet in shared memory and a token's slots are added in order.
+// A CTA's 16 rows of the output: its warps take (expert, half of inter) items in turn, their weights through rings as
+// in the first kernel, the GLU rows straight from L2 a step ahead; each pair's sums meet in shared memory and
+// a token's slots are added in order.
 constexpr int kParts = 2;
+constexpr int kSecondWarps = 16;
 
 template <int kType, int kGroups>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kSecondWarps * 32, 1)
 SecondKernel(const LayerArgs a) {
   constexpr int kGlu = GluPieces(kType);
   constexpr int kTiles = kMaxTokens / TokensATile(kGlu);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
-  auto* sums = reinterpret_cast<float*>(smem);  // [pair][part][16 rows]
+  __shared__ Choice choice;
+  const int threads = static_cast<int>(blockDim.x), warps = threads >> 5;
+  auto* sums = reinterpret_cast<float*>(smem + (warps * kSlots * kBlock));  // [pair][part][16 rows]
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   GridLaunchDependents();
   GridDependencyWait();
-  const int tile = static_cast<int>(blockIdx.x);
-  const int named = __ldcg(&a.choice->named);
+  const int tile = static_cast<int>(blockIdx.x), pairs = a.tokens * a.used;
+  for (int i = tid; i < pairs; i += threads) {
+    choice.expert[i] = __ldcg(&a.choice->expert[i]);   // (what is past the named ones is not used)
+    choice.pairs[i] = __ldcg(&a.choice->pairs[i]);
+    choice.first[i] = __ldcg(&a.choice->first[i]);
+  }
+  if (tid == 0) choice.first[pairs] = __ldcg(&a.choice->first[pairs]);
+  if (tid == threads - 1) choice.named = __ldcg(&a.choice->named);
+  __syncthreads();
+  const int items = choice.named * kParts;
   const int piece = g % Cols(kGlu);
-  for (int item = warp; item < named * kParts; item += kWarps) {
-    const int i = item / kParts, part = item % kParts;
-    const int e = __ldcg(&a.choice->expert[i]), begin = __ldcg(&a.choice->first[i]);
-    const int count = __ldcg(&a.choice->first[i + 1]) - begin;
-    const int step0 = part * a.steps_down / kParts, step1 = (part + 1) * a.steps_down / kParts;
+  auto step0_of = [&](int item) { return (item % kParts) * a.steps_down / kParts; };
+  auto steps_of = [&](int item) { return (((item % kParts) + 1) * a.steps_down / kParts) - step0_of(item); };
+  std::uint8_t* ring = smem + (warp * kSlots * kBlock);
+  int load_item = warp - warps, load_left = 0;
+  const std::uint8_t* src = nullptr;
+  auto request = [&](int slot) {
+    while (load_left == 0 && load_item < items) {
+      load_item += warps;
+      if (load_item >= items) break;
+      load_left = steps_of(load_item);
+      src = a.down + ((((static_cast<std::size_t>(choice.expert[load_item / kParts]) * a.tiles_down) + tile) * a.steps_down) +
+                      step0_of(load_item)) * kBlock + (lane * 16);
+    }
+    if (load_left > 0) {
+      const std::uint32_t dst = SharedAddress(ring) + (slot * kBlock) + (lane * 16);
+      CopyAsync16<0>(dst, src);
+      CopyAsync16<512>(dst, src);
+      if (lane < 4 * kGroups) CopyAsync16<1024>(dst, src);
+      --load_left;
+      src += kBlock;
+    }
+    CopyAsyncCommit();
+  };
+#pragma unroll
+  for (int i = 0; i < kSlots - 1; ++i) request(i);
+  int slot = 0;
+  for (int item = warp; item < items; item += warps) {
+    const int begin = choice.first[item / kParts], count = choice.first[(item / kParts) + 1] - begin;
+    const int step0 = step0_of(item), steps = steps_of(item);
     const unsigned short* column[kTiles];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int c = (nt * TokensATile(kGlu)) + (g / Cols(kGlu));
       column[nt] = nullptr;
       if (c < count && piece < kGlu) {
-        column[nt] = a.h + (((static_cast<std::size_t>(__ldcg(&a.choice->pairs[begin + c])) * kGlu) + piece) * a.inter) + (t4 * 8);
+        column[nt] = a.h + (((static_cast<std::size_t>(choice.pairs[begin + c]) * kGlu) + piece) * a.inter) + (t4 * 8);
       }
     }
+    auto fetch = [&](int nt, int step, int b) {
+      const int at = ((step0 + step) * kStep) + (32 * b);  // inter is whole 32-value blocks
+      if (column[nt] == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
+      return __ldcg(reinterpret_cast<const uint4*>(column[nt] + at));
+    };
     const int tiles = (count + TokensATile(kGlu) - 1) / TokensATile(kGlu);
     Sums total[kTiles];
-    const std::uint8_t* block =
-        a.down + ((((static_cast<std::size_t>(e) * a.tiles_down) + tile) * a.steps_down) + step0) * kBlock;
-    for (int step = step0; step < step1; ++step, block += kBlock) {
+    uint4 ahead[4];
+    if (steps > 0) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) ahead[b] = fetch(0, 0, b);
+    }
+    for (int step = 0; step < steps; ++step) {
+      uint4 now[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) now[b] = ahead[b];
+      if (step + 1 < steps) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) ahead[b] = fetch(0, step + 1, b);
+      }
+      CopyAsyncWait<kSlots - 2>();
+      __syncwarp();
+      request(slot == 0 ? kSlots - 1 : slot - 1);
       StepWeights<kGroups> w;
-      w.Load(block, lane);
-      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int b) {
-        const int at = (step * kStep) + (32 * b);  // inter is whole 32-value blocks
-        if (column[nt] == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
-        return __ldcg(reinterpret_cast<const uint4*>(column[nt] + at));
-      });
+      w.LoadShared(smem + (((warp * kSlots) + slot) * kBlock), lane);
+      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int b) { return nt == 0 ? now[b] : fetch(nt, step, b); });
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
     }
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
@@ -457,14 +641,14 @@ SecondKernel(const LayerArgs a) {
       FoldColumns<false, kGlu>(total[nt], v);
       const int c = (nt * TokensATile(kGlu)) + TokenOf<kGlu>(t4, 0);
       if (c < count) {
-        float* out = sums + (((__ldcg(&a.choice->pairs[begin + c]) * kParts) + part) * kTileRows);
+        float* out = sums + (((choice.pairs[begin + c] * kParts) + (item % kParts)) * kTileRows);
         out[g] = v[0][0];
         out[g + 8] = v[1][0];
       }
     }
   }
   __syncthreads();
-  for (int i = tid; i < a.tokens * kTileRows; i += kThreads) {
+  for (int i = tid; i < a.tokens * kTileRows; i += threads) {
     const int t = i / kTileRows, r = i % kTileRows, row = (tile * kTileRows) + r;
     if (row >= a.hidden) continue;
     float y = 0.0f;
@@ -486,19 +670,18 @@ cudaError_t Configure(Kernel kernel, int& configured_device, int smem) {
   return e;
 }
 
-constexpr int kFirstSmemLimit = 160 * 1024;
-
 template <int kType, int kGroups>
 int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   static thread_local int configured_device = -1;
   if (const cudaError_t e = Configure(FirstKernel<kType, kGroups>, configured_device, kFirstSmemLimit); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  const int smem = (a.cap * BfloatPieces(kType) * a.x_pitch) + (a.tokens * a.experts * 4);
+  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
-  const std::int64_t units = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) * a.tiles_up;
-  const std::int64_t most = std::max<std::int64_t>(1, static_cast<std::int64_t>(SmCount()) * 2 / kCluster);
-  const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (units + kCluster - 1) / kCluster));
+  const std::int64_t rounds = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) *
+                              ((a.tiles_up + kTilesARound - 1) / kTilesARound);
+  const std::int64_t most = std::max(1, SmCount() / kCluster);
+  const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + kCluster - 1) / kCluster));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(clusters * kCluster));
   config.blockDim = dim3(kThreads);
@@ -518,9 +701,15 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
 
 template <int kType, int kGroups>
 int LaunchSecond(const LayerArgs& a, cudaStream_t stream) {
-  const int smem = a.tokens * a.used * kParts * kTileRows * 4;
-  const cudaError_t e = LaunchPdl(SecondKernel<kType, kGroups>, dim3(static_cast<unsigned>(a.tiles_down)), dim3(kThreads),
-                                  static_cast<std::size_t>(smem), stream, a);
+  static thread_local int configured_device = -1;
+  if (const cudaError_t e = Configure(SecondKernel<kType, kGroups>, configured_device, 128 * 1024); e != cudaSuccess) {
+    return Failed(e, "moe_layer attribute");
+  }
+  // sixteen warps a tile while there are no more tiles than SMs, else eight, two CTAs an SM
+  const int warps = a.tiles_down <= SmCount() ? kSecondWarps : kSecondWarps / 2;
+  const int smem = (warps * kSlots * BlockBytes(kStep / kGroups)) + (a.tokens * a.used * kParts * kTileRows * 4);
+  const cudaError_t e = LaunchPdl(SecondKernel<kType, kGroups>, dim3(static_cast<unsigned>(a.tiles_down)),
+                                  dim3(static_cast<unsigned>(warps * 32)), static_cast<std::size_t>(smem), stream, a);
   return e == cudaSuccess ? 0 : Failed(e, "moe_layer down launch");
 }
 
@@ -598,7 +787,15 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.choice = static_cast<Choice*>(d.scratch);
   a.h = reinterpret_cast<unsigned short*>(static_cast<std::uint8_t*>(d.scratch) + ChoiceBytes());
   a.x_pitch = (a.steps_up * kStep * 2) + 64;
-  a.cap = std::max(1, std::min(d.tokens, kXBudget / (BfloatPieces(d.x_type) * a.x_pitch)));
+  a.parts = kWarps / kTilesARound;
+  while (a.parts > a.steps_up) a.parts /= 2;
+  a.block_down = BlockBytes(d.down.group);
+  a.prefetch_down = static_cast<double>(std::min(experts, d.tokens * d.used)) * a.tiles_down * a.steps_down * a.block_down <= 32e6;
+  a.cap = d.tokens;
+  while (a.cap > 1 && FirstLayout(BlockBytes(d.gate_up.group), a.cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes >
+                          kFirstSmemLimit) {
+    --a.cap;
+  }
   const auto s = static_cast<cudaStream_t>(stream);
   if (d.x_type == kF32) return LaunchLayer<kF32>(d.gate_up.group, d.down.group, a, s);
   if (d.x_type == kF16) return LaunchLayer<kF16>(d.gate_up.group, d.down.group, a, s);

@@ -119,12 +119,8 @@ __device__ __forceinline__ void Load8(const void* row, std::int64_t at, int vali
   }
 }
 // ... as bf16 pieces, a 16-byte quad a piece.
-template <int kType>
-__device__ __forceinline__ void LoadBfloat8(const void* row, std::int64_t at, int valid, bool vec,
-                                            uint4 (&quads)[BfloatPieces(kType)]) {
-  constexpr int kPieces = BfloatPieces(kType);
-  float v[8];
-  Load8<kType>(row, at, valid, vec, v);
+template <int kPieces>
+__device__ __forceinline__ void PackBfloat8(const float (&v)[8], uint4 (&quads)[kPieces]) {
   std::uint32_t packed[kPieces][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -136,6 +132,13 @@ __device__ __forceinline__ void LoadBfloat8(const void* row, std::int64_t at, in
   }
 #pragma unroll
   for (int s = 0; s < kPieces; ++s) quads[s] = make_uint4(packed[s][0], packed[s][1], packed[s][2], packed[s][3]);
+}
+template <int kType>
+__device__ __forceinline__ void LoadBfloat8(const void* row, std::int64_t at, int valid, bool vec,
+                                            uint4 (&quads)[BfloatPieces(kType)]) {
+  float v[8];
+  Load8<kType>(row, at, valid, vec, v);
+  PackBfloat8(v, quads);
 }
 // Eight F32 values times `scale` as two f16 pieces.
 __device__ __forceinline__ void LoadHalf8(const void* row, std::int64_t at, int valid, bool vec, float scale, uint4 (&quads)[2]) {
