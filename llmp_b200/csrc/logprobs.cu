@@ -6,6 +6,8 @@
 // x = logit / temperature, m the largest; S = sum e^(x - m), U = sum (x - m) e^(x - m), in F32:
 //   log p = x - m - log S,   entropy = log S - U / S   (two terms of one sign: nothing cancels)
 // Masked logits are -inf and add nothing.  Choices and ranks compare the logits themselves.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "w4.cuh"
@@ -13,121 +15,357 @@
 namespace llmp_b200 {
 namespace {
 
+namespace cg = cooperative_groups;
 using w4::LoadValue;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxGiven = 16, kMaxTop = 32;
+constexpr int kMaxRanks = 8;
+constexpr int kCandidates = 1024;
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+constexpr float kFar = -200.0f;  // 2^-200 is zero in F32
+
+__device__ __forceinline__ float MinusInf() { return __uint_as_float(0xff800000u); }
+__device__ __forceinline__ float Nan() { return __uint_as_float(0x7fc00000u); }
+// 2^x; below 2^-126 zero.
+__device__ __forceinline__ float Exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // (logit, lowest index first) as one unsigned number: NaN below -inf, the zeros alike.
-__device__ __forceinline__ unsigned long long Key(float v, int index) {
+using Key = unsigned long long;
+__device__ __forceinline__ Key KeyOf(float v, int index) {
   std::uint32_t k = 0;
   if (v == v) {
     const std::uint32_t b = __float_as_uint(v + 0.0f);
     k = (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
   }
-  return (static_cast<unsigned long long>(k) << 32) | (0xffffffffu - static_cast<std::uint32_t>(index));
+  return (static_cast<Key>(k) << 32) | (0xffffffffu - static_cast<std::uint32_t>(index));
 }
+__device__ __forceinline__ int IndexOf(Key k) { return static_cast<int>(0xffffffffu - static_cast<std::uint32_t>(k)); }
 
+// Over some logits, in units of 1 / c = T / log2 e: the largest, sum 2^d and sum d 2^d, d = (x - m) c.  m starts at the
+// lowest finite number, so a masked logit is 2^-inf = 0 whatever m is; a NaN or +inf makes s a NaN.
 struct Sums {
   float m, s, u;
-  bool bad;  // a NaN or +inf: no distribution
+  __device__ __forceinline__ void Rebase(float most, float c) {
+    const float d = (m - most) * c, f = Exp2(d);
+    u = d > kFar ? f * fmaf(d, s, u) : u * 0.0f;
+    s *= f;
+    m = most;
+  }
+  __device__ __forceinline__ void Join(Sums other, float c) {
+    const float most = fmaxf(m, other.m);
+    if (m != most) Rebase(most, c);
+    if (other.m != most) other.Rebase(most, c);
+    s += other.s, u += other.u;
+  }
 };
-__device__ __forceinline__ Sums Join(const Sums& a, const Sums& b, float scale) {
-  Sums r;
-  r.m = fmaxf(a.m, b.m);
-  r.bad = a.bad || b.bad;
-  const float da = a.m == r.m ? 0.0f : (a.m - r.m) * scale, db = b.m == r.m ? 0.0f : (b.m - r.m) * scale;
-  const float ea = expf(da), eb = expf(db);
-  r.s = (a.s * ea) + (b.s * eb);
-  // (x - m') e^(x - m') = e^(m - m') ((x - m) + (m - m')) e^(x - m); a side without weight adds nothing,
-  // however far below it lies (a mask of the type's lowest value)
-  r.u = (a.s * ea != 0.0f ? ea * fmaf(da, a.s, a.u) : 0.0f) + (b.s * eb != 0.0f ? eb * fmaf(db, b.s, b.u) : 0.0f);
-  return r;
-}
 
-__global__ void __launch_bounds__(kThreads)
+// A row as units of eight logits whose addresses are 16-byte aligned; the first and the last may begin before the
+// row or end behind it: those are read one by one, with -inf outside.
+template <int kType>
+struct Row {
+  const std::uint8_t* base;
+  int vocab, skew, units;  // skew: logits that unit 0 begins before the row
+  __device__ __forceinline__ Row(const void* logits, std::int64_t at, int vocab_) : vocab(vocab_) {
+    base = static_cast<const std::uint8_t*>(logits) + (at * w4::TypeBytes(kType));
+    skew = static_cast<int>((reinterpret_cast<std::uintptr_t>(base) & 15u) / w4::TypeBytes(kType));
+    units = (vocab + skew + 7) / 8;
+  }
+  __device__ __forceinline__ float At(int i) const { return LoadValue(base, i, kType); }
+  __device__ __forceinline__ int First(int unit) const { return (unit * 8) - skew; }
+  __device__ __forceinline__ void Load(int unit, float (&v)[8]) const {
+    const int first = First(unit);
+    w4::Load8<kType>(base, first, first >= 0 && first + 8 <= vocab ? 8 : 0, true, v);
+    if (first < 0 || first + 8 > vocab) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = first + i >= 0 && first + i < vocab ? At(first + i) : MinusInf();
+    }
+  }
+};
+
+struct Part {  // of a row, by one CTA
+  Sums sums;
+  int above[kMaxGiven];
+  int candidates;
+  Key top[kMaxTop];
+};
+
+// A row is divided among the CTAs of a cluster (one, where there are rows enough): one pass over the logits, kBatch
+// units of a thread in flight.  The top alternatives need no sort: the `top`-th largest of the maxima of 32 half warps
+// is a logit that at least `top` logits reach, so the few that reach it are collected by the threads whose own
+// maximum does (they look at their logits again, which L2 still holds), and a candidate's place is the number of
+// keys above its own.  Ranks are counted in the pass, the given logits being fetched before it.  Each CTA leaves its
+// sums, counts and best keys in shared memory; after one cluster barrier rank 0 joins them in rank order.
+template <int kType, int kGiven>
+__global__ void __launch_bounds__(kThreads, 2)
 LogprobsKernel(const llmp_b200_logprobs_desc a) {
-  __shared__ Sums sums[kThreads / 32];
-  __shared__ unsigned long long best[kThreads / 32];
-  __shared__ int counts[kMaxGiven];
+  constexpr int kBatch = kType == w4::kF32 ? 2 : 4;
+  __shared__ Sums warp_sums[kWarps];
+  __shared__ float maxima[32];
+  __shared__ int warp_above[kWarps][kGiven > 0 ? kGiven : 1];
+  __shared__ Key candidates[kCandidates];
+  __shared__ Key best[kWarps];
+  __shared__ Key merged[kMaxRanks * kMaxTop];
+  __shared__ Part part;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  const std::int64_t row_index = static_cast<std::int64_t>(blockIdx.x) / ranks;
+  const float c = kLog2E / a.temperature;
   GridLaunchDependents();
   GridDependencyWait();
-  const std::int64_t row = blockIdx.x;
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const std::int64_t base = row * a.stride;
-  const float scale = 1.0f / a.temperature;
-  const float kNan = __uint_as_float(0x7fc00000u), kMinusInf = __uint_as_float(0xff800000u);
-  auto logit = [&](int i) { return LoadValue(a.logits, base + i, a.type); };
-
-  Sums mine = {kMinusInf, 0.0f, 0.0f, false};
-  for (int i = tid; i < a.vocab; i += kThreads) {
-    const float x = logit(i);
-    if (x != x || x == -kMinusInf) mine.bad = true;
-    if (!(x > kMinusInf)) continue;
-    mine = Join(mine, Sums{x, 1.0f, 0.0f, false}, scale);
+  const Row<kType> row(a.logits, row_index * a.stride, a.vocab);
+  const int unit0 = static_cast<int>(static_cast<std::int64_t>(row.units) * rank / ranks);
+  const int unit1 = static_cast<int>(static_cast<std::int64_t>(row.units) * (rank + 1) / ranks);
+  float given[kGiven > 0 ? kGiven : 1];
+  int above[kGiven > 0 ? kGiven : 1];
+#pragma unroll
+  for (int j = 0; j < kGiven; ++j) {
+    above[j] = 0;
+    const int token = j < a.given ? a.tokens[(row_index * a.given) + j] : -1;
+    given[j] = token >= 0 && token < a.vocab ? row.At(token) : Nan();  // nothing is above a NaN
   }
+  if (tid == 0) part.candidates = 0;
+
+  Sums mine = {-3.402823466e38f, 0.0f, 0.0f};
+  float most = MinusInf();  // this thread's largest, of any number
+  for (int first = unit0 + tid; first < unit1; first += kBatch * kThreads) {
+    float v[kBatch][8];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int unit = first + (q * kThreads);
+      if (unit < unit1) {
+        row.Load(unit, v[q]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[q][i] = MinusInf();
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, v[q][i]);
+    }
+    if (most > mine.m) mine.Rebase(most, c);
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // (the difference first: the product of a large logit with c would lose the difference's last bits)
+        const float d = (v[q][i] - mine.m) * c, e = Exp2(d);
+        mine.s += e;
+        mine.u = fmaf(fmaxf(d, kFar), e, mine.u);
+#pragma unroll
+        for (int j = 0; j < kGiven; ++j) above[j] += v[q][i] > given[j] ? 1 : 0;
+      }
+    }
+  }
+
+  // ---- this CTA's sums and counts
+  Sums all = mine;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Sums other;
-    other.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
-    other.u = __shfl_xor_sync(0xffffffffu, mine.u, o);
-    other.bad = __shfl_xor_sync(0xffffffffu, mine.bad ? 1 : 0, o) != 0;
-    mine = Join(mine, other, scale);
+    other.m = __shfl_xor_sync(0xffffffffu, all.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, all.s, o);
+    other.u = __shfl_xor_sync(0xffffffffu, all.u, o);
+    all.Join(other, c);
   }
-  if (lane == 0) sums[warp] = mine;
-  if (tid < kMaxGiven) counts[tid] = 0;
-  __syncthreads();
-  Sums all = sums[0];
-  for (int w = 1; w < kThreads / 32; ++w) all = Join(all, sums[w], scale);
-  const float log_s = logf(all.s);
-  auto log_p = [&](float x) {
-    if (all.bad) return kNan;
-    if (x == kMinusInf) return kMinusInf;
-    return ((x - all.m) / a.temperature) - log_s;
-  };
-  if (tid == 0) a.entropy[row] = all.bad ? kNan : all.s == 0.0f ? 0.0f : log_s - (all.u / all.s);
-
-  for (int j = 0; j < a.given; ++j) {
-    const int token = a.tokens[(row * a.given) + j];
-    const bool inside = token >= 0 && token < a.vocab;
-    if (inside) {
-      const float x = logit(token);
-      int above = 0;
-      for (int i = tid; i < a.vocab; i += kThreads) above += logit(i) > x ? 1 : 0;
-      above = __reduce_add_sync(0xffffffffu, above);
-      if (lane == 0) atomicAdd(&counts[j], above);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      a.logprobs[(row * a.given) + j] = inside ? log_p(logit(token)) : kNan;
-      a.ranks[(row * a.given) + j] = inside ? counts[j] + 1 : 0;
-    }
-  }
-
-  unsigned long long below = ~0ull;
-  for (int n = 0; n < a.top; ++n) {
-    unsigned long long most = 0;
-    for (int i = tid; i < a.vocab; i += kThreads) {
-      const unsigned long long k = Key(logit(i), i);
-      if (k < below && k > most) most = k;
-    }
+  if (lane == 0) warp_sums[warp] = all;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, most, o);
-      most = other > most ? other : most;
-    }
-    __syncthreads();
-    if (lane == 0) best[warp] = most;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) most = best[w] > most ? best[w] : most;
-    below = most;
-    if (tid == 0) {
-      const int id = static_cast<int>(0xffffffffu - static_cast<std::uint32_t>(most));
-      a.top_ids[(row * a.top) + n] = id;
-      a.top_logprobs[(row * a.top) + n] = log_p(logit(id));
+  for (int j = 0; j < kGiven; ++j) {
+    const int sum = __reduce_add_sync(0xffffffffu, above[j]);
+    if (lane == 0) warp_above[warp][j] = sum;
+  }
+  if (a.top > 0) {
+    float half = most;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) half = fmaxf(half, __shfl_xor_sync(0xffffffffu, half, o));
+    if ((lane & 15) == 0) maxima[tid >> 4] = half;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    Sums sum = warp_sums[0];
+    for (int w = 1; w < kWarps; ++w) sum.Join(warp_sums[w], c);
+    if (lane == 0) part.sums = sum;
+    if constexpr (kGiven > 0) {
+      if (lane < kGiven) {
+        int count = 0;
+        for (int w = 0; w < kWarps; ++w) count += warp_above[w][lane];
+        part.above[lane] = count;
+      }
     }
   }
+
+  // ---- this CTA's best keys
+  if (a.top > 0) {
+    const int logits = min(unit1 * 8 - row.skew, a.vocab) - max(unit0 * 8 - row.skew, 0);
+    const int wanted = min(a.top, max(logits, 0));
+    float reach = MinusInf();  // at least `wanted` logits reach it
+    {
+      const float mine_max = maxima[lane];
+      int larger = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float other = maxima[i];
+        larger += other > mine_max || (other == mine_max && i < lane) ? 1 : 0;
+      }
+      const unsigned int which = __ballot_sync(0xffffffffu, larger == wanted - 1);
+      if (which != 0) reach = __shfl_sync(0xffffffffu, mine_max, __ffs(which) - 1);
+    }
+    // collected: the logits that reach it, or all above -inf (few logits, or few that are not masked)
+    if (most >= reach && most > MinusInf()) {
+      for (int unit = unit0 + tid; unit < unit1; unit += kThreads) {
+        float v[8];
+        row.Load(unit, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (v[i] >= reach && v[i] > MinusInf()) {
+            const int at = atomicAdd(&part.candidates, 1);
+            if (at < kCandidates) candidates[at] = KeyOf(v[i], row.First(unit) + i);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const int found = part.candidates;
+    if (found <= kCandidates) {
+      for (int i = tid; i < found; i += kThreads) {
+        const Key key = candidates[i];
+        int larger = 0;
+        for (int j = 0; j < found; ++j) larger += candidates[j] > key ? 1 : 0;
+        if (larger < wanted) part.top[larger] = key;
+      }
+      if (found < wanted && warp == 0) {  // the masked logits in order of their index, then the NaNs
+        int have = found;
+        const int begin = max(row.First(unit0), 0), end = min(row.First(unit1), a.vocab);
+        for (int nan = 0; nan < 2; ++nan) {
+          for (int first = begin; first < end && have < wanted; first += 32) {
+            const int i = first + lane;
+            const float x = i < end ? row.At(i) : 0.0f;
+            const bool takes = i < end && (nan == 0 ? x == MinusInf() : x != x);
+            const unsigned int takers = __ballot_sync(0xffffffffu, takes);
+            const int place = have + __popc(takers & ((1u << lane) - 1u));
+            if (takes && place < wanted) part.top[place] = KeyOf(x, i);
+            have += __popc(takers);
+          }
+        }
+      }
+    } else {
+      // more of one value than there is room for: one key at a time, each pass the largest below the one before
+      Key below = ~0ull;
+      for (int n = 0; n < wanted; ++n) {
+        Key largest = 0;
+        for (int unit = unit0 + tid; unit < unit1; unit += kThreads) {
+          float v[8];
+          row.Load(unit, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int at = row.First(unit) + i;
+            const Key key = KeyOf(v[i], at);
+            if (at >= 0 && at < a.vocab && key < below && key > largest) largest = key;
+          }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          const Key other = __shfl_xor_sync(0xffffffffu, largest, o);
+          largest = other > largest ? other : largest;
+        }
+        __syncthreads();
+        if (lane == 0) best[warp] = largest;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) largest = best[w] > largest ? best[w] : largest;
+        below = largest;
+        if (tid == 0) part.top[n] = largest;
+      }
+    }
+    __syncthreads();
+    if (tid == 0) part.candidates = wanted;
+  }
+  if (ranks > 1) cluster.sync(); else __syncthreads();
+
+  // ---- rank 0: the parts in rank order
+  if (rank == 0) {
+    auto of = [&](int r) { return ranks > 1 ? cluster.map_shared_rank(&part, r) : &part; };
+    Sums sum = of(0)->sums;
+    for (int r = 1; r < ranks; ++r) sum.Join(of(r)->sums, c);
+    const bool bad = sum.s != sum.s, nothing = sum.s == 0.0f;
+    const float log_s = logf(sum.s);
+    auto log_p = [&](float x) {
+      if (bad) return Nan();
+      if (nothing || x == MinusInf()) return MinusInf();
+      return ((x - sum.m) / a.temperature) - log_s;
+    };
+    if (tid == 0) a.entropy[row_index] = bad ? Nan() : nothing ? 0.0f : log_s - (kLn2 * (sum.u / sum.s));
+    if (tid < a.given) {
+      const std::int64_t at = (row_index * a.given) + tid;
+      const int token = a.tokens[at];
+      const bool inside = token >= 0 && token < a.vocab;
+      int count = 1;
+      for (int r = 0; r < ranks; ++r) count += of(r)->above[tid];
+      a.logprobs[at] = inside ? log_p(row.At(token)) : Nan();
+      a.ranks[at] = inside ? count : 0;
+    }
+    if (a.top > 0) {
+      // keys of all parts; a place is the number of larger ones
+      int before = 0, total = 0;
+      for (int r = 0; r < ranks; ++r) {
+        const int count = of(r)->candidates;
+        if (tid >= total && tid < total + count) before = r;
+        total += count;
+      }
+      if (tid < total) {
+        int start = 0;
+        for (int r = 0; r < before; ++r) start += of(r)->candidates;
+        merged[tid] = of(before)->top[tid - start];
+      }
+      __syncthreads();
+      if (tid < total) {
+        const Key key = merged[tid];
+        int larger = 0;
+        for (int j = 0; j < total; ++j) larger += merged[j] > key ? 1 : 0;
+        if (larger < a.top) {
+          const int id = IndexOf(key);
+          a.top_ids[(row_index * a.top) + larger] = id;
+          a.top_logprobs[(row_index * a.top) + larger] = log_p(row.At(id));
+        }
+      }
+    }
+  }
+  if (ranks > 1) cluster.sync();  // nobody leaves while rank 0 reads its part
+}
+
+template <int kType, int kGiven>
+int LaunchGiven(const llmp_b200_logprobs_desc& a, int ranks, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(a.rows * ranks));
+  config.blockDim = dim3(kThreads);
+  config.stream = stream;
+  cudaLaunchAttribute attribute[2];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  attribute[1].id = cudaLaunchAttributeClusterDimension;
+  attribute[1].val.clusterDim.x = static_cast<unsigned>(ranks);
+  attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
+  config.attrs = attribute;
+  config.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&config, LogprobsKernel<kType, kGiven>, a);
+  return e == cudaSuccess ? 0 : Failed(e, "logprobs launch");
+}
+
+template <int kType>
+int LaunchType(const llmp_b200_logprobs_desc& a, cudaStream_t stream) {
+  // CTAs a row: while they do not fill the device twice over and have 4096 logits each
+  int ranks = 1;
+  while (ranks < kMaxRanks && a.rows * ranks < 2 * SmCount() && a.vocab / (2 * ranks) >= 4096) ranks *= 2;
+  if (a.given == 0) return LaunchGiven<kType, 0>(a, ranks, stream);
+  if (a.given == 1) return LaunchGiven<kType, 1>(a, ranks, stream);
+  if (a.given <= 4) return LaunchGiven<kType, 4>(a, ranks, stream);
+  return LaunchGiven<kType, 16>(a, ranks, stream);
 }
 
 }  // namespace
@@ -139,7 +377,7 @@ extern "C" int llmp_b200_logprobs(const llmp_b200_logprobs_desc* desc, void* str
   const llmp_b200_logprobs_desc& a = *desc;
   if (!w4::FloatType(a.type)) return Reject("logprobs: F32, F16 or BF16 logits");
   if (a.vocab < 1 || a.vocab > (1 << 24)) return Reject("logprobs: rows of 1 to 2^24 logits");
-  if (a.rows < 0 || a.rows > 0x7fffffffLL) return Reject("logprobs: 0 to 2^31 - 1 rows");
+  if (a.rows < 0 || a.rows > 0x0fffffffLL) return Reject("logprobs: 0 to 2^28 - 1 rows");
   if (a.given < 0 || a.given > kMaxGiven || a.top < 0 || a.top > kMaxTop || a.top > a.vocab) {
     return Reject("logprobs: up to 16 given tokens a row and up to 32 alternatives, no more than there are logits");
   }
@@ -155,7 +393,8 @@ extern "C" int llmp_b200_logprobs(const llmp_b200_logprobs_desc* desc, void* str
     return Reject("logprobs: operands aligned to their elements, no negative stride");
   }
   if (const int status = DeviceStatus(); status != 0) return status;
-  const cudaError_t e = LaunchPdl(LogprobsKernel, dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0,
-                                  static_cast<cudaStream_t>(stream), a);
-  return e == cudaSuccess ? 0 : Failed(e, "logprobs launch");
+  const auto s = static_cast<cudaStream_t>(stream);
+  if (a.type == w4::kF32) return LaunchType<w4::kF32>(a, s);
+  if (a.type == w4::kF16) return LaunchType<w4::kF16>(a, s);
+  return LaunchType<w4::kBF16>(a, s);
 }
