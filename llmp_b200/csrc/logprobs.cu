@@ -18,7 +18,7 @@ namespace {
 namespace cg = cooperative_groups;
 using w4::LoadValue;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kFewRows = 512, kManyRows = 128;  // threads a CTA
 constexpr int kMaxGiven = 16, kMaxTop = 32;
 constexpr int kMaxRanks = 8;
 constexpr int kCandidates = 1024;
@@ -70,13 +70,56 @@ template <int kType>
 struct Row {
   const std::uint8_t* base;
   int vocab, skew, units;  // skew: logits that unit 0 begins before the row
+  int whole0, whole1;      // the units that lie inside the row
   __device__ __forceinline__ Row(const void* logits, std::int64_t at, int vocab_) : vocab(vocab_) {
     base = static_cast<const std::uint8_t*>(logits) + (at * w4::TypeBytes(kType));
     skew = static_cast<int>((reinterpret_cast<std::uintptr_t>(base) & 15u) / w4::TypeBytes(kType));
     units = (vocab + skew + 7) / 8;
+    whole0 = skew > 0 ? 1 : 0;
+    whole1 = (vocab + skew) / 8;
   }
   __device__ __forceinline__ float At(int i) const { return LoadValue(base, i, kType); }
   __device__ __forceinline__ int First(int unit) const { return (unit * 8) - skew; }
+  static constexpr int kQuads = kType == w4::kF32 ? 2 : 1;
+  __device__ __forceinline__ void LoadWhole(int unit, uint4 (&raw)[kQuads]) const {
+    const auto* p = reinterpret_cast<const uint4*>(base + (static_cast<std::int64_t>(First(unit)) * w4::TypeBytes(kType)));
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) raw[i] = p[i];
+  }
+  static __device__ __forceinline__ void Expand(const uint4 (&raw)[kQuads], float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const std::uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (kType == w4::kF32) {
+          v[(4 * i) + j] = __uint_as_float(w[j]);
+        } else if constexpr (kType == w4::kBF16) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[(2 * j) + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+          v[2 * j] = HalfBitsToFloat(w[j] & 0xffffu);
+          v[(2 * j) + 1] = HalfBitsToFloat(w[j] >> 16);
+        }
+      }
+    }
+  }
+  // The largest of a unit that is a number (16-bit ones two at a time); NaN where none is.
+  static __device__ __forceinline__ float Largest(const uint4 (&raw)[kQuads]) {
+    if constexpr (kType == w4::kF32) {
+      float v[8];
+      Expand(raw, v);
+      return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    } else if constexpr (kType == w4::kBF16) {
+      const auto* p = reinterpret_cast<const __nv_bfloat162*>(&raw[0]);
+      const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      const auto* p = reinterpret_cast<const __half2*>(&raw[0]);
+      const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
   __device__ __forceinline__ void Load(int unit, float (&v)[8]) const {
     const int first = First(unit);
     w4::Load8<kType>(base, first, first >= 0 && first + 8 <= vocab ? 8 : 0, true, v);
@@ -95,14 +138,15 @@ struct Part {  // of a row, by one CTA
 };
 
 // A row is divided among the CTAs of a cluster (one, where there are rows enough): one pass over the logits, kBatch
-// units of a thread in flight.  The top alternatives need no sort: the `top`-th largest of the maxima of 32 half warps
+// units of a thread in flight.  The top alternatives need no sort: the `top`-th largest of the maxima of 32 groups of threads
 // is a logit that at least `top` logits reach, so the few that reach it are collected by the threads whose own
 // maximum does (they look at their logits again, which L2 still holds), and a candidate's place is the number of
 // keys above its own.  Ranks are counted in the pass, the given logits being fetched before it.  Each CTA leaves its
 // sums, counts and best keys in shared memory; after one cluster barrier rank 0 joins them in rank order.
-template <int kType, int kGiven>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int kType, int kGiven, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 LogprobsKernel(const llmp_b200_logprobs_desc a) {
+  constexpr int kWarps = kThreads / 32, kGroup = kThreads / 32;  // threads whose maximum is one of 32
   constexpr int kBatch = kType == w4::kF32 ? 2 : 4;
   __shared__ Sums warp_sums[kWarps];
   __shared__ float maxima[32];
@@ -133,36 +177,51 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
 
   Sums mine = {-3.402823466e38f, 0.0f, 0.0f};
   float most = MinusInf();  // this thread's largest, of any number
-  for (int first = unit0 + tid; first < unit1; first += kBatch * kThreads) {
-    float v[kBatch][8];
+  auto take = [&](const float (&v)[8]) {
 #pragma unroll
-    for (int q = 0; q < kBatch; ++q) {
-      const int unit = first + (q * kThreads);
-      if (unit < unit1) {
-        row.Load(unit, v[q]);
-      } else {
+    for (int i = 0; i < 8; ++i) {
+      // (the difference first: the product of a large logit with c would lose the difference's last bits)
+      const float d = (v[i] - mine.m) * c, e = Exp2(d);
+      mine.s += e;
+      mine.u = fmaf(fmaxf(d, kFar), e, mine.u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[q][i] = MinusInf();
-      }
+      for (int j = 0; j < kGiven; ++j) above[j] += v[i] > given[j] ? 1 : 0;
     }
+  };
+  const int first_whole = max(unit0, row.whole0), end_whole = min(unit1, row.whole1);
+  int unit = first_whole + tid;
+  for (; unit + ((kBatch - 1) * kThreads) < end_whole; unit += kBatch * kThreads) {
+    uint4 raw[kBatch][kType == w4::kF32 ? 2 : 1];
 #pragma unroll
-    for (int q = 0; q < kBatch; ++q) {
+    for (int q = 0; q < kBatch; ++q) row.LoadWhole(unit + (q * kThreads), raw[q]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) most = fmaxf(most, v[q][i]);
-    }
+    for (int q = 0; q < kBatch; ++q) most = fmaxf(most, Row<kType>::Largest(raw[q]));
     if (most > mine.m) mine.Rebase(most, c);
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // (the difference first: the product of a large logit with c would lose the difference's last bits)
-        const float d = (v[q][i] - mine.m) * c, e = Exp2(d);
-        mine.s += e;
-        mine.u = fmaf(fmaxf(d, kFar), e, mine.u);
-#pragma unroll
-        for (int j = 0; j < kGiven; ++j) above[j] += v[q][i] > given[j] ? 1 : 0;
-      }
+      float v[8];
+      Row<kType>::Expand(raw[q], v);
+      take(v);
     }
+  }
+  for (; unit < end_whole; unit += kThreads) {
+    uint4 raw[kType == w4::kF32 ? 2 : 1];
+    row.LoadWhole(unit, raw);
+    most = fmaxf(most, Row<kType>::Largest(raw));
+    if (most > mine.m) mine.Rebase(most, c);
+    float v[8];
+    Row<kType>::Expand(raw, v);
+    take(v);
+  }
+  // the units that reach over an end of the row, by two threads
+  const int edge = tid == 0 && unit0 < row.whole0 ? 0 : tid == 32 && unit1 > row.whole1 && row.whole1 >= row.whole0 ? row.whole1 : -1;
+  if (edge >= unit0 && edge < unit1) {
+    float v[8];
+    row.Load(edge, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaxf(most, v[i]);
+    if (most > mine.m) mine.Rebase(most, c);
+    take(v);
   }
 
   // ---- this CTA's sums and counts
@@ -182,10 +241,10 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
     if (lane == 0) warp_above[warp][j] = sum;
   }
   if (a.top > 0) {
-    float half = most;
+    float group = most;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) half = fmaxf(half, __shfl_xor_sync(0xffffffffu, half, o));
-    if ((lane & 15) == 0) maxima[tid >> 4] = half;
+    for (int o = kGroup / 2; o > 0; o >>= 1) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, o));
+    if (tid % kGroup == 0) maxima[tid / kGroup] = group;
   }
   __syncthreads();
   if (warp == 0) {
@@ -217,19 +276,25 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
       const unsigned int which = __ballot_sync(0xffffffffu, larger == wanted - 1);
       if (which != 0) reach = __shfl_sync(0xffffffffu, mine_max, __ffs(which) - 1);
     }
-    // collected: the logits that reach it, or all above -inf (few logits, or few that are not masked)
-    if (most >= reach && most > MinusInf()) {
-      for (int unit = unit0 + tid; unit < unit1; unit += kThreads) {
+    // collected: the logits that reach it, or all above -inf (few logits, or few that are not masked); a warp goes over
+    // the logits of each of its threads whose maximum does
+    for (unsigned int flagged = __ballot_sync(0xffffffffu, most >= reach && most > MinusInf()); flagged != 0; flagged &= flagged - 1) {
+      const int owner = (warp * 32) + __ffs(flagged) - 1;
+      auto collect = [&](int at) {
         float v[8];
-        row.Load(unit, v);
+        row.Load(at, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if (v[i] >= reach && v[i] > MinusInf()) {
-            const int at = atomicAdd(&part.candidates, 1);
-            if (at < kCandidates) candidates[at] = KeyOf(v[i], row.First(unit) + i);
+            const int place = atomicAdd(&part.candidates, 1);
+            if (place < kCandidates) candidates[place] = KeyOf(v[i], row.First(at) + i);
           }
         }
-      }
+      };
+      for (int at = first_whole + owner + (lane * kThreads); at < end_whole; at += 32 * kThreads) collect(at);
+      const int owned_edge = owner == 0 && unit0 < row.whole0 ? 0
+                             : owner == 32 && unit1 > row.whole1 && row.whole1 >= row.whole0 ? row.whole1 : -1;
+      if (lane == 0 && owned_edge >= unit0 && owned_edge < unit1) collect(owned_edge);
     }
     __syncthreads();
     const int found = part.candidates;
@@ -312,20 +377,16 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
     }
     if (a.top > 0) {
       // keys of all parts; a place is the number of larger ones
-      int before = 0, total = 0;
-      for (int r = 0; r < ranks; ++r) {
-        const int count = of(r)->candidates;
-        if (tid >= total && tid < total + count) before = r;
-        total += count;
-      }
-      if (tid < total) {
-        int start = 0;
-        for (int r = 0; r < before; ++r) start += of(r)->candidates;
-        merged[tid] = of(before)->top[tid - start];
+      int total = 0;
+      for (int r = 0; r < ranks; ++r) total += of(r)->candidates;
+      for (int i = tid; i < total; i += kThreads) {
+        int r = 0, start = 0;
+        while (i >= start + of(r)->candidates) start += of(r)->candidates, ++r;
+        merged[i] = of(r)->top[i - start];
       }
       __syncthreads();
-      if (tid < total) {
-        const Key key = merged[tid];
+      for (int i = tid; i < total; i += kThreads) {
+        const Key key = merged[i];
         int larger = 0;
         for (int j = 0; j < total; ++j) larger += merged[j] > key ? 1 : 0;
         if (larger < a.top) {
@@ -339,8 +400,8 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
   if (ranks > 1) cluster.sync();  // nobody leaves while rank 0 reads its part
 }
 
-template <int kType, int kGiven>
-int LaunchGiven(const llmp_b200_logprobs_desc& a, int ranks, cudaStream_t stream) {
+template <int kType, int kGiven, int kThreads>
+int LaunchThreads(const llmp_b200_logprobs_desc& a, int ranks, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(a.rows * ranks));
   config.blockDim = dim3(kThreads);
@@ -353,19 +414,27 @@ int LaunchGiven(const llmp_b200_logprobs_desc& a, int ranks, cudaStream_t stream
   attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&config, LogprobsKernel<kType, kGiven>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&config, LogprobsKernel<kType, kGiven, kThreads>, a);
   return e == cudaSuccess ? 0 : Failed(e, "logprobs launch");
+}
+
+template <int kType, int kGiven>
+int LaunchGiven(const llmp_b200_logprobs_desc& a, cudaStream_t stream) {
+  // Many rows: a small CTA each, eight an SM, so that one row's short steps between its barriers run beside another's
+  // pass (2048 rows of 32003 bf16 logits: 109 us with 512 threads a row).  Few: as many CTAs a row as fill the
+  // device twice over, with 4096 logits each.
+  if (a.rows >= 4 * SmCount()) return LaunchThreads<kType, kGiven, kManyRows>(a, 1, stream);
+  int ranks = 1;
+  while (ranks < kMaxRanks && a.rows * ranks < 2 * SmCount() && a.vocab / (2 * ranks) >= 4096) ranks *= 2;
+  return LaunchThreads<kType, kGiven, kFewRows>(a, ranks, stream);
 }
 
 template <int kType>
 int LaunchType(const llmp_b200_logprobs_desc& a, cudaStream_t stream) {
-  // CTAs a row: while they do not fill the device twice over and have 4096 logits each
-  int ranks = 1;
-  while (ranks < kMaxRanks && a.rows * ranks < 2 * SmCount() && a.vocab / (2 * ranks) >= 4096) ranks *= 2;
-  if (a.given == 0) return LaunchGiven<kType, 0>(a, ranks, stream);
-  if (a.given == 1) return LaunchGiven<kType, 1>(a, ranks, stream);
-  if (a.given <= 4) return LaunchGiven<kType, 4>(a, ranks, stream);
-  return LaunchGiven<kType, 16>(a, ranks, stream);
+  if (a.given == 0) return LaunchGiven<kType, 0>(a, stream);
+  if (a.given == 1) return LaunchGiven<kType, 1>(a, stream);
+  if (a.given <= 4) return LaunchGiven<kType, 4>(a, stream);
+  return LaunchGiven<kType, 16>(a, stream);
 }
 
 }  // namespace
