@@ -44,6 +44,10 @@ __device__ __forceinline__ Key KeyOf(float v, int index) {
   }
   return (static_cast<Key>(k) << 32) | (0xffffffffu - static_cast<std::uint32_t>(index));
 }
+__device__ __forceinline__ float ValueOf(Key k) {
+  const std::uint32_t b = static_cast<std::uint32_t>(k >> 32);
+  return b == 0 ? Nan() : __uint_as_float((b & 0x80000000u) != 0 ? b & 0x7fffffffu : ~b);
+}
 __device__ __forceinline__ int IndexOf(Key k) { return static_cast<int>(0xffffffffu - static_cast<std::uint32_t>(k)); }
 
 // Over some logits, in units of 1 / c = T / log2 e: the largest, sum 2^d and sum d 2^d, d = (x - m) c.  m starts at the
@@ -56,11 +60,18 @@ struct Sums {
     s *= f;
     m = most;
   }
-  __device__ __forceinline__ void Join(Sums other, float c) {
-    const float most = fmaxf(m, other.m);
+  // All lanes' sums: the largest first, one change of base, then plain sums in a fixed order.
+  template <int kLanes>
+  __device__ __forceinline__ void JoinLanes(float c) {
+    float most = m;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (m != most) Rebase(most, c);
-    if (other.m != most) other.Rebase(most, c);
-    s += other.s, u += other.u;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
   }
 };
 
@@ -141,8 +152,8 @@ struct Part {  // of a row, by one CTA
 // units of a thread in flight.  The top alternatives need no sort: the `top`-th largest of the maxima of 32 groups of threads
 // is a logit that at least `top` logits reach, so the few that reach it are collected by the threads whose own
 // maximum does (they look at their logits again, which L2 still holds), and a candidate's place is the number of
-// keys above its own.  Ranks are counted in the pass, the given logits being fetched before it.  Each CTA leaves its
-// sums, counts and best keys in shared memory; after one cluster barrier rank 0 joins them in rank order.
+// keys above its own.  Ranks are counted in the pass, the given logits being fetched before it.  Each CTA stores its
+// sums, counts and best keys into rank 0's shared memory, which joins them in rank order after one cluster barrier.
 template <int kType, int kGiven, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 LogprobsKernel(const llmp_b200_logprobs_desc a) {
@@ -154,7 +165,9 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
   __shared__ Key candidates[kCandidates];
   __shared__ Key best[kWarps];
   __shared__ Key merged[kMaxRanks * kMaxTop];
-  __shared__ Part part;
+  __shared__ Part part, parts[kMaxRanks];
+  __shared__ float given_logit[kMaxGiven];
+  __shared__ int given_token[kMaxGiven];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
@@ -165,13 +178,24 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
   const Row<kType> row(a.logits, row_index * a.stride, a.vocab);
   const int unit0 = static_cast<int>(static_cast<std::int64_t>(row.units) * rank / ranks);
   const int unit1 = static_cast<int>(static_cast<std::int64_t>(row.units) * (rank + 1) / ranks);
+  if (ranks > 1) cluster.barrier_arrive();  // this CTA has begun: its shared memory may be written
+  for (int i = 0; i < kBatch; ++i) {  // on their way while the given logits are looked up
+    const int ahead = unit0 + tid + (i * kThreads);
+    if (ahead < unit1 && ahead >= row.whole0) {
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(row.base + (static_cast<std::int64_t>(row.First(ahead)) * w4::TypeBytes(kType))));
+    }
+  }
   float given[kGiven > 0 ? kGiven : 1];
   int above[kGiven > 0 ? kGiven : 1];
+  if constexpr (kGiven > 0) {
+    if (tid < kGiven) {
+      const int token = tid < a.given ? a.tokens[(row_index * a.given) + tid] : -1;
+      given_token[tid] = token;
+      given_logit[tid] = token >= 0 && token < a.vocab ? row.At(token) : Nan();  // nothing is above a NaN
+    }
+    __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kGiven; ++j) {
-    above[j] = 0;
-    const int token = j < a.given ? a.tokens[(row_index * a.given) + j] : -1;
-    given[j] = token >= 0 && token < a.vocab ? row.At(token) : Nan();  // nothing is above a NaN
+    for (int j = 0; j < kGiven; ++j) above[j] = 0, given[j] = given_logit[j];
   }
   if (tid == 0) part.candidates = 0;
 
@@ -225,16 +249,8 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
   }
 
   // ---- this CTA's sums and counts
-  Sums all = mine;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Sums other;
-    other.m = __shfl_xor_sync(0xffffffffu, all.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, all.s, o);
-    other.u = __shfl_xor_sync(0xffffffffu, all.u, o);
-    all.Join(other, c);
-  }
-  if (lane == 0) warp_sums[warp] = all;
+  mine.JoinLanes<32>(c);
+  if (lane == 0) warp_sums[warp] = mine;
 #pragma unroll
   for (int j = 0; j < kGiven; ++j) {
     const int sum = __reduce_add_sync(0xffffffffu, above[j]);
@@ -248,8 +264,8 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
   }
   __syncthreads();
   if (warp == 0) {
-    Sums sum = warp_sums[0];
-    for (int w = 1; w < kWarps; ++w) sum.Join(warp_sums[w], c);
+    Sums sum = warp_sums[lane % kWarps];
+    sum.JoinLanes<kWarps>(c);
     if (lane == 0) part.sums = sum;
     if constexpr (kGiven > 0) {
       if (lane < kGiven) {
@@ -276,25 +292,29 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
       const unsigned int which = __ballot_sync(0xffffffffu, larger == wanted - 1);
       if (which != 0) reach = __shfl_sync(0xffffffffu, mine_max, __ffs(which) - 1);
     }
-    // collected: the logits that reach it, or all above -inf (few logits, or few that are not masked); a warp goes over
-    // the logits of each of its threads whose maximum does
-    for (unsigned int flagged = __ballot_sync(0xffffffffu, most >= reach && most > MinusInf()); flagged != 0; flagged &= flagged - 1) {
-      const int owner = (warp * 32) + __ffs(flagged) - 1;
-      auto collect = [&](int at) {
-        float v[8];
-        row.Load(at, v);
+    // collected: the logits that reach it, or all above -inf (few logits, or few that are not masked)
+    auto collect = [&](int at) {
+      float v[8];
+      row.Load(at, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (v[i] >= reach && v[i] > MinusInf()) {
-            const int place = atomicAdd(&part.candidates, 1);
-            if (place < kCandidates) candidates[place] = KeyOf(v[i], row.First(at) + i);
-          }
+      for (int i = 0; i < 8; ++i) {
+        if (v[i] >= reach && v[i] > MinusInf()) {
+          const int place = atomicAdd(&part.candidates, 1);
+          if (place < kCandidates) candidates[place] = KeyOf(v[i], row.First(at) + i);
         }
-      };
-      for (int at = first_whole + owner + (lane * kThreads); at < end_whole; at += 32 * kThreads) collect(at);
-      const int owned_edge = owner == 0 && unit0 < row.whole0 ? 0
-                             : owner == 32 && unit1 > row.whole1 && row.whole1 >= row.whole0 ? row.whole1 : -1;
-      if (lane == 0 && owned_edge >= unit0 && owned_edge < unit1) collect(owned_edge);
+      }
+    };
+    const bool flagged_me = most >= reach && most > MinusInf();
+    if (flagged_me && edge >= unit0 && edge < unit1) collect(edge);
+    if (end_whole - first_whole <= 2 * kThreads) {  // a thread's own one or two units
+      if (flagged_me) {
+        for (int at = first_whole + tid; at < end_whole; at += kThreads) collect(at);
+      }
+    } else {  // a warp goes over the units of each of its threads whose maximum does
+      for (unsigned int flagged = __ballot_sync(0xffffffffu, flagged_me); flagged != 0; flagged &= flagged - 1) {
+        const int owner = (warp * 32) + __ffs(flagged) - 1;
+        for (int at = first_whole + owner + (lane * kThreads); at < end_whole; at += 32 * kThreads) collect(at);
+      }
     }
     __syncthreads();
     const int found = part.candidates;
@@ -351,53 +371,60 @@ LogprobsKernel(const llmp_b200_logprobs_desc a) {
     __syncthreads();
     if (tid == 0) part.candidates = wanted;
   }
-  if (ranks > 1) cluster.sync(); else __syncthreads();
+  __syncthreads();
+  const Part* joined = &part;
+  if (ranks > 1) {
+    cluster.barrier_wait();
+    constexpr int kWords = sizeof(Part) / 4;
+    auto* to = reinterpret_cast<std::uint32_t*>(cluster.map_shared_rank(&parts[rank], 0));
+    for (int i = tid; i < kWords; i += kThreads) to[i] = reinterpret_cast<const std::uint32_t*>(&part)[i];
+    cluster.sync();
+    joined = parts;
+  }
+  if (rank != 0) return;
 
   // ---- rank 0: the parts in rank order
-  if (rank == 0) {
-    auto of = [&](int r) { return ranks > 1 ? cluster.map_shared_rank(&part, r) : &part; };
-    Sums sum = of(0)->sums;
-    for (int r = 1; r < ranks; ++r) sum.Join(of(r)->sums, c);
-    const bool bad = sum.s != sum.s, nothing = sum.s == 0.0f;
-    const float log_s = logf(sum.s);
-    auto log_p = [&](float x) {
-      if (bad) return Nan();
-      if (nothing || x == MinusInf()) return MinusInf();
-      return ((x - sum.m) / a.temperature) - log_s;
-    };
-    if (tid == 0) a.entropy[row_index] = bad ? Nan() : nothing ? 0.0f : log_s - (kLn2 * (sum.u / sum.s));
+  Sums sum = joined[lane % ranks].sums;  // (ranks is a power of two; every warp for itself)
+  if (ranks == 2) sum.JoinLanes<2>(c);
+  if (ranks == 4) sum.JoinLanes<4>(c);
+  if (ranks == 8) sum.JoinLanes<8>(c);
+  const bool bad = sum.s != sum.s, nothing = sum.s == 0.0f;
+  const float log_s = logf(sum.s);
+  auto log_p = [&](float x) {
+    if (bad) return Nan();
+    if (nothing || x == MinusInf()) return MinusInf();
+    return ((x - sum.m) / a.temperature) - log_s;
+  };
+  if (tid == 0) a.entropy[row_index] = bad ? Nan() : nothing ? 0.0f : log_s - (kLn2 * (sum.u / sum.s));
+  if constexpr (kGiven > 0) {
     if (tid < a.given) {
-      const std::int64_t at = (row_index * a.given) + tid;
-      const int token = a.tokens[at];
-      const bool inside = token >= 0 && token < a.vocab;
+      const bool inside = given_token[tid] >= 0 && given_token[tid] < a.vocab;
       int count = 1;
-      for (int r = 0; r < ranks; ++r) count += of(r)->above[tid];
-      a.logprobs[at] = inside ? log_p(row.At(token)) : Nan();
-      a.ranks[at] = inside ? count : 0;
+      for (int r = 0; r < ranks; ++r) count += joined[r].above[tid];
+      a.logprobs[(row_index * a.given) + tid] = inside ? log_p(given_logit[tid]) : Nan();
+      a.ranks[(row_index * a.given) + tid] = inside ? count : 0;
     }
-    if (a.top > 0) {
-      // keys of all parts; a place is the number of larger ones
-      int total = 0;
-      for (int r = 0; r < ranks; ++r) total += of(r)->candidates;
-      for (int i = tid; i < total; i += kThreads) {
-        int r = 0, start = 0;
-        while (i >= start + of(r)->candidates) start += of(r)->candidates, ++r;
-        merged[i] = of(r)->top[i - start];
-      }
-      __syncthreads();
-      for (int i = tid; i < total; i += kThreads) {
-        const Key key = merged[i];
-        int larger = 0;
-        for (int j = 0; j < total; ++j) larger += merged[j] > key ? 1 : 0;
-        if (larger < a.top) {
-          const int id = IndexOf(key);
-          a.top_ids[(row_index * a.top) + larger] = id;
-          a.top_logprobs[(row_index * a.top) + larger] = log_p(row.At(id));
-        }
+  }
+  if (a.top > 0) {
+    // keys of all parts; a place is the number of larger ones
+    int total = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const int count = joined[r].candidates;
+      for (int i = tid; i < count; i += kThreads) merged[total + i] = joined[r].top[i];
+      total += count;
+    }
+    __syncthreads();
+    for (int i = tid; i < total; i += kThreads) {
+      const Key key = merged[i];
+      int larger = 0;
+#pragma unroll 8
+      for (int j = 0; j < total; ++j) larger += merged[j] > key ? 1 : 0;
+      if (larger < a.top) {
+        a.top_ids[(row_index * a.top) + larger] = IndexOf(key);
+        a.top_logprobs[(row_index * a.top) + larger] = log_p(ValueOf(key));
       }
     }
   }
-  if (ranks > 1) cluster.sync();  // nobody leaves while rank 0 reads its part
 }
 
 template <int kType, int kGiven, int kThreads>
