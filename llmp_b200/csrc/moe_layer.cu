@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "w4.cuh"
 
@@ -25,16 +26,16 @@ using namespace w4;
 constexpr int kWarps = 16, kReducers = 2;          // of the first kernel: that multiply, that add up
 constexpr int kThreads = (kWarps + kReducers) * 32;
 constexpr int kSlots = 4;                          // steps a warp's ring holds
-constexpr int kTilesARound = 2;                    // each divided among kWarps / 2 warps
 constexpr int kCluster = 8;
 constexpr int kMaxTokens = 16, kMaxUsed = 16, kMaxExperts = 512;
 constexpr int kMaxPairs = kMaxTokens * kMaxUsed;
 constexpr int kFirstSmemLimit = 196 * 1024;        // dynamic; the choice's lists are static
 
-// The choice as the first kernel leaves it for the second: the named experts in ascending order, expert
-// i's (token, slot) pairs (t * used + j, in token order) being pairs[first[i]] .. pairs[first[i + 1] - 1].
+// The choice as the first kernel leaves it for the second: groups of tokens that name one expert, experts in ascending
+// order, a group's (token, slot) pairs (t * used + j, in token order) being pairs[first[i]] .. pairs[first[i + 1] - 1].
+// A group holds no more tokens than GroupTokens: an expert that more name has several, whose weights come from L2 again.
 struct Choice {
-  std::int32_t named;
+  std::int32_t groups;
   std::int32_t expert[kMaxPairs], first[kMaxPairs + 1], pairs[kMaxPairs];
 };
 
@@ -62,12 +63,17 @@ struct LayerArgs {
   Choice* choice;
   unsigned short* h;  // bf16 pieces of the GLU rows: [pair][piece][inter]
   int cap;            // tokens staged at a time
+  int group_cap;      // tokens of a group
   int x_pitch;        // bytes of a staged piece of a token
   int parts;          // warps that divide a tile's steps of hidden
+  int round_tiles;    // tiles that a round's warps work on
   int block_down;     // bytes of a step of the down slab
   bool prefetch_down; // small enough for L2 while the first kernel works
 };
 
+// Column tiles that a group's tokens take in the products: one or two, in registers.
+__host__ __device__ constexpr int GroupTokens(int type) { return type == kF32 ? 4 : 8; }
+__host__ __device__ constexpr int GroupTiles(int tokens, int pieces) { return (tokens + TokensATile(pieces) - 1) / TokensATile(pieces); }
 // Pieces of a GLU value: 16-bit activations keep 16 bits of it, F32 ones all 24.
 __host__ __device__ constexpr int GluPieces(int type) { return type == kF32 ? 3 : 2; }
 
@@ -83,22 +89,20 @@ struct FirstShared {
   float weights[kMaxPairs];
   std::uint32_t mask[kMaxExperts];  // tokens that name the expert
   std::int32_t start[kMaxExperts];
-  std::int32_t group_expert[kMaxPairs], group_first[kMaxPairs], group_count[kMaxPairs];
   std::int32_t token[kMaxPairs];    // of choice.pairs
-  std::int32_t groups;
+  std::int32_t chunk[kMaxExperts / 32];
   Choice choice;
 };
 
-// Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums and
-// the scores that a bias changes), two buffers of partial sums, the staged tokens and a column of zeros, logits.
+// Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums), two buffers of partial sums, the staged tokens and a column of zeros, logits.
 struct FirstLayout {
   int ring, meet, staged, logits, bytes;
-  __host__ __device__ FirstLayout(int block_bytes, int cap, int pieces, int x_pitch, int tokens, int experts) {
+  __host__ __device__ FirstLayout(int block_bytes, int cap, int group_cap, int pieces, int x_pitch, int tokens, int experts) {
     ring = kWarps * kSlots * block_bytes;
-    const int before = (kWarps * kTileRows * kMaxTokens * 8) + (tokens * experts * 4);
+    const int before = kWarps * kTileRows * kMaxTokens * 8;
     if (ring < before) ring = (before + 255) / 256 * 256;
     meet = ring;
-    staged = meet + (2 * kWarps * kTileRows * cap * 4);
+    staged = meet + (2 * kWarps * kTileRows * group_cap * 4);
     logits = staged + (((cap * pieces) + 1) * x_pitch);
     bytes = logits + (tokens * experts * 4);
   }
@@ -182,6 +186,72 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
   }
 }
 
+// The same of an F32 router for kFew tokens at a time on the multiply-add pipes: a value's pieces are joined again, a
+// lane's 8 products are added in F32, those sums in 64 bits.  (On the tensor core the router would have to be split in
+// three; that alone took 4 K cycles, the whole of this 5 K with one token.)
+constexpr int kFew = 4;
+template <int kType>
+__device__ __forceinline__ void RouterFew(const LayerArgs& a, const std::uint8_t* smem, int staged, int first_expert,
+                                          int first_token, int tokens, int warp, int lane, double (&partial)[kTileRows][kMaxTokens]) {
+  constexpr int kPieces = BfloatPieces(kType), kRouter = kF32;
+  constexpr int kBatch = 2;
+  const int g = lane >> 2, t = lane & 3;
+  double total[2][kFew];
+#pragma unroll
+  for (int c = 0; c < kFew; ++c) total[0][c] = total[1][c] = 0.0;
+  const int row_a = first_expert + g, row_b = row_a + 8;
+  const auto* base = static_cast<const std::uint8_t*>(a.router);
+  const std::int64_t row_bytes = a.router_stride * TypeBytes(kRouter);
+  const int blocks = a.hidden / 32, end = (warp + 1) * blocks / kWarps;
+  for (int first = warp * blocks / kWarps; first < end; first += kBatch) {
+    float va[kBatch][8], vb[kBatch][8];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int at = (32 * (first + q)) + (8 * t);
+      Load8<kRouter>(base + (row_a * row_bytes), at, first + q < end && row_a < a.experts ? 8 : 0, a.router_vec, va[q]);
+      Load8<kRouter>(base + (row_b * row_bytes), at, first + q < end && row_b < a.experts ? 8 : 0, a.router_vec, vb[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (first + q >= end) break;
+#pragma unroll
+      for (int c = 0; c < kFew; ++c) {
+        if (first_token + c >= tokens) break;
+        float sum_a = 0.0f, sum_b = 0.0f;
+        uint4 x[kPieces];
+#pragma unroll
+        for (int s = 0; s < kPieces; ++s) {
+          x[s] = *reinterpret_cast<const uint4*>(smem + staged + ((((first_token + c) * kPieces) + s) * a.x_pitch) + ((first + q) * 64) + (t * 16));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v = 0.0f;
+#pragma unroll
+          for (int s = kPieces - 1; s >= 0; --s) {
+            const std::uint32_t w = i < 2 ? x[s].x : i < 4 ? x[s].y : i < 6 ? x[s].z : x[s].w;
+            v += __uint_as_float((i & 1) != 0 ? w & 0xffff0000u : w << 16);
+          }
+          sum_a = fmaf(va[q][i], v, sum_a);
+          sum_b = fmaf(vb[q][i], v, sum_b);
+        }
+        total[0][c] += sum_a;
+        total[1][c] += sum_b;
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kFew; ++c) {
+    if (first_token + c >= tokens) break;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      double v = total[r][c];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      if (t == 0) partial[g + (8 * r)][first_token + c] = v;
+    }
+  }
+}
+
 // Tokens token_of(0 .. count - 1) of x as pieces in shared memory, by threads tid, tid + threads, ...
 template <int kType, typename Token>
 __device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* staged, int count, int tid, int threads,
@@ -205,45 +275,52 @@ __device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* st
   CopyAsyncCommit();
 }
 
-// A warp: token t's experts, best first, and their weights from its logits; `by`: room for what a bias makes of them.
-__device__ __forceinline__ void Choose(const LayerArgs& a, const float* row, float* by, int t, int lane, FirstShared& s) {
+// A warp: token t's experts, best first, and their weights from its logits.  A lane holds the order keys of experts
+// lane, lane + 32, ...: each round the warp's largest key, then its lowest index, is taken and struck out.
+template <int kPer>
+__device__ __forceinline__ void Choose(const LayerArgs& a, const float* row, int t, int lane, FirstShared& s) {
   const bool softmax = a.score == LLMP_B200_SCORE_SOFTMAX;
-  float top = __uint_as_float(0xff800000u), total = 1.0f;
+  const float kMinusInf = __uint_as_float(0xff800000u);
+  float logit[kPer];
+  float top = kMinusInf, total = 1.0f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = lane + (32 * i);
+    logit[i] = e < a.experts ? row[e] : kMinusInf;
+    top = fmaxf(top, logit[i]);
+  }
   if (softmax) {
-    for (int e = lane; e < a.experts; e += 32) top = fmaxf(top, row[e]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     total = 0.0f;
-    for (int e = lane; e < a.experts; e += 32) total += expf(row[e] - top);  // a NaN makes it one
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (lane + (32 * i) < a.experts) total += expf(logit[i] - top);  // a NaN makes it one
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
   auto score = [&](float l) { return softmax ? expf(l - top) / total : 1.0f / (1.0f + expf(-l)); };
-  const float* values = row;
-  if (a.bias != nullptr) {
-    for (int e = lane; e < a.experts; e += 32) by[e] = score(row[e]) + a.bias[e];
-    values = by;
+  std::uint32_t keys[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = lane + (32 * i);
+    keys[i] = e < a.experts ? OrderKey(a.bias == nullptr ? logit[i] : score(logit[i]) + a.bias[e]) : 0u;
   }
-  // a lane's best of its experts; the one that is taken is struck out and its lane looks again
-  std::uint32_t taken = 0;  // bit i: expert lane + 32 i
-  std::uint32_t best = 0;
-  int best_at = 0;
-  auto look = [&]() {
-    best = 0;
-    for (int e = lane, i = 0; e < a.experts; e += 32, ++i) {
-      const std::uint32_t k = ((taken >> i) & 1u) != 0 ? 0u : OrderKey(values[e]);
-      if (k > best) best = k, best_at = e;
-    }
-  };
-  look();
   int mine = 0;
   for (int j = 0; j < a.used; ++j) {
+    std::uint32_t best = 0;
+    int at_i = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (keys[i] > best) best = keys[i], at_i = i;
+    }
     const std::uint32_t most = __reduce_max_sync(0xffffffffu, best);
-    const int at = static_cast<int>(__reduce_min_sync(0xffffffffu, best == most ? static_cast<unsigned>(best_at) : 0x7fffffffu));
-    if (lane == j) mine = at;
-    if ((at & 31) == lane) {
-      taken |= 1u << (at >> 5);
-      look();
+    const unsigned int taken = __reduce_min_sync(0xffffffffu, best == most ? static_cast<unsigned>(lane + (32 * at_i)) : 0x7fffffffu);
+    if (lane == j) mine = static_cast<int>(taken);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (taken == static_cast<unsigned>(lane + (32 * i))) keys[i] = 0;
     }
   }
   const float p = lane < a.used ? score(row[mine]) : 0.0f;
@@ -255,6 +332,7 @@ __device__ __forceinline__ void Choose(const LayerArgs& a, const float* row, flo
   if (lane < a.used) {
     s.ids[(t * a.used) + lane] = mine;
     s.weights[(t * a.used) + lane] = (a.renormalize != 0 ? p / sum : p) * a.scale;
+    atomicOr(&s.mask[mine], 1u << t);
   }
 }
 
@@ -269,11 +347,11 @@ template <int kType, int kGroups>
 __global__ void __launch_bounds__(kThreads, 1)
 FirstKernel(const LayerArgs a) {
   constexpr int kPieces = BfloatPieces(kType);
-  constexpr int kTiles = kMaxTokens / TokensATile(kPieces);
+  constexpr int kTiles = GroupTiles(GroupTokens(kType), kPieces);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ FirstShared s;
-  const FirstLayout at(kBlock, a.cap, kPieces, a.x_pitch, a.tokens, a.experts);
+  const FirstLayout at(kBlock, a.cap, a.group_cap, kPieces, a.x_pitch, a.tokens, a.experts);
   std::uint8_t* staged = smem + at.staged;
   float* logits = reinterpret_cast<float*>(smem + at.logits);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
@@ -312,16 +390,26 @@ FirstKernel(const LayerArgs a) {
     __syncthreads();
     for (int m = rank; m < expert_tiles; m += kCluster) {
       if (warp < kWarps) {
-        constexpr int kAtOnce = kTiles < 2 ? kTiles : 2;
-        const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
-        for (int nt = 0; nt < tiles; nt += kAtOnce) {
-          if (a.router_type == kF32) {
-            RouterTile<kType, kF32, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
-          } else if (a.router_type == kF16) {
-            RouterTile<kType, kF16, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
+        auto multiply = [&](auto router) {
+          constexpr int kRouter = decltype(router)::value;
+          if constexpr (kRouter == kF32) {  // by its type alone: a token's logits stay the same whatever its company
+            for (int c = 0; c < count; c += kFew) {
+              RouterFew<kType>(a, smem, at.staged, m * 16, c, count, warp, lane, partial[warp]);
+            }
           } else {
-            RouterTile<kType, kBF16, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
+          constexpr int kAtOnce = kTiles < 2 ? kTiles : 2;
+          const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
+          for (int nt = 0; nt < tiles; nt += kAtOnce) {
+            RouterTile<kType, kRouter, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
           }
+          }
+        };
+        if (a.router_type == kF32) {
+          multiply(std::integral_constant<int, kF32>{});
+        } else if (a.router_type == kF16) {
+          multiply(std::integral_constant<int, kF16>{});
+        } else {
+          multiply(std::integral_constant<int, kBF16>{});
         }
       }
       __syncthreads();
@@ -344,43 +432,43 @@ FirstKernel(const LayerArgs a) {
 
   // ---- the choice, the same in every CTA
   if (warp < a.tokens) {
-    auto* by = reinterpret_cast<float*>(smem + (kWarps * kTileRows * kMaxTokens * 8));
-    Choose(a, logits + (warp * a.experts), by + (warp * a.experts), warp, lane, s);
-    if (lane < a.used) atomicOr(&s.mask[s.ids[(warp * a.used) + lane]], 1u << warp);
+    const float* row = logits + (warp * a.experts);
+    if (a.experts <= 128) {
+      Choose<4>(a, row, warp, lane, s);
+    } else {
+      Choose<kMaxExperts / 32>(a, row, warp, lane, s);
+    }
   }
   __syncthreads();
   const int pairs = a.tokens * a.used;
-  if (warp == 0) {
-    int named = 0, first = 0, groups = 0;
-    for (int base = 0; base < a.experts; base += 32) {
-      const int e = base + lane;
-      const int count = e < a.experts ? __popc(s.mask[e]) : 0;
-      const int pieces = count <= a.cap ? (count > 0 ? 1 : 0) : (count + a.cap - 1) / a.cap;
-      int packed = (count > 0 ? 1 : 0) | (count << 10) | (pieces << 20);  // each at most 256 in all
+  // warp w looks at experts 32 w .. + 31: how many pairs and groups come before each
+  {
+    const int e = tid;
+    const int count = warp < kMaxExperts / 32 && e < a.experts ? __popc(s.mask[e]) : 0;
+    const int pieces = (count + a.group_cap - 1) / a.group_cap;
+    int packed = count | (pieces << 16);  // each at most 256 in all
+    const int own = packed;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int below = __shfl_up_sync(0xffffffffu, packed, o);
-        if (lane >= o) packed += below;
-      }
-      if (count > 0) {
-        const int i = named + (packed & 0x3ff) - 1, begin = first + ((packed >> 10) & 0x3ff) - count;
-        const int group = groups + (packed >> 20) - pieces;
-        s.choice.expert[i] = e;
-        s.choice.first[i] = begin;
-        s.start[e] = begin;
-        for (int q = 0; q < pieces; ++q) {
-          s.group_expert[group + q] = e;
-          s.group_first[group + q] = begin + (q * a.cap);
-          s.group_count[group + q] = min(a.cap, count - (q * a.cap));
-        }
-      }
-      const int all = __shfl_sync(0xffffffffu, packed, 31);
-      named += all & 0x3ff, first += (all >> 10) & 0x3ff, groups += all >> 20;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, packed, o);
+      if (lane >= o) packed += below;
     }
-    if (lane == 0) {
-      s.choice.named = named;
-      s.choice.first[named] = first;
-      s.groups = groups;
+    if (lane == 31 && warp < kMaxExperts / 32) s.chunk[warp] = packed;
+    __syncthreads();
+    int before = packed - own;
+    for (int w = 0; w < warp && w < kMaxExperts / 32; ++w) before += s.chunk[w];
+    if (count > 0) {
+      const int begin = before & 0xffff, group = before >> 16;
+      s.start[e] = begin;
+      for (int q = 0; q < pieces; ++q) {
+        s.choice.expert[group + q] = e;
+        s.choice.first[group + q] = begin + (q * a.group_cap);
+      }
+    }
+    if (tid == kMaxExperts - 1) {
+      const int all = before + own;
+      s.choice.groups = all >> 16;
+      s.choice.first[all >> 16] = all & 0xffff;
     }
   }
   __syncthreads();
@@ -392,16 +480,17 @@ FirstKernel(const LayerArgs a) {
   }
   __syncthreads();
 
-  // ---- this CTA's rounds: a group's two neighbouring tiles of 8 gate and 8 up rows, each divided among the warps
-  const int rounds_a_group = (a.tiles_up + kTilesARound - 1) / kTilesARound;
-  const std::int64_t rounds = static_cast<std::int64_t>(s.groups) * rounds_a_group;
+  // ---- this CTA's rounds: a group's next tiles of 8 gate and 8 up rows, each divided among a few warps
+  const int round_tiles = a.round_tiles, tile_warps = kWarps / round_tiles;
+  const int rounds_a_group = (a.tiles_up + round_tiles - 1) / round_tiles;
+  const std::int64_t rounds = static_cast<std::int64_t>(s.choice.groups) * rounds_a_group;
   const int first_round = static_cast<int>(rounds * blockIdx.x / gridDim.x);
   const int end_round = static_cast<int>(rounds * (blockIdx.x + 1) / gridDim.x);
   const bool all_staged = a.tokens <= a.cap;
   float* meet = reinterpret_cast<float*>(smem + at.meet);
-  const int meet_floats = kWarps * kTileRows * a.cap;
+  const int meet_floats = kWarps * kTileRows * a.group_cap;
   if (warp < kWarps) {
-    const int my_tile = warp / (kWarps / kTilesARound), part = warp % (kWarps / kTilesARound);
+    const int my_tile = warp / tile_warps, part = warp % tile_warps;
     const int begin = part < a.parts ? a.steps_up * part / a.parts : 0;
     const int steps = part < a.parts ? (a.steps_up * (part + 1) / a.parts) - begin : 0;
     std::uint8_t* ring = smem + (warp * kSlots * kBlock);
@@ -411,9 +500,9 @@ FirstKernel(const LayerArgs a) {
     const std::uint8_t* src = nullptr;
     auto next_load_round = [&]() {  // the next round in which this warp has a tile
       while (load_left == 0 && load_rounds > 0 && steps > 0) {
-        const int tile = (load_pair * kTilesARound) + my_tile;
+        const int tile = (load_pair * round_tiles) + my_tile;
         if (tile < a.tiles_up) {
-          src = a.gate_up + ((((static_cast<std::size_t>(s.group_expert[load_group]) * a.tiles_up) + tile) * a.steps_up) + begin) * kBlock +
+          src = a.gate_up + ((((static_cast<std::size_t>(s.choice.expert[load_group]) * a.tiles_up) + tile) * a.steps_up) + begin) * kBlock +
                 (lane * 16);
           load_left = steps;
         }
@@ -437,7 +526,7 @@ FirstKernel(const LayerArgs a) {
     for (int i = 0; i < kSlots - 1; ++i) request(i);
     if (a.prefetch_down) {  // the named experts' down rows, on their way while this kernel works
       const std::int64_t lines = static_cast<std::int64_t>(a.tiles_down) * a.steps_down * a.block_down / 128;  // an expert's
-      const std::int64_t all = lines * s.choice.named, stride = static_cast<std::int64_t>(gridDim.x) * kWarps * 32;
+      const std::int64_t all = lines * s.choice.groups, stride = static_cast<std::int64_t>(gridDim.x) * kWarps * 32;
       for (std::int64_t i = (static_cast<std::int64_t>(blockIdx.x) * kWarps * 32) + tid; i < all; i += stride) {
         const std::int64_t n = i / lines;
         asm volatile("prefetch.global.L2 [%0];" ::"l"(a.down + ((s.choice.expert[n] * lines) + (i - (n * lines))) * 128));
@@ -447,7 +536,7 @@ FirstKernel(const LayerArgs a) {
     int group = first_round / rounds_a_group, pair = first_round % rounds_a_group;
     int slot = 0, buffer = 0, staged_group = -1;
     for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
-      const int first = s.group_first[group], count = s.group_count[group];
+      const int first = s.choice.first[group], count = s.choice.first[group + 1] - first;
       if (!all_staged && staged_group != group) {
         if (staged_group >= 0) BarrierSync(5, kWarps * 32);
         StageTokens<kType>(a, staged, count, tid, kWarps * 32, [&](int c) { return static_cast<std::int64_t>(s.token[first + c]); });
@@ -465,7 +554,7 @@ FirstKernel(const LayerArgs a) {
         column[nt] = at.staged + (row * a.x_pitch) + (t4 * 16) + (begin * 256);
       }
       Sums total[kTiles];
-      if ((pair * kTilesARound) + my_tile < a.tiles_up) {
+      if ((pair * round_tiles) + my_tile < a.tiles_up) {
         for (int step = 0; step < steps; ++step) {
           CopyAsyncWait<kSlots - 2>();
           __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
@@ -480,7 +569,7 @@ FirstKernel(const LayerArgs a) {
       }
       // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
       if (round - first_round >= 2) BarrierSync(3 + buffer, kThreads);
-      float* mine = meet + (buffer * meet_floats) + (warp * kTileRows * a.cap);
+      float* mine = meet + (buffer * meet_floats) + (warp * kTileRows * a.group_cap);
 #pragma unroll
       for (int nt = 0; nt < kTiles; ++nt) {
         if (nt >= tiles) break;
@@ -505,31 +594,33 @@ FirstKernel(const LayerArgs a) {
         a.weights[p] = s.weights[p];
         a.choice->pairs[p] = s.choice.pairs[p];
       }
-      for (int i = tid - (kWarps * 32); i < s.choice.named; i += kReducers * 32) a.choice->expert[i] = s.choice.expert[i];
-      for (int i = tid - (kWarps * 32); i <= s.choice.named; i += kReducers * 32) a.choice->first[i] = s.choice.first[i];
-      if (tid == kWarps * 32) a.choice->named = s.choice.named;
+      for (int i = tid - (kWarps * 32); i < s.choice.groups; i += kReducers * 32) a.choice->expert[i] = s.choice.expert[i];
+      for (int i = tid - (kWarps * 32); i <= s.choice.groups; i += kReducers * 32) a.choice->first[i] = s.choice.first[i];
+      if (tid == kWarps * 32) a.choice->groups = s.choice.groups;
     }
-    // a warp a tile of the round; a lane a row of four tokens
-    const int my_tile = warp - kWarps, row = lane & 7;
+    // a warp every other tile of the round; a lane a row of every fourth token
+    const int row = lane & 7;
     int group = first_round / rounds_a_group, pair = first_round % rounds_a_group, buffer = 0;
     for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
       BarrierSync(1 + buffer, kThreads);
-      const int first = s.group_first[group], count = s.group_count[group];
-      const int out = (((pair * kTilesARound) + my_tile) * 8) + row;
-      const float* p = meet + (buffer * meet_floats) + (my_tile * (kWarps / kTilesARound) * kTileRows * a.cap) + row;
-      for (int c = lane >> 3; c < count && out < a.inter; c += 4) {
-        float gate = 0.0f, up = 0.0f;
+      const int first = s.choice.first[group], count = s.choice.first[group + 1] - first;
+      for (int tile = warp - kWarps; tile < round_tiles; tile += kReducers) {
+        const int out = (((pair * round_tiles) + tile) * 8) + row;
+        const float* p = meet + (buffer * meet_floats) + (tile * tile_warps * kTileRows * a.group_cap) + row;
+        for (int c = lane >> 3; c < count && out < a.inter; c += 4) {
+          float gate = 0.0f, up = 0.0f;
 #pragma unroll 4
-        for (int q = 0; q < a.parts; ++q) {
-          gate += p[((q * a.cap) + c) * kTileRows];
-          up += p[(((q * a.cap) + c) * kTileRows) + 8];
-        }
-        constexpr int kGlu = GluPieces(kType);
-        std::uint32_t bits[kGlu];
-        Split<kGlu>(Glu(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
-        unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[first + c]) * kGlu * a.inter) + out;
+          for (int q = 0; q < a.parts; ++q) {
+            gate += p[((q * a.group_cap) + c) * kTileRows];
+            up += p[(((q * a.group_cap) + c) * kTileRows) + 8];
+          }
+          constexpr int kGlu = GluPieces(kType);
+          std::uint32_t bits[kGlu];
+          Split<kGlu>(Glu(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
+          unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[first + c]) * kGlu * a.inter) + out;
 #pragma unroll
-        for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);
+          for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);
+        }
       }
       BarrierArrive(3 + buffer, kThreads);
       if (++pair == rounds_a_group) pair = 0, ++group;
@@ -537,7 +628,7 @@ FirstKernel(const LayerArgs a) {
   }
 }
 
-// A CTA's 16 rows of the output: its warps take (expert, half of inter) items in turn, their weights through rings as
+// A CTA's 16 rows of the output: its warps take (group, half of inter) items in turn, their weights through rings as
 // in the first kernel, the GLU rows straight from L2 a step ahead; each pair's sums meet in shared memory and
 // a token's slots are added in order.
 constexpr int kParts = 2;
@@ -547,7 +638,7 @@ template <int kType, int kGroups>
 __global__ void __launch_bounds__(kSecondWarps * 32, 1)
 SecondKernel(const LayerArgs a) {
   constexpr int kGlu = GluPieces(kType);
-  constexpr int kTiles = kMaxTokens / TokensATile(kGlu);
+  constexpr int kTiles = GroupTiles(GroupTokens(kType), kGlu);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ Choice choice;
@@ -559,14 +650,14 @@ SecondKernel(const LayerArgs a) {
   GridDependencyWait();
   const int tile = static_cast<int>(blockIdx.x), pairs = a.tokens * a.used;
   for (int i = tid; i < pairs; i += threads) {
-    choice.expert[i] = __ldcg(&a.choice->expert[i]);   // (what is past the named ones is not used)
+    choice.expert[i] = __ldcg(&a.choice->expert[i]);   // (what is past the groups is not used)
     choice.pairs[i] = __ldcg(&a.choice->pairs[i]);
     choice.first[i] = __ldcg(&a.choice->first[i]);
   }
   if (tid == 0) choice.first[pairs] = __ldcg(&a.choice->first[pairs]);
-  if (tid == threads - 1) choice.named = __ldcg(&a.choice->named);
+  if (tid == threads - 1) choice.groups = __ldcg(&a.choice->groups);
   __syncthreads();
-  const int items = choice.named * kParts;
+  const int items = choice.groups * kParts;
   const int piece = g % Cols(kGlu);
   auto step0_of = [&](int item) { return (item % kParts) * a.steps_down / kParts; };
   auto steps_of = [&](int item) { return (((item % kParts) + 1) * a.steps_down / kParts) - step0_of(item); };
@@ -670,17 +761,46 @@ cudaError_t Configure(Kernel kernel, int& configured_device, int smem) {
   return e;
 }
 
+// Clusters of the first kernel that the device holds at once (a GPC holds whole clusters: more would be a second wave).
+template <typename Kernel>
+int ResidentClusters(Kernel kernel, int smem) {
+  struct Known {
+    int device = -1, smem = -1, clusters = 1;
+  };
+  static thread_local Known known;
+  int device = -1;
+  cudaGetDevice(&device);
+  if (known.device == device && known.smem == smem) return known.clusters;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(SmCount() / kCluster * kCluster));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = static_cast<std::size_t>(smem);
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = kCluster;
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess || clusters < 1) {
+    cudaGetLastError();
+    clusters = std::max(1, SmCount() / (2 * kCluster));
+  }
+  known.device = device, known.smem = smem, known.clusters = clusters;
+  return clusters;
+}
+
 template <int kType, int kGroups>
 int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   static thread_local int configured_device = -1;
   if (const cudaError_t e = Configure(FirstKernel<kType, kGroups>, configured_device, kFirstSmemLimit); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
+  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.cap, a.group_cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
   const std::int64_t rounds = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) *
-                              ((a.tiles_up + kTilesARound - 1) / kTilesARound);
-  const std::int64_t most = std::max(1, SmCount() / kCluster);
+                              ((a.tiles_up + a.round_tiles - 1) / a.round_tiles);
+  const std::int64_t most = ResidentClusters(FirstKernel<kType, kGroups>, smem);
   const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + kCluster - 1) / kCluster));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(clusters * kCluster));
@@ -787,14 +907,21 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.choice = static_cast<Choice*>(d.scratch);
   a.h = reinterpret_cast<unsigned short*>(static_cast<std::uint8_t*>(d.scratch) + ChoiceBytes());
   a.x_pitch = (a.steps_up * kStep * 2) + 64;
-  a.parts = kWarps / kTilesARound;
-  while (a.parts > a.steps_up) a.parts /= 2;
+  // A warp's run of a tile is four steps and more where hidden allows it (each round costs a warp about two steps'
+  // instructions besides), but a tile has at least four warps: few tokens name few tiles.  Not by the number of tokens:
+  // a token's sums stay the same whatever its company.
+  int tile_warps = 4;
+  while (tile_warps < kWarps && a.steps_up >= 8 * tile_warps) tile_warps *= 2;
+  a.round_tiles = kWarps / tile_warps;
+  a.parts = std::min(tile_warps, a.steps_up);
   a.block_down = BlockBytes(d.down.group);
   a.prefetch_down = static_cast<double>(std::min(experts, d.tokens * d.used)) * a.tiles_down * a.steps_down * a.block_down <= 32e6;
   a.cap = d.tokens;
-  while (a.cap > 1 && FirstLayout(BlockBytes(d.gate_up.group), a.cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes >
+  a.group_cap = std::min(d.tokens, GroupTokens(d.x_type));
+  while (a.cap > 1 && FirstLayout(BlockBytes(d.gate_up.group), a.cap, a.group_cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes >
                           kFirstSmemLimit) {
     --a.cap;
+    a.group_cap = std::min(a.group_cap, a.cap);
   }
   const auto s = static_cast<cudaStream_t>(stream);
   if (d.x_type == kF32) return LaunchLayer<kF32>(d.gate_up.group, d.down.group, a, s);
