@@ -25,8 +25,9 @@ using namespace w4;
 
 constexpr int kWarps = 16, kReducers = 2;          // of the first kernel: that multiply, that add up
 constexpr int kThreads = (kWarps + kReducers) * 32;
-constexpr int kSlots = 4;                          // steps a warp's ring holds
-constexpr int kCluster = 8;
+constexpr int kFewSlots = 4, kManySlots = 6;       // steps a warp's ring of the first kernel holds, where they fit
+constexpr int kSecondSlots = 6;
+constexpr int kMaxCluster = 8;
 constexpr int kMaxTokens = 16, kMaxUsed = 16, kMaxExperts = 512;
 constexpr int kMaxPairs = kMaxTokens * kMaxUsed;
 constexpr int kFirstSmemLimit = 196 * 1024;        // dynamic; the choice's lists are static
@@ -65,6 +66,7 @@ struct LayerArgs {
   int cap;            // tokens staged at a time
   int group_cap;      // tokens of a group
   int x_pitch;        // bytes of a staged piece of a token
+  int slots;          // of the first kernel's rings
   int parts;          // warps that divide a tile's steps of hidden
   int round_tiles;    // tiles that a round's warps work on
   int block_down;     // bytes of a step of the down slab
@@ -97,8 +99,8 @@ struct FirstShared {
 // Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums), two buffers of partial sums, the staged tokens and a column of zeros, logits.
 struct FirstLayout {
   int ring, meet, staged, logits, bytes;
-  __host__ __device__ FirstLayout(int block_bytes, int cap, int group_cap, int pieces, int x_pitch, int tokens, int experts) {
-    ring = kWarps * kSlots * block_bytes;
+  __host__ __device__ FirstLayout(int block_bytes, int slots, int cap, int group_cap, int pieces, int x_pitch, int tokens, int experts) {
+    ring = kWarps * slots * block_bytes;
     const int before = kWarps * kTileRows * kMaxTokens * 8;
     if (ring < before) ring = (before + 255) / 256 * 256;
     meet = ring;
@@ -109,14 +111,14 @@ struct FirstLayout {
 };
 
 // 16 experts' logits for the staged tokens over this warp's share of hidden.  Products of two bf16 pieces are
-// exact; a 32-value block's sum is F32 and the blocks are added in 64 bits, because the choice compares
-// values that may lie next to each other.  kBatch blocks' router rows are in flight together.
+// exact; kBatch blocks of 32 values are in flight together and added in F32, the batches in 64 bits, because the choice
+// compares values that may lie next to each other.
 template <int kType, int kRouter, int kTiles>
 __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_t* smem, int staged, int first_expert,
                                            int first_tile, int tokens, int warp, int lane,
                                            double (&partial)[kTileRows][kMaxTokens]) {
   constexpr int kPieces = BfloatPieces(kType), kRouterPieces = BfloatPieces(kRouter);
-  constexpr int kBatch = kRouter == kF32 ? 2 : 4;
+  constexpr int kBatch = kRouter == kF16 ? 2 : 4;
   const int g = lane >> 2, t = lane & 3;
   const int piece = g % Cols(kPieces);
   double total[kTiles][4];
@@ -133,31 +135,36 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
   const auto* base = static_cast<const std::uint8_t*>(a.router);
   const std::int64_t row_bytes = a.router_stride * TypeBytes(kRouter);
   const int blocks = a.hidden / 32, end = (warp + 1) * blocks / kWarps;
+  auto load = [&](int row, int block, uint4 (&quads)[kRouterPieces]) {
+    const int at = (32 * block) + (8 * t), valid = block < end && row < a.experts ? 8 : 0;
+    const std::uint8_t* p = base + (row * row_bytes);
+    if (kRouter == kBF16 && a.router_vec && valid == 8) {
+      quads[0] = *reinterpret_cast<const uint4*>(p + (at * 2));
+    } else {
+      LoadBfloat8<kRouter>(p, at, valid, a.router_vec, quads);
+    }
+  };
   for (int first = warp * blocks / kWarps; first < end; first += kBatch) {
-    float va[kBatch][8], vb[kBatch][8];
+    uint4 qa[kBatch][kRouterPieces], qb[kBatch][kRouterPieces];
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      const int at = (32 * (first + q)) + (8 * t);
-      Load8<kRouter>(base + (row_a * row_bytes), at, first + q < end && row_a < a.experts ? 8 : 0, a.router_vec, va[q]);
-      Load8<kRouter>(base + (row_b * row_bytes), at, first + q < end && row_b < a.experts ? 8 : 0, a.router_vec, vb[q]);
+      load(row_a, first + q, qa[q]);  // (zero from the share's end on)
+      load(row_b, first + q, qb[q]);
     }
 #pragma unroll
-    for (int q = 0; q < kBatch; ++q) {
-      if (first + q >= end) break;
-      uint4 qa[kRouterPieces], qb[kRouterPieces];
-      PackBfloat8(va[q], qa);
-      PackBfloat8(vb[q], qb);
+    for (int nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
-      for (int nt = 0; nt < kTiles; ++nt) {
-        const uint4 x = *reinterpret_cast<const uint4*>(smem + column[nt] + ((first + q) * 64));
+      for (int r = 0; r < kRouterPieces; ++r) {
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int r = 0; r < kRouterPieces; ++r) {
-          float sum[4];
-          Mma<false, true>(sum, qa[r].x, qb[r].x, qa[r].y, qb[r].y, x.x, x.y);
-          Mma<false, false>(sum, qa[r].z, qb[r].z, qa[r].w, qb[r].w, x.z, x.w);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) total[nt][c] += sum[c];
+        for (int q = 0; q < kBatch; ++q) {
+          const uint4 x = first + q < end ? *reinterpret_cast<const uint4*>(smem + column[nt] + ((first + q) * 64))
+                                          : make_uint4(0, 0, 0, 0);
+          Mma<false, false>(sum, qa[q][r].x, qb[q][r].x, qa[q][r].y, qb[q][r].y, x.x, x.y);
+          Mma<false, false>(sum, qa[q][r].z, qb[q][r].z, qa[q][r].w, qb[q][r].w, x.z, x.w);
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) total[nt][c] += sum[c];
       }
     }
   }
@@ -258,18 +265,17 @@ __device__ __forceinline__ void StageTokens(const LayerArgs& a, std::uint8_t* st
                                             Token token_of) {
   constexpr int kPieces = BfloatPieces(kType);
   const int octets = a.steps_up * (kStep / 8);
-  for (int c = 0; c < count; ++c) {
+  for (int n = tid; n < count * octets; n += threads) {
+    const int c = n / octets, i = n - (c * octets);
     const auto* row = static_cast<const std::uint8_t*>(a.x) + (token_of(c) * a.x_stride * TypeBytes(kType));
-    for (int i = tid; i < octets; i += threads) {
-      std::uint8_t* out = staged + ((c * kPieces) * a.x_pitch) + (i * 16);
-      if constexpr (kType == kBF16) {
-        Stage8(out, row, i * 8, a.hidden - (i * 8), a.x_vec);
-      } else {
-        uint4 quads[kPieces];
-        LoadBfloat8<kType>(row, i * 8, a.hidden - (i * 8), a.x_vec, quads);
+    std::uint8_t* out = staged + ((c * kPieces) * a.x_pitch) + (i * 16);
+    if constexpr (kType == kBF16) {
+      Stage8(out, row, i * 8, a.hidden - (i * 8), a.x_vec);
+    } else {
+      uint4 quads[kPieces];
+      LoadBfloat8<kType>(row, i * 8, a.hidden - (i * 8), a.x_vec, quads);
 #pragma unroll
-        for (int s = 0; s < kPieces; ++s) *reinterpret_cast<uint4*>(out + (s * a.x_pitch)) = quads[s];
-      }
+      for (int s = 0; s < kPieces; ++s) *reinterpret_cast<uint4*>(out + (s * a.x_pitch)) = quads[s];
     }
   }
   CopyAsyncCommit();
@@ -351,19 +357,19 @@ FirstKernel(const LayerArgs a) {
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ FirstShared s;
-  const FirstLayout at(kBlock, a.cap, a.group_cap, kPieces, a.x_pitch, a.tokens, a.experts);
+  const FirstLayout at(kBlock, a.slots, a.cap, a.group_cap, kPieces, a.x_pitch, a.tokens, a.experts);
   std::uint8_t* staged = smem + at.staged;
   float* logits = reinterpret_cast<float*>(smem + at.logits);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank());
+  const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
   GridLaunchDependents();
   const int expert_tiles = (a.experts + 15) / 16;
   {  // this CTA's router rows into L2 while the kernel before ends
     const std::size_t row_bytes = static_cast<std::size_t>(a.hidden) * TypeBytes(a.router_type);
     const int lines = static_cast<int>((row_bytes + 127) / 128);
-    for (int m = rank; m < expert_tiles; m += kCluster) {
+    for (int m = rank; m < expert_tiles; m += ranks) {
       for (int i = tid; i < 16 * lines; i += kThreads) {
         const int e = (m * 16) + (i / lines);
         if (e < a.experts) {
@@ -388,7 +394,7 @@ FirstKernel(const LayerArgs a) {
     StageTokens<kType>(a, staged, count, tid, kThreads, [&](int c) { return static_cast<std::int64_t>(first + c); });
     CopyAsyncWait<0>();
     __syncthreads();
-    for (int m = rank; m < expert_tiles; m += kCluster) {
+    for (int m = rank; m < expert_tiles; m += ranks) {
       if (warp < kWarps) {
         auto multiply = [&](auto router) {
           constexpr int kRouter = decltype(router)::value;
@@ -415,14 +421,16 @@ FirstKernel(const LayerArgs a) {
       __syncthreads();
       if (!met) cluster.sync();  // every CTA of the cluster has begun: its shared memory may be written
       met = true;
-      // eight threads a logit, each storing to one rank
-      for (int i = tid; i < 16 * count * kCluster; i += kThreads) {
-        const int r = i % kCluster, row = (i / kCluster) % 16, c = (i / kCluster) / 16, e = (m * 16) + row;
-        if (e >= a.experts) continue;
+      // eight threads a logit: each adds two warps' sums, all of them up in a fixed order, each stores to a rank
+      for (int first_i = 0; first_i < 16 * count * 8; first_i += kThreads) {
+        const int i = first_i + tid, q = i % 8, row = (i / 8) % 16, c = (i / 8) / 16, e = (m * 16) + row;
         double sum = 0.0;
+        if (c < count) sum = partial[2 * q][row][c] + partial[(2 * q) + 1][row][c];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += partial[w][row][c];
-        cluster.map_shared_rank(logits, r)[((first + c) * a.experts) + e] = static_cast<float>(sum);
+        for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (c < count && q < ranks && e < a.experts) {
+          cluster.map_shared_rank(logits, q)[((first + c) * a.experts) + e] = static_cast<float>(sum);
+        }
       }
       __syncthreads();
     }
@@ -493,7 +501,8 @@ FirstKernel(const LayerArgs a) {
     const int my_tile = warp / tile_warps, part = warp % tile_warps;
     const int begin = part < a.parts ? a.steps_up * part / a.parts : 0;
     const int steps = part < a.parts ? (a.steps_up * (part + 1) / a.parts) - begin : 0;
-    std::uint8_t* ring = smem + (warp * kSlots * kBlock);
+    const int slots = a.slots;
+    std::uint8_t* ring = smem + (warp * slots * kBlock);
     // where the next request reads
     int load_group = first_round / rounds_a_group, load_pair = first_round % rounds_a_group;
     int load_rounds = end_round - first_round, load_left = 0;
@@ -522,8 +531,7 @@ FirstKernel(const LayerArgs a) {
       }
       CopyAsyncCommit();
     };
-#pragma unroll
-    for (int i = 0; i < kSlots - 1; ++i) request(i);
+    for (int i = 0; i < slots - 1; ++i) request(i);
     if (a.prefetch_down) {  // the named experts' down rows, on their way while this kernel works
       const std::int64_t lines = static_cast<std::int64_t>(a.tiles_down) * a.steps_down * a.block_down / 128;  // an expert's
       const std::int64_t all = lines * s.choice.groups, stride = static_cast<std::int64_t>(gridDim.x) * kWarps * 32;
@@ -556,15 +564,15 @@ FirstKernel(const LayerArgs a) {
       Sums total[kTiles];
       if ((pair * round_tiles) + my_tile < a.tiles_up) {
         for (int step = 0; step < steps; ++step) {
-          CopyAsyncWait<kSlots - 2>();
+          if (slots == kManySlots) CopyAsyncWait<kManySlots - 2>(); else CopyAsyncWait<kFewSlots - 2>();
           __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
-          request(slot == 0 ? kSlots - 1 : slot - 1);
+          request(slot == 0 ? slots - 1 : slot - 1);
           StepWeights<kGroups> w;
-          w.LoadShared(smem + (((warp * kSlots) + slot) * kBlock), lane);
+          w.LoadShared(smem + (((warp * slots) + slot) * kBlock), lane);
           MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int i) {
             return *reinterpret_cast<const uint4*>(smem + column[nt] + (step * 256) + (i * 64));
           });
-          slot = slot == kSlots - 1 ? 0 : slot + 1;
+          slot = slot == slots - 1 ? 0 : slot + 1;
         }
       }
       // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
@@ -643,7 +651,7 @@ SecondKernel(const LayerArgs a) {
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ Choice choice;
   const int threads = static_cast<int>(blockDim.x), warps = threads >> 5;
-  auto* sums = reinterpret_cast<float*>(smem + (warps * kSlots * kBlock));  // [pair][part][16 rows]
+  auto* sums = reinterpret_cast<float*>(smem + (warps * kSecondSlots * kBlock));  // [pair][part][16 rows]
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   GridLaunchDependents();
@@ -661,7 +669,7 @@ SecondKernel(const LayerArgs a) {
   const int piece = g % Cols(kGlu);
   auto step0_of = [&](int item) { return (item % kParts) * a.steps_down / kParts; };
   auto steps_of = [&](int item) { return (((item % kParts) + 1) * a.steps_down / kParts) - step0_of(item); };
-  std::uint8_t* ring = smem + (warp * kSlots * kBlock);
+  std::uint8_t* ring = smem + (warp * kSecondSlots * kBlock);
   int load_item = warp - warps, load_left = 0;
   const std::uint8_t* src = nullptr;
   auto request = [&](int slot) {
@@ -683,47 +691,68 @@ SecondKernel(const LayerArgs a) {
     CopyAsyncCommit();
   };
 #pragma unroll
-  for (int i = 0; i < kSlots - 1; ++i) request(i);
-  int slot = 0;
-  for (int item = warp; item < items; item += warps) {
+  for (int i = 0; i < kSecondSlots - 1; ++i) request(i);
+  // the columns of an item's pairs: this lane's in each column tile
+  struct Columns {
+    const unsigned short* at[kTiles];
+  };
+  auto columns_of = [&](int item) {
+    Columns columns;
     const int begin = choice.first[item / kParts], count = choice.first[(item / kParts) + 1] - begin;
-    const int step0 = step0_of(item), steps = steps_of(item);
-    const unsigned short* column[kTiles];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int c = (nt * TokensATile(kGlu)) + (g / Cols(kGlu));
-      column[nt] = nullptr;
+      columns.at[nt] = nullptr;
       if (c < count && piece < kGlu) {
-        column[nt] = a.h + (((static_cast<std::size_t>(choice.pairs[begin + c]) * kGlu) + piece) * a.inter) + (t4 * 8);
+        columns.at[nt] = a.h + (((static_cast<std::size_t>(choice.pairs[begin + c]) * kGlu) + piece) * a.inter) + (t4 * 8);
       }
     }
-    auto fetch = [&](int nt, int step, int b) {
-      const int at = ((step0 + step) * kStep) + (32 * b);  // inter is whole 32-value blocks
-      if (column[nt] == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
-      return __ldcg(reinterpret_cast<const uint4*>(column[nt] + at));
-    };
-    const int tiles = (count + TokensATile(kGlu) - 1) / TokensATile(kGlu);
-    Sums total[kTiles];
-    uint4 ahead[4];
-    if (steps > 0) {
+    return columns;
+  };
+  auto fetch = [&](const unsigned short* column, int step, int b) {
+    const int at = (step * kStep) + (32 * b);  // inter is whole 32-value blocks
+    if (column == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
+    return __ldcg(reinterpret_cast<const uint4*>(column + at));
+  };
+  auto next_item = [&](int item) {  // with a step to it
+    do {
+      item += warps;
+    } while (item < items && steps_of(item) == 0);
+    return item;
+  };
+  int slot = 0, item = next_item(warp - warps);
+  Columns columns = {};
+  uint4 ahead[4];
+  if (item < items) {
+    columns = columns_of(item);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) ahead[b] = fetch(0, 0, b);
-    }
-    for (int step = 0; step < steps; ++step) {
+    for (int b = 0; b < 4; ++b) ahead[b] = fetch(columns.at[0], step0_of(item), b);
+  }
+  while (item < items) {
+    const int begin = choice.first[item / kParts], count = choice.first[(item / kParts) + 1] - begin;
+    const int step0 = step0_of(item), end = step0 + steps_of(item), after = next_item(item);
+    const int tiles = (count + TokensATile(kGlu) - 1) / TokensATile(kGlu);
+    Columns next = columns;
+    Sums total[kTiles];
+    for (int step = step0; step < end; ++step) {
       uint4 now[4];
 #pragma unroll
       for (int b = 0; b < 4; ++b) now[b] = ahead[b];
-      if (step + 1 < steps) {
+      int ahead_step = step + 1;
+      if (ahead_step == end && after < items) next = columns_of(after), ahead_step = step0_of(after);
+      if (step + 1 < end || after < items) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b) ahead[b] = fetch(0, step + 1, b);
+        for (int b = 0; b < 4; ++b) ahead[b] = fetch(next.at[0], ahead_step, b);
       }
-      CopyAsyncWait<kSlots - 2>();
+      CopyAsyncWait<kSecondSlots - 2>();
       __syncwarp();
-      request(slot == 0 ? kSlots - 1 : slot - 1);
+      request(slot == 0 ? kSecondSlots - 1 : slot - 1);
       StepWeights<kGroups> w;
-      w.LoadShared(smem + (((warp * kSlots) + slot) * kBlock), lane);
-      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int b) { return nt == 0 ? now[b] : fetch(nt, step, b); });
-      slot = slot == kSlots - 1 ? 0 : slot + 1;
+      w.LoadShared(smem + (((warp * kSecondSlots) + slot) * kBlock), lane);
+      MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int b) {
+        return nt == 0 ? now[b] : fetch(columns.at[nt], step, b);
+      });
+      slot = slot == kSecondSlots - 1 ? 0 : slot + 1;
     }
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
@@ -737,6 +766,12 @@ SecondKernel(const LayerArgs a) {
         out[g + 8] = v[1][0];
       }
     }
+    item = after;
+    columns = next;
+  }
+  if (a.steps_down < kParts) {  // the first part of a single step has none
+    __syncthreads();
+    for (int i = tid; i < pairs * kTileRows; i += threads) sums[((i / kTileRows) * kParts * kTileRows) + (i % kTileRows)] = 0.0f;
   }
   __syncthreads();
   for (int i = tid; i < a.tokens * kTileRows; i += threads) {
@@ -761,32 +796,34 @@ cudaError_t Configure(Kernel kernel, int& configured_device, int smem) {
   return e;
 }
 
-// Clusters of the first kernel that the device holds at once (a GPC holds whole clusters: more would be a second wave).
+// Clusters of `size` CTAs of the first kernel that the device holds at once (a GPC holds whole clusters: more would be a
+// second wave).
 template <typename Kernel>
-int ResidentClusters(Kernel kernel, int smem) {
+int ResidentClusters(Kernel kernel, int size, int smem) {
   struct Known {
-    int device = -1, smem = -1, clusters = 1;
+    int device = -1, size = 0, smem = -1, clusters = 1;
   };
-  static thread_local Known known;
+  static thread_local Known known[2];
+  Known& k = known[size == kMaxCluster ? 1 : 0];
   int device = -1;
   cudaGetDevice(&device);
-  if (known.device == device && known.smem == smem) return known.clusters;
+  if (k.device == device && k.size == size && k.smem == smem) return k.clusters;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(SmCount() / kCluster * kCluster));
+  config.gridDim = dim3(static_cast<unsigned>(SmCount() / size * size));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = static_cast<std::size_t>(smem);
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = kCluster;
+  attribute[0].val.clusterDim.x = static_cast<unsigned>(size);
   attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
   int clusters = 0;
   if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess || clusters < 1) {
     cudaGetLastError();
-    clusters = std::max(1, SmCount() / (2 * kCluster));
+    clusters = std::max(1, SmCount() / (2 * size));
   }
-  known.device = device, known.smem = smem, known.clusters = clusters;
+  k.device = device, k.size = size, k.smem = smem, k.clusters = clusters;
   return clusters;
 }
 
@@ -796,20 +833,23 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   if (const cudaError_t e = Configure(FirstKernel<kType, kGroups>, configured_device, kFirstSmemLimit); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.cap, a.group_cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
+  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.slots, a.cap, a.group_cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
   const std::int64_t rounds = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) *
                               ((a.tiles_up + a.round_tiles - 1) / a.round_tiles);
-  const std::int64_t most = ResidentClusters(FirstKernel<kType, kGroups>, smem);
-  const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + kCluster - 1) / kCluster));
+  // Clusters of four fill more of the device's SMs (on B200 36 against 15 of eight), each working the whole router out:
+  // worth it where the products outlast that.
+  const int size = rounds > 8 * SmCount() ? kMaxCluster / 2 : kMaxCluster;
+  const std::int64_t most = ResidentClusters(FirstKernel<kType, kGroups>, size, smem);
+  const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + size - 1) / size));
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(clusters * kCluster));
+  config.gridDim = dim3(static_cast<unsigned>(clusters * size));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = static_cast<std::size_t>(smem);
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = kCluster;
+  attribute[0].val.clusterDim.x = static_cast<unsigned>(size);
   attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
   attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[1].val.programmaticStreamSerializationAllowed = 1;
@@ -822,12 +862,12 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
 template <int kType, int kGroups>
 int LaunchSecond(const LayerArgs& a, cudaStream_t stream) {
   static thread_local int configured_device = -1;
-  if (const cudaError_t e = Configure(SecondKernel<kType, kGroups>, configured_device, 128 * 1024); e != cudaSuccess) {
+  if (const cudaError_t e = Configure(SecondKernel<kType, kGroups>, configured_device, 160 * 1024); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
   // sixteen warps a tile while there are no more tiles than SMs, else eight, two CTAs an SM
   const int warps = a.tiles_down <= SmCount() ? kSecondWarps : kSecondWarps / 2;
-  const int smem = (warps * kSlots * BlockBytes(kStep / kGroups)) + (a.tokens * a.used * kParts * kTileRows * 4);
+  const int smem = (warps * kSecondSlots * BlockBytes(kStep / kGroups)) + (a.tokens * a.used * kParts * kTileRows * 4);
   const cudaError_t e = LaunchPdl(SecondKernel<kType, kGroups>, dim3(static_cast<unsigned>(a.tiles_down)),
                                   dim3(static_cast<unsigned>(warps * 32)), static_cast<std::size_t>(smem), stream, a);
   return e == cudaSuccess ? 0 : Failed(e, "moe_layer down launch");
@@ -918,8 +958,11 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.prefetch_down = static_cast<double>(std::min(experts, d.tokens * d.used)) * a.tiles_down * a.steps_down * a.block_down <= 32e6;
   a.cap = d.tokens;
   a.group_cap = std::min(d.tokens, GroupTokens(d.x_type));
-  while (a.cap > 1 && FirstLayout(BlockBytes(d.gate_up.group), a.cap, a.group_cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes >
-                          kFirstSmemLimit) {
+  auto bytes = [&](int slots) {
+    return FirstLayout(BlockBytes(d.gate_up.group), slots, a.cap, a.group_cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes;
+  };
+  a.slots = bytes(kManySlots) <= kFirstSmemLimit ? kManySlots : kFewSlots;
+  while (a.cap > 1 && bytes(a.slots) > kFirstSmemLimit) {
     --a.cap;
     a.group_cap = std::min(a.group_cap, a.cap);
   }

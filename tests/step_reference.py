@@ -82,8 +82,8 @@ def choose(logits, used, score, bias, renormalize, scale):
 def moe(x, router, bias, gate_up, down, used, score, renormalize, scale, glu_name, limit, group_up, group_down):
     """(y, its slack, ids, weights, their slack)."""
     logits = x.double() @ router.double().T
-    # a 32-value block's products are added in F32 for each pair of pieces, the blocks and pairs in 64 bits
-    logit_slack = (x.double().abs() @ router.double().abs().T).amax() * 34 * 2 * U
+    # up to 128 values' products are added in F32 for each pair of pieces, these sums in 64 bits
+    logit_slack = (x.double().abs() @ router.double().abs().T).amax() * 130 * 2 * U
     ids, weights = choose(logits, used, score, bias, renormalize, scale)
     # p moves by exp of twice the logits' error, expf and the sums' roundings; renormalizing doubles that
     weight_slack = weights.abs() * (4 * logit_slack + 2 * (router.shape[0] / 32 + 24) * U)
