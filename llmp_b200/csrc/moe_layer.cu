@@ -96,7 +96,7 @@ struct FirstShared {
   Choice choice;
 };
 
-// Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums), two buffers of partial sums, the staged tokens and a column of zeros, logits.
+// Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums), two buffers of partial sums, the staged tokens, logits.
 struct FirstLayout {
   int ring, meet, staged, logits, bytes;
   __host__ __device__ FirstLayout(int block_bytes, int slots, int cap, int group_cap, int pieces, int x_pitch, int tokens, int experts) {
@@ -105,7 +105,7 @@ struct FirstLayout {
     if (ring < before) ring = (before + 255) / 256 * 256;
     meet = ring;
     staged = meet + (2 * kWarps * kTileRows * group_cap * 4);
-    logits = staged + (((cap * pieces) + 1) * x_pitch);
+    logits = staged + (cap * pieces * x_pitch);
     bytes = logits + (tokens * experts * 4);
   }
 };
@@ -128,7 +128,7 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
 #pragma unroll
   for (int nt = 0; nt < kTiles; ++nt) {
     const int token = ((first_tile + nt) * TokensATile(kPieces)) + (g / Cols(kPieces));
-    const int c = token < tokens && piece < kPieces ? (token * kPieces) + piece : a.cap * kPieces;
+    const int c = token < tokens && piece < kPieces ? (token * kPieces) + piece : 0;  // (a column that nobody reads)
     column[nt] = staged + (c * a.x_pitch) + (t * 16);
   }
   const int row_a = first_expert + g, row_b = row_a + 8;
@@ -171,6 +171,7 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
 #pragma unroll
   for (int nt = 0; nt < kTiles; ++nt) {
     double v[2][2];
+    if (kPieces == 3 && (t & 1) != 0) total[nt][1] = total[nt][3] = 0.0;  // the fourth column stands for nothing
     if constexpr (kPieces == 1) {
       v[0][0] = total[nt][0], v[0][1] = total[nt][1], v[1][0] = total[nt][2], v[1][1] = total[nt][3];
     } else {
@@ -379,9 +380,6 @@ FirstKernel(const LayerArgs a) {
       }
     }
   }
-  for (int i = tid; i < a.x_pitch / 16; i += kThreads) {
-    *reinterpret_cast<uint4*>(staged + (a.cap * kPieces * a.x_pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
-  }
   for (int e = tid; e < a.experts; e += kThreads) s.mask[e] = 0;
   GridDependencyWait();
 
@@ -505,16 +503,19 @@ FirstKernel(const LayerArgs a) {
     std::uint8_t* ring = smem + (warp * slots * kBlock);
     // where the next request reads
     int load_group = first_round / rounds_a_group, load_pair = first_round % rounds_a_group;
-    int load_rounds = end_round - first_round, load_left = 0;
+    int load_rounds = steps > 0 ? end_round - first_round : 0, load_left = 0;
     const std::uint8_t* src = nullptr;
+    const std::size_t tile_bytes = static_cast<std::size_t>(a.steps_up) * kBlock;
     auto next_load_round = [&]() {  // the next round in which this warp has a tile
-      while (load_left == 0 && load_rounds > 0 && steps > 0) {
+      while (load_left == 0 && load_rounds > 0) {
         const int tile = (load_pair * round_tiles) + my_tile;
-        if (tile < a.tiles_up) {
-          src = a.gate_up + ((((static_cast<std::size_t>(s.choice.expert[load_group]) * a.tiles_up) + tile) * a.steps_up) + begin) * kBlock +
-                (lane * 16);
-          load_left = steps;
+        if (load_pair == 0 || src == nullptr) {
+          src = a.gate_up + ((static_cast<std::size_t>(s.choice.expert[load_group]) * a.tiles_up) + tile) * tile_bytes +
+                (static_cast<std::size_t>(begin) * kBlock) + (lane * 16);
+        } else {
+          src += (round_tiles * tile_bytes) - (static_cast<std::size_t>(steps) * kBlock);
         }
+        if (tile < a.tiles_up) load_left = steps;
         --load_rounds;
         if (++load_pair == rounds_a_group) load_pair = 0, ++load_group;
       }
@@ -542,7 +543,8 @@ FirstKernel(const LayerArgs a) {
     }
     const int piece = g % Cols(kPieces);
     int group = first_round / rounds_a_group, pair = first_round % rounds_a_group;
-    int slot = 0, buffer = 0, staged_group = -1;
+    int slot = 0, buffer = 0, staged_group = -1, column_group = -1, tiles = 1;
+    std::uint32_t column[kTiles];
     for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
       const int first = s.choice.first[group], count = s.choice.first[group + 1] - first;
       if (!all_staged && staged_group != group) {
@@ -552,14 +554,16 @@ FirstKernel(const LayerArgs a) {
         BarrierSync(5, kWarps * 32);
         staged_group = group;
       }
-      const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
-      std::uint32_t column[kTiles];
+      if (column_group != group) {
+        column_group = group;
+        tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
 #pragma unroll
-      for (int nt = 0; nt < kTiles; ++nt) {
-        const int c = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-        int row = a.cap * kPieces;
-        if (c < count && piece < kPieces) row = ((all_staged ? s.token[first + c] : c) * kPieces) + piece;
-        column[nt] = at.staged + (row * a.x_pitch) + (t4 * 16) + (begin * 256);
+        for (int nt = 0; nt < kTiles; ++nt) {
+          const int c = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
+          int row = 0;  // (a column that nobody reads)
+          if (c < count && piece < kPieces) row = ((all_staged ? s.token[first + c] : c) * kPieces) + piece;
+          column[nt] = at.staged + (row * a.x_pitch) + (t4 * 16) + (begin * 256);
+        }
       }
       Sums total[kTiles];
       if ((pair * round_tiles) + my_tile < a.tiles_up) {
@@ -702,16 +706,14 @@ SecondKernel(const LayerArgs a) {
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int c = (nt * TokensATile(kGlu)) + (g / Cols(kGlu));
-      columns.at[nt] = nullptr;
-      if (c < count && piece < kGlu) {
-        columns.at[nt] = a.h + (((static_cast<std::size_t>(choice.pairs[begin + c]) * kGlu) + piece) * a.inter) + (t4 * 8);
-      }
+      const bool real = c < count && piece < kGlu;  // (a column that nobody reads is the first pair's)
+      columns.at[nt] = a.h + (((static_cast<std::size_t>(choice.pairs[real ? begin + c : begin]) * kGlu) + (real ? piece : 0)) * a.inter) + (t4 * 8);
     }
     return columns;
   };
   auto fetch = [&](const unsigned short* column, int step, int b) {
     const int at = (step * kStep) + (32 * b);  // inter is whole 32-value blocks
-    if (column == nullptr || at >= a.inter) return make_uint4(0, 0, 0, 0);
+    if (at >= a.inter) return make_uint4(0, 0, 0, 0);
     return __ldcg(reinterpret_cast<const uint4*>(column + at));
   };
   auto next_item = [&](int item) {  // with a step to it

@@ -113,7 +113,6 @@ struct VectorArgs {
   int parts;          // warps that divide a tile's steps
   int rounds;         // of warps / parts tiles each
   int meet_floats;    // one buffer of partial sums
-  bool zero_column;
   const void* x;
   std::int64_t x_stride;
   bool x_vec;
@@ -167,12 +166,12 @@ VectorKernel(const VectorArgs a) {
   const int tiles_a_round = kWarps / a.parts;
   const int my_tile = warp / a.parts, part = warp % a.parts;
   const int begin = steps * part / a.parts, count = (steps * (part + 1) / a.parts) - begin;  // this warp's
-  const int pitch = Pitch(steps), columns = a.rows * kPieces;
+  const int pitch = Pitch(steps);
   const bool multiplies = warp < kWarps;
   const std::uint32_t ring = SharedAddress(smem) + (warp * kSlots * kBlock) + (lane * 16);  // + this lane's piece
   float* meet = reinterpret_cast<float*>(smem + (kWarps * kSlots * kBlock));  // [2][warps][rows][16]
   const std::uint32_t staged_at = (kWarps * kSlots * kBlock) + (2 * a.meet_floats * 4);
-  std::uint8_t* staged = smem + staged_at;  // and a column of zeros
+  std::uint8_t* staged = smem + staged_at;
 
   // this warp's steps, round after round: where the next request reads
   const int first_tile = (first_round * tiles_a_round) + my_tile;
@@ -207,11 +206,6 @@ VectorKernel(const VectorArgs a) {
 
   const int octets = steps * (kStep / 8), x0 = step0 * kStep;
   auto row_of = [&](int token) { return static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType)); };
-  if (a.zero_column) {
-    for (int i = tid; i < octets; i += threads) {
-      *reinterpret_cast<uint4*>(staged + (columns * pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
-    }
-  }
   if constexpr (kType == kF32) {
     // twice over the rows, four octets of a thread in flight at once: the largest magnitudes, then the pieces
     if (tid < kMaxRows) magnitude[tid] = 0;
@@ -259,13 +253,13 @@ VectorKernel(const VectorArgs a) {
 
   // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
   if (multiplies) {
-    // this lane's column of each column tile: the token and piece it stands for, or the zeros
+    // this lane's column of each column tile: the token and piece it stands for (or one that nobody reads)
     const int piece = g % Cols(kPieces);
     std::uint32_t column[kTiles];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-      column[nt] = staged_at + ((token < a.rows ? (token * kPieces) + piece : columns) * pitch) + (t * 16) + (begin * 256);
+      column[nt] = staged_at + ((token < a.rows ? (token * kPieces) + piece : 0) * pitch) + (t * 16) + (begin * 256);
     }
     int slot = 0, buffer = 0;
     for (int round = first_round, n = 0; round < a.rounds; round += clusters, buffer ^= 1, ++n) {
@@ -347,13 +341,10 @@ VectorKernel(const VectorArgs a) {
 
 constexpr int kSmemLimit = 226 * 1024, kSmemOfTwo = 112 * 1024;
 constexpr int kMaxRanks = 8;
-// Shared memory of a CTA: rings, two buffers of sums, the staged activations (and a column of zeros, unless
-// they fill every column tile).
-bool ZeroColumn(int rows, int type) { return type == kF32 ? rows % 4 != 0 : rows % 8 != 0; }
+// Shared memory of a CTA: rings, two buffers of sums, the staged activations.
 std::int64_t SmemBytes(bool wide, int ranks, int rows, int steps, int type, int block_bytes) {
-  const int columns = (rows * HalfPieces(type)) + (ZeroColumn(rows, type) ? 1 : 0);
   return (static_cast<std::int64_t>(Warps(wide)) * Slots(wide) * block_bytes) + (2 * Warps(wide) * kTileRows * rows * 4) +
-         (columns * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
+         (rows * HalfPieces(type) * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
 }
 
 template <int kTiles, int kType, int kGroups, bool kWide>
@@ -395,7 +386,6 @@ int LaunchPlanned(VectorArgs a, cudaStream_t stream) {
   auto bytes = [&](bool wide, int ranks) {
     return SmemBytes(wide, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
   };
-  a.zero_column = ZeroColumn(a.rows, kType);
   if (const std::int64_t smem = bytes(false, 1); smem <= kSmemOfTwo) {
     return LaunchVector<kTiles, kType, kGroups, false>(a, 1, smem, stream);
   }

@@ -390,10 +390,12 @@ __device__ __forceinline__ void FoldColumns(const Sums& sums, float (&values)[2]
     values[0][0] = total[0], values[0][1] = total[1], values[1][0] = total[2], values[1][1] = total[3];
   } else {
     constexpr float kSecond = kHalf ? 0x1p-11f : 1.0f;
+    // (the fourth column of three pieces stands for nothing and may hold anything)
+    if (kPieces == 3 && (threadIdx.x & 1) != 0) total[1] = total[3] = 0.0f;
     values[0][0] = fmaf(total[1], kSecond, total[0]);
     values[1][0] = fmaf(total[3], kSecond, total[2]);
     values[0][1] = values[1][1] = 0.0f;
-    if constexpr (kPieces == 3) {  // columns 0, 1 in an even lane, 2 (and a zero) in the next
+    if constexpr (kPieces == 3) {  // columns 0, 1 in an even lane, 2 in the next
 #pragma unroll
       for (int r = 0; r < 2; ++r) values[r][0] += __shfl_xor_sync(0xffffffffu, values[r][0], 1);
     }
