@@ -886,25 +886,37 @@ def decode_grouped(decoder: int, data: torch.Tensor, x: torch.Tensor, k: int, ou
 _FLOAT = {torch.float32: N.TYPE_F32, torch.float16: N.TYPE_F16, torch.bfloat16: N.TYPE_BF16}
 
 
-def _rows(t: torch.Tensor, what: str) -> int:
-    """The element type of a float [rows, values] tensor of the current device whose rows are contiguous."""
+def _rows(t: torch.Tensor, device: int, what: str) -> tuple[int, int]:
+    """(element type, elements between rows) of a float [rows, values] tensor of the current device, `device`,
+    whose rows are contiguous."""
     kind = _FLOAT.get(t.dtype) if isinstance(t, torch.Tensor) else None
-    if kind is None or t.dim() != 2 or not t.is_cuda:
-        raise Rejected(f"{what}: a CUDA F32, F16 or BF16 tensor of rows")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    if kind is None or t.get_device() != device or t.dim() != 2:
+        raise Rejected(f"{what}: rows of F32, F16 or BF16 on the current CUDA device")
+    between, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
         raise Rejected(f"{what}: contiguous rows")
-    if t.get_device() != torch.cuda.current_device():
-        raise Rejected(f"{what}: on the current device")
-    return kind
+    return kind, between
 
 
-def _out(out: torch.Tensor | None, rows: int, width: int, dtype, like: torch.Tensor, what: str):
+def _out(out: torch.Tensor | None, rows: int, width: int, like: torch.Tensor, device: int, what: str):
+    """(the output, its element type, elements between its rows)."""
     if out is None:
-        return torch.empty((rows, width), dtype=dtype, device=like.device)
-    _rows(out, what)
-    if tuple(out.shape) != (rows, width) or (rows > 1 and out.stride(0) < width):
+        return like.new_empty((rows, width)), _FLOAT[like.dtype], width
+    kind, between = _rows(out, device, what)
+    if out.shape != (rows, width) or (rows > 1 and between < width):
         raise Rejected(f"{what}: [{rows}, {width}]")
-    return out
+    return out, kind, between
+
+
+def _current(t: torch.Tensor, what: str) -> int:
+    """The current device, for a call whose first tensor is t."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise Rejected(f"{what}: a CUDA tensor")
+    return torch.cuda.current_device()
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class W4Matrix:
@@ -967,14 +979,14 @@ def w4_vector(w: W4Matrix, x: torch.Tensor, *, glu: int = GLU_NONE, limit: float
               out: torch.Tensor | None = None) -> torch.Tensor:
     """x F32, F16 or BF16 [rows <= 16, k] times 4-bit weights -> [rows, n] (glu: of gate and up
     products), in x's type or `out`'s."""
-    kind = _rows(x, "w4_vector x")
-    rows = x.shape[0]
-    if x.shape[1] != w.k or w.device != x.get_device():
+    device = _current(x, "w4_vector x")
+    kind, between = _rows(x, device, "w4_vector x")
+    rows, k = x.shape
+    if k != w.k or w.device != device:
         raise Rejected("w4_vector: x [rows, k] on the weights' device")
-    out = _out(out, rows, w.n, x.dtype, x, "w4_vector output")
-    p = N.W4Product(w.desc, x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0), rows, kind,
-                    _FLOAT[out.dtype], glu, limit)
-    N.check(N.lib().llmp_b200_w4_vector(C.byref(p), _stream()), "llmp_b200_w4_vector")
+    out, out_kind, out_between = _out(out, rows, w.n, x, device, "w4_vector output")
+    p = N.W4Product(w.desc, x.data_ptr(), between, out.data_ptr(), out_between, rows, kind, out_kind, glu, limit)
+    N.check(N.lib().llmp_b200_w4_vector(C.byref(p), _raw_stream(device)), "llmp_b200_w4_vector")
     return out
 
 
@@ -986,10 +998,11 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, gate_up: W4Matrix, down: W4
     router [experts, hidden] in F32, F16 or BF16, bias F32 [experts]; gate_up of [experts, 2 inter, hidden]
     (w4_relayout glu=True), down of [experts, hidden, inter].  Returns (y [tokens, hidden] in x's type or
     `out`'s, ids I32 [tokens, used], weights F32 [tokens, used])."""
-    kind, router_kind = _rows(x, "moe_layer x"), _rows(router, "moe_layer router")
+    device = _current(x, "moe_layer x")
+    kind, between = _rows(x, device, "moe_layer x")
+    router_kind, router_between = _rows(router, device, "moe_layer router")
     tokens, hidden = x.shape
-    device = x.get_device()
-    if hidden != gate_up.k or tuple(router.shape) != (gate_up.experts, hidden) or gate_up.device != device or \
+    if hidden != gate_up.k or router.shape != (gate_up.experts, hidden) or gate_up.device != device or \
             down.device != device:
         raise Rejected("moe_layer: x [tokens, hidden], router [experts, hidden] and experts on one device")
     if bias is not None:
@@ -998,16 +1011,16 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, gate_up: W4Matrix, down: W4
             raise Rejected("moe_layer: bias F32 [experts]")
     if not 1 <= used <= min(16, gate_up.experts) or tokens > 16:
         raise Rejected("moe_layer: 1 to 16 experts a token, no more than there are, 1 to 16 tokens")
-    out = _out(out, tokens, hidden, x.dtype, x, "moe_layer output")
-    ids = torch.empty((tokens, used), dtype=torch.int32, device=x.device)
-    weights = torch.empty((tokens, used), dtype=torch.float32, device=x.device)
+    out, out_kind, out_between = _out(out, tokens, hidden, x, device, "moe_layer output")
+    ids = x.new_empty((tokens, used), dtype=torch.int32)
+    weights = x.new_empty((tokens, used), dtype=torch.float32)
     L = N.lib()
-    scratch = torch.empty((int(L.llmp_b200_moe_layer_scratch(used, tokens, gate_up.n)),), dtype=torch.uint8, device=x.device)
-    d = N.MoeLayerDesc(x.data_ptr(), x.stride(0), router.data_ptr(), router.stride(0),
+    scratch = x.new_empty((int(L.llmp_b200_moe_layer_scratch(used, tokens, gate_up.n)),), dtype=torch.uint8)
+    d = N.MoeLayerDesc(x.data_ptr(), between, router.data_ptr(), router_between,
                        bias.data_ptr() if bias is not None else None, gate_up.desc, down.desc, out.data_ptr(),
-                       out.stride(0), ids.data_ptr(), weights.data_ptr(), scratch.data_ptr(), kind, router_kind,
-                       _FLOAT[out.dtype], tokens, used, score, int(renormalize), scale, glu, limit)
-    N.check(L.llmp_b200_moe_layer(C.byref(d), _stream()), "llmp_b200_moe_layer")
+                       out_between, ids.data_ptr(), weights.data_ptr(), scratch.data_ptr(), kind, router_kind,
+                       out_kind, tokens, used, score, int(renormalize), scale, glu, limit)
+    N.check(L.llmp_b200_moe_layer(C.byref(d), _raw_stream(device)), "llmp_b200_moe_layer")
     return out, ids, weights
 
 
@@ -1021,51 +1034,54 @@ def block_norm(block: torch.Tensor, residual: torch.Tensor | None = None, *, pre
     [rows, width], post and pre [width] of that type or F32; each but block may be None.  Returns (r, h), h
     None without pre; with q8 (F32 rows) (r, h, h's Q8_1 rows as quantize_q8 makes them).  out_residual
     may be residual."""
-    kind = _rows(block, "block_norm block")
-    rows, width = block.shape
-    device = block.get_device()
-    d = N.BlockNormDesc()
-    d.block, d.block_stride, d.rows, d.width, d.type = block.data_ptr(), block.stride(0), rows, width, kind
+    device = _current(block, "block_norm block")
+    kind, between = _rows(block, device, "block_norm block")
+    shape = rows, width = block.shape
+    residual_at, residual_between = None, 0
     if residual is not None:
-        if _rows(residual, "block_norm residual") != kind or residual.shape != block.shape:
+        residual_kind, residual_between = _rows(residual, device, "block_norm residual")
+        if residual_kind != kind or residual.shape != shape:
             raise Rejected("block_norm: a residual like the block's output")
-        d.residual, d.residual_stride = residual.data_ptr(), residual.stride(0)
+        residual_at = residual.data_ptr()
+    gate_at, gate_between = None, 0
     if gate is not None:
-        if gate.dim() == 1:
+        if isinstance(gate, torch.Tensor) and gate.dim() == 1:
             gate = gate.unsqueeze(0)
-        if _rows(gate, "block_norm gate") != kind or tuple(gate.shape) not in ((1, width), (rows, width)):
+        gate_kind, gate_between = _rows(gate, device, "block_norm gate")
+        if gate_kind != kind or gate.shape[1] != width or gate.shape[0] not in (1, rows):
             raise Rejected("block_norm: a gate [width] or [rows, width] of the rows' type")
-        d.gate, d.gate_stride = gate.data_ptr(), gate.stride(0) if gate.shape[0] > 1 else 0
-    d.weight_type = kind
-    for name, weight in (("post", post), ("pre", pre)):
-        if weight is None:
-            continue
-        if not isinstance(weight, torch.Tensor) or weight.get_device() != device or tuple(weight.shape) != (width,) or \
-                (weight.stride(0) != 1 and width > 1) or weight.dtype not in (block.dtype, torch.float32):
-            raise Rejected(f"block_norm: {name} [width] of the rows' type or F32")
-        setattr(d, name, weight.data_ptr())
-        d.weight_type = _FLOAT[weight.dtype]
-    if post is not None and pre is not None and post.dtype != pre.dtype:
+        if gate.shape[0] == 1:
+            gate_between = 0
+        gate_at = gate.data_ptr()
+    post_at, weight_kind = (None, kind) if post is None else _norm_weight(post, block, device)
+    pre_at, pre_kind = (None, weight_kind) if pre is None else _norm_weight(pre, block, device)
+    if post is not None and pre_kind != weight_kind:
         raise Rejected("block_norm: post and pre of one type")
     if pre is None and (out is not None or q8):
         raise Rejected("block_norm: a second norm's weight")
-    for t in (out_residual, out):
-        if t is not None and t.dtype != block.dtype:
-            raise Rejected("block_norm: outputs of the rows' type")
-    out_residual = _out(out_residual, rows, width, block.dtype, block, "block_norm out_residual")
-    d.out_residual, d.out_residual_stride = out_residual.data_ptr(), out_residual.stride(0)
-    blocks = None
+    if q8 and kind != N.TYPE_F32:
+        raise Rejected("block_norm: Q8_1 rows of F32 ones")
+    out_residual, r_kind, r_between = _out(out_residual, rows, width, block, device, "block_norm out_residual")
+    out_at, out_kind, out_between, blocks = None, kind, 0, None
     if pre is not None:
-        out = _out(out, rows, width, block.dtype, block, "block_norm output")
-        d.out, d.out_stride = out.data_ptr(), out.stride(0)
+        out, out_kind, out_between = _out(out, rows, width, block, device, "block_norm output")
+        out_at = out.data_ptr()
         if q8:
-            if kind != N.TYPE_F32:
-                raise Rejected("block_norm: Q8_1 rows of F32 ones")
-            blocks = torch.empty((rows, q8_1_row_blocks(width) * 36), dtype=torch.uint8, device=block.device)
-            d.q8 = blocks.data_ptr()
-    d.scale, d.offset, d.eps = scale, offset, eps
-    N.check(N.lib().llmp_b200_block_norm(C.byref(d), _stream()), "llmp_b200_block_norm")
+            blocks = block.new_empty((rows, q8_1_row_blocks(width) * 36), dtype=torch.uint8)
+    if r_kind != kind or out_kind != kind:
+        raise Rejected("block_norm: outputs of the rows' type")
+    d = N.BlockNormDesc(block.data_ptr(), between, residual_at, residual_between, gate_at, gate_between, post_at,
+                        pre_at, out_residual.data_ptr(), r_between, out_at, out_between,
+                        blocks.data_ptr() if blocks is not None else None, rows, width, kind, pre_kind, scale, offset, eps)
+    N.check(N.lib().llmp_b200_block_norm(C.byref(d), _raw_stream(device)), "llmp_b200_block_norm")
     return (out_residual, out, blocks) if q8 else (out_residual, out)
+
+
+def _norm_weight(weight: torch.Tensor, block: torch.Tensor, device: int) -> tuple[int, int]:
+    if not isinstance(weight, torch.Tensor) or weight.get_device() != device or weight.shape != block.shape[1:] or \
+            (weight.stride(0) != 1 and weight.shape[0] > 1) or weight.dtype not in (block.dtype, torch.float32):
+        raise Rejected("block_norm: norm weights [width] of the rows' type or F32")
+    return weight.data_ptr(), _FLOAT[weight.dtype]
 
 
 class Logprobs(NamedTuple):
@@ -1082,25 +1098,24 @@ def logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: i
     """Log probabilities and ranks of given tokens (I32 [rows, given <= 16] or None), the entropy and the
     `top` <= 32 largest of logits F32, F16 or BF16 [rows, vocab] (llmp_b200_logprobs).  Masked logits are
     -inf."""
-    kind = _rows(logits, "logprobs logits")
+    device = _current(logits, "logprobs logits")
+    kind, between = _rows(logits, device, "logprobs logits")
     rows, vocab = logits.shape
-    given = 0
+    given, tokens_at = 0, None
     if tokens is not None:
         _need(tokens, torch.int32, "logprobs tokens")
         if tokens.dim() != 2 or tokens.shape[0] != rows or not tokens.is_contiguous() or \
-                tokens.get_device() != logits.get_device():
+                tokens.get_device() != device:
             raise Rejected("logprobs: packed tokens I32 [rows, given] on the logits' device")
-        given = tokens.shape[1]
+        given, tokens_at = tokens.shape[1], tokens.data_ptr()
     if not 0 <= given <= 16 or not 0 <= top <= min(32, vocab):
         raise Rejected("logprobs: up to 16 given tokens a row and 32 alternatives, no more than there are logits")
-    device = logits.device
-    r = Logprobs(torch.empty((rows, given), dtype=torch.float32, device=device),
-                 torch.empty((rows, given), dtype=torch.int32, device=device),
-                 torch.empty((rows,), dtype=torch.float32, device=device),
-                 torch.empty((rows, top), dtype=torch.int32, device=device),
-                 torch.empty((rows, top), dtype=torch.float32, device=device))
-    d = N.LogprobsDesc(logits.data_ptr(), logits.stride(0), tokens.data_ptr() if given else None,
-                       r.logprobs.data_ptr(), r.ranks.data_ptr(), r.entropy.data_ptr(), r.top_ids.data_ptr(),
-                       r.top_logprobs.data_ptr(), rows, kind, vocab, given, top, temperature)
-    N.check(N.lib().llmp_b200_logprobs(C.byref(d), _stream()), "llmp_b200_logprobs")
-    return r
+    lp = logits.new_empty((rows, given), dtype=torch.float32)
+    ranks = logits.new_empty((rows, given), dtype=torch.int32)
+    entropy = logits.new_empty((rows,), dtype=torch.float32)
+    top_ids = logits.new_empty((rows, top), dtype=torch.int32)
+    top_lp = logits.new_empty((rows, top), dtype=torch.float32)
+    d = N.LogprobsDesc(logits.data_ptr(), between, tokens_at if given else None, lp.data_ptr(), ranks.data_ptr(),
+                       entropy.data_ptr(), top_ids.data_ptr(), top_lp.data_ptr(), rows, kind, vocab, given, top, temperature)
+    N.check(N.lib().llmp_b200_logprobs(C.byref(d), _raw_stream(device)), "llmp_b200_logprobs")
+    return Logprobs(lp, ranks, entropy, top_ids, top_lp)
