@@ -67,6 +67,7 @@ struct LayerArgs {
   int group_cap;      // tokens of a group
   int x_pitch;        // bytes of a staged piece of a token
   int slots;          // of the first kernel's rings
+  int router_rows;    // experts of a router tile: 16, or 8 where those would leave CTAs of the cluster without one
   int parts;          // warps that divide a tile's steps of hidden
   int round_tiles;    // tiles that a round's warps work on
   int block_down;     // bytes of a step of the down slab
@@ -131,7 +132,7 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
     const int c = token < tokens && piece < kPieces ? (token * kPieces) + piece : 0;  // (a column that nobody reads)
     column[nt] = staged + (c * a.x_pitch) + (t * 16);
   }
-  const int row_a = first_expert + g, row_b = row_a + 8;
+  const int row_a = first_expert + g, row_b = a.router_rows == 16 ? row_a + 8 : a.experts;
   const auto* base = static_cast<const std::uint8_t*>(a.router);
   const std::int64_t row_bytes = a.router_stride * TypeBytes(kRouter);
   const int blocks = a.hidden / 32, end = (warp + 1) * blocks / kWarps;
@@ -194,68 +195,91 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
   }
 }
 
-// The same of an F32 router for kFew tokens at a time on the multiply-add pipes: a value's pieces are joined again, a
-// lane's 8 products are added in F32, those sums in 64 bits.  (On the tensor core the router would have to be split in
+// The same of an F32 router for kFew tokens at a time on the multiply-add pipes (the staged
+// tokens c_first ..., x's first + c_first ...): a 16-bit value's pieces are joined again, a lane's 8 products are added in F32, those sums in 64 bits.  (On the tensor core the router would have to be split in
 // three; that alone took 4 K cycles, the whole of this 5 K with one token.)
-constexpr int kFew = 4;
+constexpr int kFew = 8;
 template <int kType>
 __device__ __forceinline__ void RouterFew(const LayerArgs& a, const std::uint8_t* smem, int staged, int first_expert,
-                                          int first_token, int tokens, int warp, int lane, double (&partial)[kTileRows][kMaxTokens]) {
+                                          int first, int c_first, int tokens, int warp, int lane, double (&partial)[kTileRows][kMaxTokens]) {
   constexpr int kPieces = BfloatPieces(kType), kRouter = kF32;
   constexpr int kBatch = 2;
   const int g = lane >> 2, t = lane & 3;
   double total[2][kFew];
 #pragma unroll
   for (int c = 0; c < kFew; ++c) total[0][c] = total[1][c] = 0.0;
-  const int row_a = first_expert + g, row_b = row_a + 8;
+  const int row_a = first_expert + g, row_b = a.router_rows == 16 ? row_a + 8 : a.experts;
   const auto* base = static_cast<const std::uint8_t*>(a.router);
   const std::int64_t row_bytes = a.router_stride * TypeBytes(kRouter);
   const int blocks = a.hidden / 32, end = (warp + 1) * blocks / kWarps;
-  for (int first = warp * blocks / kWarps; first < end; first += kBatch) {
+  for (int block = warp * blocks / kWarps; block < end; block += kBatch) {
     float va[kBatch][8], vb[kBatch][8];
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      const int at = (32 * (first + q)) + (8 * t);
-      Load8<kRouter>(base + (row_a * row_bytes), at, first + q < end && row_a < a.experts ? 8 : 0, a.router_vec, va[q]);
-      Load8<kRouter>(base + (row_b * row_bytes), at, first + q < end && row_b < a.experts ? 8 : 0, a.router_vec, vb[q]);
+      const int at = (32 * (block + q)) + (8 * t);
+      Load8<kRouter>(base + (row_a * row_bytes), at, block + q < end && row_a < a.experts ? 8 : 0, a.router_vec, va[q]);
+      Load8<kRouter>(base + (row_b * row_bytes), at, block + q < end && row_b < a.experts ? 8 : 0, a.router_vec, vb[q]);
     }
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      if (first + q >= end) break;
-#pragma unroll
-      for (int c = 0; c < kFew; ++c) {
-        if (first_token + c >= tokens) break;
+      if (block + q >= end) break;
+      auto multiply = [&](const float (&v)[8], int c) {
         float sum_a = 0.0f, sum_b = 0.0f;
-        uint4 x[kPieces];
-#pragma unroll
-        for (int s = 0; s < kPieces; ++s) {
-          x[s] = *reinterpret_cast<const uint4*>(smem + staged + ((((first_token + c) * kPieces) + s) * a.x_pitch) + ((first + q) * 64) + (t * 16));
-        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          float v = 0.0f;
-#pragma unroll
-          for (int s = kPieces - 1; s >= 0; --s) {
-            const std::uint32_t w = i < 2 ? x[s].x : i < 4 ? x[s].y : i < 6 ? x[s].z : x[s].w;
-            v += __uint_as_float((i & 1) != 0 ? w & 0xffff0000u : w << 16);
-          }
-          sum_a = fmaf(va[q][i], v, sum_a);
-          sum_b = fmaf(vb[q][i], v, sum_b);
+          sum_a = fmaf(va[q][i], v[i], sum_a);
+          sum_b = fmaf(vb[q][i], v[i], sum_b);
         }
         total[0][c] += sum_a;
         total[1][c] += sum_b;
+      };
+      if constexpr (kType == kF32) {
+        // from L1, where staging left them, four tokens' loads in flight: cheaper than joining three pieces
+#pragma unroll
+        for (int c4 = 0; c4 < kFew; c4 += 4) {
+          if (c_first + c4 >= tokens) break;
+          float v[4][8];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const std::int64_t token = first + min(c_first + c4 + c, tokens - 1);
+            Load8<kF32>(static_cast<const float*>(a.x) + (token * a.x_stride), (32 * (block + q)) + (8 * t), 8, a.x_vec, v[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) multiply(v[c], c4 + c);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < kFew; ++c) {
+          if (c_first + c >= tokens) break;
+          uint4 x[kPieces];
+#pragma unroll
+          for (int s = 0; s < kPieces; ++s) {
+            x[s] = *reinterpret_cast<const uint4*>(smem + staged + ((((c_first + c) * kPieces) + s) * a.x_pitch) + ((block + q) * 64) + (t * 16));
+          }
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[i] = 0.0f;
+#pragma unroll
+            for (int s = kPieces - 1; s >= 0; --s) {
+              const std::uint32_t w = i < 2 ? x[s].x : i < 4 ? x[s].y : i < 6 ? x[s].z : x[s].w;
+              v[i] += __uint_as_float((i & 1) != 0 ? w & 0xffff0000u : w << 16);
+            }
+          }
+          multiply(v, c);
+        }
       }
     }
   }
 #pragma unroll
   for (int c = 0; c < kFew; ++c) {
-    if (first_token + c >= tokens) break;
+    if (c_first + c >= tokens) break;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       double v = total[r][c];
       v += __shfl_xor_sync(0xffffffffu, v, 1);
       v += __shfl_xor_sync(0xffffffffu, v, 2);
-      if (t == 0) partial[g + (8 * r)][first_token + c] = v;
+      if (t == 0) partial[g + (8 * r)][c_first + c] = v;
     }
   }
 }
@@ -366,13 +390,18 @@ FirstKernel(const LayerArgs a) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
   GridLaunchDependents();
-  const int expert_tiles = (a.experts + 15) / 16;
+  const int round_tiles = a.round_tiles, tile_warps = kWarps / round_tiles;
+  const int rounds_a_group = (a.tiles_up + round_tiles - 1) / round_tiles;
+  const int my_tile = warp / tile_warps, part = warp % tile_warps;
+  const int begin = part < a.parts ? a.steps_up * part / a.parts : 0;
+  const int steps = part < a.parts ? (a.steps_up * (part + 1) / a.parts) - begin : 0;
+  const int router_rows = a.router_rows, expert_tiles = (a.experts + router_rows - 1) / router_rows;
   {  // this CTA's router rows into L2 while the kernel before ends
     const std::size_t row_bytes = static_cast<std::size_t>(a.hidden) * TypeBytes(a.router_type);
     const int lines = static_cast<int>((row_bytes + 127) / 128);
     for (int m = rank; m < expert_tiles; m += ranks) {
-      for (int i = tid; i < 16 * lines; i += kThreads) {
-        const int e = (m * 16) + (i / lines);
+      for (int i = tid; i < router_rows * lines; i += kThreads) {
+        const int e = (m * router_rows) + (i / lines);
         if (e < a.experts) {
           asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const std::uint8_t*>(a.router) +
                                                        (e * a.router_stride * TypeBytes(a.router_type)) + ((i % lines) * 128)));
@@ -398,13 +427,13 @@ FirstKernel(const LayerArgs a) {
           constexpr int kRouter = decltype(router)::value;
           if constexpr (kRouter == kF32) {  // by its type alone: a token's logits stay the same whatever its company
             for (int c = 0; c < count; c += kFew) {
-              RouterFew<kType>(a, smem, at.staged, m * 16, c, count, warp, lane, partial[warp]);
+              RouterFew<kType>(a, smem, at.staged, m * router_rows, first, c, count, warp, lane, partial[warp]);
             }
           } else {
           constexpr int kAtOnce = kTiles < 2 ? kTiles : 2;
           const int tiles = (count + TokensATile(kPieces) - 1) / TokensATile(kPieces);
           for (int nt = 0; nt < tiles; nt += kAtOnce) {
-            RouterTile<kType, kRouter, kAtOnce>(a, smem, at.staged, m * 16, nt, count, warp, lane, partial[warp]);
+            RouterTile<kType, kRouter, kAtOnce>(a, smem, at.staged, m * router_rows, nt, count, warp, lane, partial[warp]);
           }
           }
         };
@@ -421,12 +450,12 @@ FirstKernel(const LayerArgs a) {
       met = true;
       // eight threads a logit: each adds two warps' sums, all of them up in a fixed order, each stores to a rank
       for (int first_i = 0; first_i < 16 * count * 8; first_i += kThreads) {
-        const int i = first_i + tid, q = i % 8, row = (i / 8) % 16, c = (i / 8) / 16, e = (m * 16) + row;
+        const int i = first_i + tid, q = i % 8, row = (i / 8) % 16, c = (i / 8) / 16, e = (m * router_rows) + row;
         double sum = 0.0;
         if (c < count) sum = partial[2 * q][row][c] + partial[(2 * q) + 1][row][c];
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (c < count && q < ranks && e < a.experts) {
+        if (c < count && q < ranks && row < router_rows && e < a.experts) {
           cluster.map_shared_rank(logits, q)[((first + c) * a.experts) + e] = static_cast<float>(sum);
         }
       }
@@ -487,22 +516,21 @@ FirstKernel(const LayerArgs a) {
   __syncthreads();
 
   // ---- this CTA's rounds: a group's next tiles of 8 gate and 8 up rows, each divided among a few warps
-  const int round_tiles = a.round_tiles, tile_warps = kWarps / round_tiles;
-  const int rounds_a_group = (a.tiles_up + round_tiles - 1) / round_tiles;
-  const std::int64_t rounds = static_cast<std::int64_t>(s.choice.groups) * rounds_a_group;
-  const int first_round = static_cast<int>(rounds * blockIdx.x / gridDim.x);
-  const int end_round = static_cast<int>(rounds * (blockIdx.x + 1) / gridDim.x);
+  // (a division is some 150 cycles of everyone's latency here: these two, the rest before the dependency wait)
+  const unsigned int rounds = static_cast<unsigned int>(s.choice.groups * rounds_a_group);
+  const unsigned int quota = rounds / gridDim.x, extra = rounds - (quota * gridDim.x);
+  const int first_round = static_cast<int>((quota * blockIdx.x) + min(blockIdx.x, extra));
+  const int end_round = first_round + static_cast<int>(quota + (blockIdx.x < extra ? 1u : 0u));
+  const int first_group = static_cast<int>(static_cast<unsigned int>(first_round) / static_cast<unsigned int>(rounds_a_group));
+  const int first_pair = first_round - (first_group * rounds_a_group);
   const bool all_staged = a.tokens <= a.cap;
   float* meet = reinterpret_cast<float*>(smem + at.meet);
   const int meet_floats = kWarps * kTileRows * a.group_cap;
   if (warp < kWarps) {
-    const int my_tile = warp / tile_warps, part = warp % tile_warps;
-    const int begin = part < a.parts ? a.steps_up * part / a.parts : 0;
-    const int steps = part < a.parts ? (a.steps_up * (part + 1) / a.parts) - begin : 0;
     const int slots = a.slots;
     std::uint8_t* ring = smem + (warp * slots * kBlock);
     // where the next request reads
-    int load_group = first_round / rounds_a_group, load_pair = first_round % rounds_a_group;
+    int load_group = first_group, load_pair = first_pair;
     int load_rounds = steps > 0 ? end_round - first_round : 0, load_left = 0;
     const std::uint8_t* src = nullptr;
     const std::size_t tile_bytes = static_cast<std::size_t>(a.steps_up) * kBlock;
@@ -533,16 +561,8 @@ FirstKernel(const LayerArgs a) {
       CopyAsyncCommit();
     };
     for (int i = 0; i < slots - 1; ++i) request(i);
-    if (a.prefetch_down) {  // the named experts' down rows, on their way while this kernel works
-      const std::int64_t lines = static_cast<std::int64_t>(a.tiles_down) * a.steps_down * a.block_down / 128;  // an expert's
-      const std::int64_t all = lines * s.choice.groups, stride = static_cast<std::int64_t>(gridDim.x) * kWarps * 32;
-      for (std::int64_t i = (static_cast<std::int64_t>(blockIdx.x) * kWarps * 32) + tid; i < all; i += stride) {
-        const std::int64_t n = i / lines;
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(a.down + ((s.choice.expert[n] * lines) + (i - (n * lines))) * 128));
-      }
-    }
     const int piece = g % Cols(kPieces);
-    int group = first_round / rounds_a_group, pair = first_round % rounds_a_group;
+    int group = first_group, pair = first_pair;
     int slot = 0, buffer = 0, staged_group = -1, column_group = -1, tiles = 1;
     std::uint32_t column[kTiles];
     for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
@@ -610,9 +630,19 @@ FirstKernel(const LayerArgs a) {
       for (int i = tid - (kWarps * 32); i <= s.choice.groups; i += kReducers * 32) a.choice->first[i] = s.choice.first[i];
       if (tid == kWarps * 32) a.choice->groups = s.choice.groups;
     }
+    if (a.prefetch_down) {  // the named experts' down rows, on their way while this kernel works
+      const int lines = a.tiles_down * a.steps_down * (a.block_down / 64) / 2;  // of 128 bytes, an expert's
+      const int first_line = (static_cast<int>(blockIdx.x) * kReducers * 32) + tid - (kWarps * 32);
+      for (int n = 0; n < s.choice.groups; ++n) {
+        const std::uint8_t* rows = a.down + (static_cast<std::size_t>(s.choice.expert[n]) * a.tiles_down * a.steps_down * a.block_down);
+        for (int i = first_line; i < lines; i += static_cast<int>(gridDim.x) * kReducers * 32) {
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(rows + (static_cast<std::size_t>(i) * 128)));
+        }
+      }
+    }
     // a warp every other tile of the round; a lane a row of every fourth token
     const int row = lane & 7;
-    int group = first_round / rounds_a_group, pair = first_round % rounds_a_group, buffer = 0;
+    int group = first_group, pair = first_pair, buffer = 0;
     for (int round = first_round; round < end_round; ++round, buffer ^= 1) {
       BarrierSync(1 + buffer, kThreads);
       const int first = s.choice.first[group], count = s.choice.first[group + 1] - first;
@@ -942,6 +972,7 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.down = static_cast<const std::uint8_t*>(d.down.slab);
   a.experts = experts, a.used = d.used, a.tokens = d.tokens, a.hidden = hidden, a.inter = inter;
   a.tiles_up = Tiles(d.gate_up.n, 1), a.steps_up = Steps(hidden);
+  a.router_rows = experts <= 8 * kMaxCluster ? 8 : 16;
   a.tiles_down = Tiles(d.down.n, 0), a.steps_down = Steps(inter);
   a.glu = d.glu, a.limit = d.limit;
   a.y = d.y, a.y_stride = d.y_stride, a.y_type = d.y_type;
