@@ -678,8 +678,10 @@ size_t llmp_b200_w4_slab_bytes(int n, int k, int group, int experts, int glu);
  * code byte).  Queues one ordinary launch; a product after it on the stream sees the whole slab. */
 int llmp_b200_w4_relayout(const llmp_b200_w4_source* source, const llmp_b200_w4_matrix* matrix, void* stream);
 /* y[t] = W x[t] for 1 to 16 rows of activations (0: nothing is queued); with a GLU slab glu(gate x[t], up x[t]).
- * Codes and activations multiply exactly, sums are F32 (an F16 or F32 activation enters as the
- * bf16 values whose sum it is), the result is rounded once, to y's type.  y apart from x. */
+ * k up to 131072.  Codes and 16-bit activations multiply exactly, F32 ones within a unit of their last bit (within
+ * 2^-51 of the row's largest finite value where they are below 2^-29 of it); sums are F32, the result is
+ * rounded once, to y's type.  How a sum is divided depends on the number of rows, never on the other rows' values.
+ * y apart from x. */
 typedef struct llmp_b200_w4_product {
   llmp_b200_w4_matrix w;
   const void* x;
@@ -700,10 +702,9 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream);
  *     ties to the lowest index, a NaN below everything
  *   weights = p of those (renormalize: over their sum) * scale
  *   y[t] = sum_j weights[j] * down_e glu(gate_e x[t], up_e x[t]),  e = ids[t][j], added in slot order
- * Logits are exact products added in 64 bits block by block; expert sums are as llmp_b200_w4_vector's,
+ * Logits are added in 64 bits, up to 128 values at a time in F32; expert sums are F32 over exact products,
  * the GLU rows stay 16 bits wide (F32 activations: 24).  A token's results do not depend on the
- * others of the call, up to the passes that x takes through shared memory.  Each call that may overlap another
- * brings its own scratch; nothing in it outlives the call. */
+ * others of the call.  Each call that may overlap another brings its own scratch; nothing in it outlives the call. */
 #define LLMP_B200_SCORE_SOFTMAX 0
 #define LLMP_B200_SCORE_SIGMOID 1
 typedef struct llmp_b200_moe_layer_desc {

@@ -30,7 +30,8 @@ constexpr int kSecondSlots = 6;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxTokens = 16, kMaxUsed = 16, kMaxExperts = 512;
 constexpr int kMaxPairs = kMaxTokens * kMaxUsed;
-constexpr int kFirstSmemLimit = 196 * 1024;        // dynamic; the choice's lists are static
+constexpr int kFirstSmemLimit = 211 * 1024;        // dynamic; the choice's lists are static (one token of 16384 F32
+                                                   // values, 16 x 512 logits and rings of groups of 32 fit)
 
 // The choice as the first kernel leaves it for the second: groups of tokens that name one expert, experts in ascending
 // order, a group's (token, slot) pairs (t * used + j, in token order) being pairs[first[i]] .. pairs[first[i + 1] - 1].

@@ -22,8 +22,8 @@
 // comes before its scale and may be 15 * 128 times an activation, hence bf16's 2^-11 (taken back in
 // the result): it overflows only where the scaled product would.  F32 activations are two f16
 // pieces of the value times a power of two a row, which brings the row's largest finite value to 2^14..2^15: the second
-// piece 2^11 larger, the two within a unit of the value's last bit, and exact bf16 pieces (3, without
-// a scale) where values must not lose that.
+// piece 2^11 larger, the two within a unit of the value's last bit (below 2^-29 of the row's largest within 2^-51
+// of that), and exact bf16 pieces (3, without a scale) where values must not lose that.
 #ifndef LLMP_B200_CSRC_W4_CUH_
 #define LLMP_B200_CSRC_W4_CUH_
 

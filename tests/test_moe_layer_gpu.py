@@ -82,6 +82,13 @@ def test_more_tokens_than_are_staged_at_once(cuda):
     _check(cuda, ops, c, 2)
 
 
+def test_the_largest_shapes_that_are_taken(cuda):
+    """One F32 token of 16384 values a pass, 512 experts, groups of 32: all of a CTA's shared memory."""
+    import llmp_b200 as ops
+    c = _case(cuda, 14, 16, 512, 16384, 32, 32, 32, kind="f32")
+    _check(cuda, ops, c, 2)
+
+
 def test_ties_go_to_the_lowest_index(cuda):
     torch = cuda
     import llmp_b200 as ops

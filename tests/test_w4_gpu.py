@@ -59,6 +59,15 @@ def test_many_rows_of_weights_and_a_long_k(cuda):
     _check(cuda, ops, source, x, 40, 64)
 
 
+@pytest.mark.parametrize("kind,rows,k", [("bf16", 16, 4096), ("bf16", 16, 8192), ("f16", 9, 16384), ("f32", 16, 4096),
+                                         ("f32", 7, 12288), ("f32", 16, 16384), ("f32", 1, 131072)])
+@pytest.mark.parametrize("n,glu", [(40, "none"), (300, "none"), (133, "swiglu")])
+def test_activations_that_fill_shared_memory_or_a_cluster_s(cuda, kind, rows, k, n, glu):
+    import llmp_b200 as ops
+    source, x = _case(cuda, rows + n, rows, n, k, 128, kind=kind, glu=glu != "none")
+    _check(cuda, ops, source, x, n, 128, glu)
+
+
 def test_strides_alignment_and_outputs(cuda):
     torch = cuda
     import llmp_b200 as ops
