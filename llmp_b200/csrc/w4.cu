@@ -113,6 +113,8 @@ struct VectorArgs {
   int parts;          // warps that divide a tile's steps
   int rounds;         // of warps / parts tiles each
   int meet_floats;    // one buffer of partial sums
+  bool zero_column;   // behind the staged columns, for the MMA's columns that stand for no token: any values would
+                      // do, but zeros are faster (4096 -> 20480, one f16 row: 13.5 us against 17.3)
   const void* x;
   std::int64_t x_stride;
   bool x_vec;
@@ -206,6 +208,11 @@ VectorKernel(const VectorArgs a) {
 
   const int octets = steps * (kStep / 8), x0 = step0 * kStep;
   auto row_of = [&](int token) { return static_cast<const std::uint8_t*>(a.x) + (token * a.x_stride * TypeBytes(kType)); };
+  if (a.zero_column) {
+    for (int i = tid; i < octets; i += threads) {
+      *reinterpret_cast<uint4*>(staged + (a.rows * kPieces * pitch) + (i * 16)) = make_uint4(0, 0, 0, 0);
+    }
+  }
   if constexpr (kType == kF32) {
     // twice over the rows, four octets of a thread in flight at once: the largest magnitudes, then the pieces
     if (tid < kMaxRows) magnitude[tid] = 0;
@@ -253,13 +260,13 @@ VectorKernel(const VectorArgs a) {
 
   // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
   if (multiplies) {
-    // this lane's column of each column tile: the token and piece it stands for (or one that nobody reads)
+    // this lane's column of each column tile: the token and piece it stands for, or the zeros
     const int piece = g % Cols(kPieces);
     std::uint32_t column[kTiles];
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-      column[nt] = staged_at + ((token < a.rows ? (token * kPieces) + piece : 0) * pitch) + (t * 16) + (begin * 256);
+      column[nt] = staged_at + ((token < a.rows ? (token * kPieces) + piece : a.rows * kPieces) * pitch) + (t * 16) + (begin * 256);
     }
     int slot = 0, buffer = 0;
     for (int round = first_round, n = 0; round < a.rounds; round += clusters, buffer ^= 1, ++n) {
@@ -306,30 +313,38 @@ VectorKernel(const VectorArgs a) {
         const int tile = (round * tiles_a_round) + o;
         if (tile >= a.tiles) break;
         for (int token = ((warp - kWarps) * 8) + (lane >> 2); token < a.rows; token += Reducers(kWide) * 8) {
-          float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // four rows, or two gate rows and two up rows
+          float4 first = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // four rows, or two gate rows and two up rows
           for (int q = 0; q < ranks; ++q) {
             const float* p = (ranks > 1 ? cluster.map_shared_rank(meet, q) : meet) + (buffer * a.meet_floats) +
                              (((o * a.parts * a.rows) + token) * kTileRows) + lane_row;
-            const int far = glu ? 8 : 2;
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (glu) {
 #pragma unroll 4
-            for (int s = 0; s < a.parts; ++s, p += kTileRows * a.rows) {
-              const float2 v = *reinterpret_cast<const float2*>(p), u = *reinterpret_cast<const float2*>(p + far);
-              part[0] += v.x, part[1] += v.y, part[2] += u.x, part[3] += u.y;
+              for (int s = 0; s < a.parts; ++s, p += kTileRows * a.rows) {
+                const float2 v = *reinterpret_cast<const float2*>(p), u = *reinterpret_cast<const float2*>(p + 8);
+                sum.x += v.x, sum.y += v.y, sum.z += u.x, sum.w += u.y;
+              }
+            } else {
+#pragma unroll 8
+              for (int s = 0; s < a.parts; ++s, p += kTileRows * a.rows) {
+                const float4 v = *reinterpret_cast<const float4*>(p);
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+              }
             }
             float up = Up(kType != kBF16);  // (each rank's F32 activations have their own scale)
             if constexpr (kType == kF32) {
               up = PowerOfTwo(-ScaleExponent(ranks > 1 ? *cluster.map_shared_rank(&magnitude[token], q) : magnitude[token]));
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) sums[r] = fmaf(part[r], up, sums[r]);
+            first.x = fmaf(sum.x, up, first.x), first.y = fmaf(sum.y, up, first.y);
+            first.z = fmaf(sum.z, up, first.z), first.w = fmaf(sum.w, up, first.w);
           }
-          if (glu) sums[0] = Glu(a.glu, sums[0], sums[2], a.limit), sums[1] = Glu(a.glu, sums[1], sums[3], a.limit);
+          float out[4] = {first.x, first.y, first.z, first.w};
+          if (glu) out[0] = Glu(a.glu, first.x, first.z, a.limit), out[1] = Glu(a.glu, first.y, first.w, a.limit);
           const int row = (tile * (glu ? 8 : 16)) + lane_row;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if (row + r >= a.outputs || (glu && r >= 2)) break;
-            StoreValue(a.y, (token * a.y_stride) + row + r, a.y_type, sums[r]);
+            StoreValue(a.y, (token * a.y_stride) + row + r, a.y_type, out[r]);
           }
         }
       }
@@ -341,10 +356,13 @@ VectorKernel(const VectorArgs a) {
 
 constexpr int kSmemLimit = 226 * 1024, kSmemOfTwo = 112 * 1024;
 constexpr int kMaxRanks = 8;
-// Shared memory of a CTA: rings, two buffers of sums, the staged activations.
+// Shared memory of a CTA: rings, two buffers of sums, the staged activations (and a column of zeros, unless
+// they fill every column tile).
+bool ZeroColumn(int rows, int type) { return type == kF32 ? rows % 4 != 0 : rows % 8 != 0; }
 std::int64_t SmemBytes(bool wide, int ranks, int rows, int steps, int type, int block_bytes) {
+  const int columns = (rows * HalfPieces(type)) + (ZeroColumn(rows, type) ? 1 : 0);
   return (static_cast<std::int64_t>(Warps(wide)) * Slots(wide) * block_bytes) + (2 * Warps(wide) * kTileRows * rows * 4) +
-         (rows * HalfPieces(type) * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
+         (columns * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
 }
 
 template <int kTiles, int kType, int kGroups, bool kWide>
@@ -360,8 +378,17 @@ int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream
     configured_device = device;
   }
   const int ctas = std::max(1, SmCount() * (smem <= kSmemOfTwo ? 2 : 1) / ranks);
-  a.parts = kWarps;
-  while (a.parts > 1 && (a.parts > a.steps / ranks || a.tiles >= 4 * ctas * (2 * kWarps / a.parts))) a.parts /= 2;
+  // The busiest CTA's rounds times a warp's steps in one, a round costing about 0.7 of a step besides: many parts balance
+  // the CTAs where tiles are few, few parts make long runs where they are many, two rounds a CTA and more.
+  const int steps = a.steps / ranks;
+  double best = 0.0;
+  for (int parts = kWarps; parts >= 1; parts /= 2) {
+    if (parts > steps && parts > 1) continue;
+    const int rounds = (a.tiles + (kWarps / parts) - 1) / (kWarps / parts);
+    if (best != 0.0 && rounds < 2 * ctas) break;
+    const double cost = ((rounds + ctas - 1) / ctas) * (((steps + parts - 1) / parts) + 0.7);
+    if (best == 0.0 || cost < 0.97 * best) best = cost, a.parts = parts;
+  }
   a.rounds = (a.tiles + (kWarps / a.parts) - 1) / (kWarps / a.parts);
   a.meet_floats = kWarps * kTileRows * a.rows;
   cudaLaunchConfig_t config = {};
@@ -386,6 +413,7 @@ int LaunchPlanned(VectorArgs a, cudaStream_t stream) {
   auto bytes = [&](bool wide, int ranks) {
     return SmemBytes(wide, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
   };
+  a.zero_column = ZeroColumn(a.rows, kType);
   if (const std::int64_t smem = bytes(false, 1); smem <= kSmemOfTwo) {
     return LaunchVector<kTiles, kType, kGroups, false>(a, 1, smem, stream);
   }
