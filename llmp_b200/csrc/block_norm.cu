@@ -36,8 +36,9 @@ __device__ __forceinline__ float BlockSum(float v, float* shared) {
 
 // A CTA a row.  A thread holds kUnits units of eight values in registers from the first load to the
 // last store, every row operand's loads in flight together, so a row is read once and the kernel is bound by
-// memory where there are many rows (4096 rows of 4096 bf16 values with a gate a token: see the table of cases) and by
-// two reductions and a few trips to memory where there is one.  kVec: 16-byte loads (whole rows of eight
+// memory where there are many rows (4096 rows of 4096 bf16 values with a gate a token: 32 to 34 us, 5.0 to 5.3 TB/s, 76 to
+// 81 % of the copy rate) and by two reductions and three trips to memory where there is one (2560 F32 values: 2.6 us).
+// A thread a value 1024 threads apart, unpacked as it comes, took 395 and 9.2 us.  kVec: 16-byte loads (whole rows of eight
 // values, aligned); otherwise unit u's value i is column (8 u + i) threads + tid, so that a warp's
 // loads are still neighbours.
 template <int kType>

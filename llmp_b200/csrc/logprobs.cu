@@ -154,6 +154,10 @@ struct Part {  // of a row, by one CTA
 // maximum does (they look at their logits again, which L2 still holds), and a candidate's place is the number of
 // keys above its own.  Ranks are counted in the pass, the given logits being fetched before it.  Each CTA stores its
 // sums, counts and best keys into rank 0's shared memory, which joins them in rank order after one cluster barrier.
+//
+// Measured: 32000 bf16 logits, twenty alternatives 7.7 us, bound by its chain of barriers; 16 x 131072 F32 13.4 us; 2048 x
+// 32003 bf16 49 us (2.7 TB/s, issue slots 66 % full): some 10 instructions a logit, an exponential among them, and a
+// row's joining and alternatives, about a third as much again.
 template <int kType, int kGiven, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 LogprobsKernel(const llmp_b200_logprobs_desc a) {

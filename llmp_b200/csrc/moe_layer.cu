@@ -8,6 +8,10 @@
 // eighth of the experts, and meets through its own hardware barrier: 0.5 MB of router weights from
 // L2 a cluster instead of a kernel of its own or a grid barrier, and no counter that two calls
 // could share.  Then every CTA knows the choice and takes its share of (expert, tile) units.
+// What bounds it, 128 experts, top 8, 2048 x 768: one bf16 token 23 us, of which the first kernel's way to the choice is 8
+// (staging, the router's rows through one SM's share of L2, two cluster barriers, the picks one after the other),
+// its products 5 and the second kernel 7; sixteen tokens 105 us for 211 MB, issue slots 50 and 70 % full, 250 and 330
+// instructions a warp and step of 1.1 KB: the steps' own, and a round's or item's shares of addresses and meetings.
 // The second kernel's CTA owns 16 output rows and adds a token's experts up in slot order, so a
 // token's sums do not depend on the other tokens of the call.
 #include <cooperative_groups.h>
