@@ -125,10 +125,6 @@ struct VectorArgs {
   float limit;
 };
 
-// Staged activations: a column's values at a pitch of 64 more bytes than whole steps, so the two
-// columns that a quarter warp reads (64 bytes each) lie in different halves of the banks.
-__host__ __device__ constexpr int Pitch(int steps) { return (steps * kStep * 2) + 64; }
-
 // Persistent CTAs.  A round is a few tiles of 16 weight rows, each tile's steps divided among `parts`
 // warps, whose sums meet in shared memory: with one token a matrix of 4096 x 4096 is 8.7 MB in 256 tiles,
 // too few for a warp each.  The activations are staged (scaled, split) once a CTA.  Weights come
@@ -146,11 +142,6 @@ __host__ __device__ constexpr int Pitch(int steps) { return (steps * kStep * 2) 
 // every call, so that each CTA stages an eighth of the activations: 31 and 83 us for the last two, the clusters leave
 // SMs idle and their barrier waits for the copies in flight.)
 constexpr int kMaxRows = 16;
-// Two CTAs of eight warps an SM, or one of sixteen where the activations take the shared memory of both; rings of what fits.
-__host__ __device__ constexpr int Warps(bool wide) { return wide ? 16 : 8; }
-__host__ __device__ constexpr int Reducers(bool wide) { return wide ? 2 : 1; }
-__host__ __device__ constexpr int Slots(bool wide) { return wide ? 3 : 5; }
-__host__ __device__ constexpr int Threads(bool wide) { return (Warps(wide) + Reducers(wide)) * 32; }
 
 __device__ __forceinline__ void BarrierSync(int id, int threads) {
   asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
@@ -180,7 +171,7 @@ VectorKernel(const VectorArgs a) {
   const bool multiplies = warp < kWarps;
   const std::uint32_t ring = SharedAddress(smem) + (warp * kSlots * kBlock) + (lane * 16);  // + this lane's piece
   float* meet = reinterpret_cast<float*>(smem + (kWarps * kSlots * kBlock));  // [2][warps][rows][16]
-  const std::uint32_t staged_at = (kWarps * kSlots * kBlock) + (2 * a.meet_floats * 4);
+  const std::uint32_t staged_at = StagedAt(kWide, a.rows, kBlock);
   std::uint8_t* staged = smem + staged_at;
 
   // this warp's steps, round after round: where the next request reads
@@ -274,7 +265,7 @@ VectorKernel(const VectorArgs a) {
 #pragma unroll
     for (int nt = 0; nt < kTiles; ++nt) {
       const int token = (nt * TokensATile(kPieces)) + (g / Cols(kPieces));
-      column[nt] = staged_at + ((token < a.rows ? (token * kPieces) + piece : a.rows * kPieces) * pitch) + (t * 16) + (begin * 256);
+      column[nt] = staged_at + (StagedColumn(token, piece, a.rows, kPieces) * pitch) + (t * 16) + (begin * 256);
     }
     int slot = 0, buffer = 0;
     for (int round = first_round, n = 0; round < a.rounds; round += clusters, buffer ^= 1, ++n) {
@@ -364,14 +355,6 @@ VectorKernel(const VectorArgs a) {
 
 constexpr int kSmemLimit = 226 * 1024, kSmemOfTwo = 112 * 1024;
 constexpr int kMaxRanks = 8;
-// Shared memory of a CTA: rings, two buffers of sums, the staged activations (and a column of zeros, unless
-// they fill every column tile).
-bool ZeroColumn(int rows, int type) { return type == kF32 ? rows % 4 != 0 : rows % 8 != 0; }
-std::int64_t SmemBytes(bool wide, int ranks, int rows, int steps, int type, int block_bytes) {
-  const int columns = (rows * HalfPieces(type)) + (ZeroColumn(rows, type) ? 1 : 0);
-  return (static_cast<std::int64_t>(Warps(wide)) * Slots(wide) * block_bytes) + (2 * Warps(wide) * kTileRows * rows * 4) +
-         (columns * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
-}
 
 template <int kTiles, int kType, int kGroups, bool kWide>
 int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream) {
@@ -422,9 +405,9 @@ int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream
 template <int kTiles, int kType, int kGroups>
 int LaunchPlanned(VectorArgs a, cudaStream_t stream) {
   auto bytes = [&](bool wide, int ranks) {
-    return SmemBytes(wide, ranks, a.rows, a.steps, kType, BlockBytes(kStep / kGroups));
+    return SmemBytes(wide, ranks, a.rows, a.steps, HalfPieces(kType), BlockBytes(kStep / kGroups));
   };
-  a.zero_column = ZeroColumn(a.rows, kType);
+  a.zero_column = ZeroColumn(a.rows, HalfPieces(kType));
   if (const std::int64_t smem = bytes(false, 1); smem <= kSmemOfTwo) {
     return LaunchVector<kTiles, kType, kGroups, false>(a, 1, smem, stream);
   }
@@ -445,10 +428,11 @@ int LaunchGroups(int group, const VectorArgs& a, cudaStream_t stream) {
 
 template <int kType>
 int LaunchTiles(int group, const VectorArgs& a, cudaStream_t stream) {
-  constexpr int kTokens = TokensATile(HalfPieces(kType));
-  if (a.rows <= kTokens) return LaunchGroups<1, kType>(group, a, stream);
-  if (a.rows <= 2 * kTokens) return LaunchGroups<2, kType>(group, a, stream);
-  if constexpr (kTokens <= 4) return LaunchGroups<4, kType>(group, a, stream);
+  constexpr int kPieces = HalfPieces(kType);
+  const int tiles = ColumnTiles(a.rows, kPieces);
+  if (tiles == 1) return LaunchGroups<1, kType>(group, a, stream);
+  if (tiles == 2) return LaunchGroups<2, kType>(group, a, stream);
+  if constexpr (TokensATile(kPieces) <= 4) return LaunchGroups<4, kType>(group, a, stream);
   return Reject("w4_vector: too many rows");
 }
 
@@ -527,7 +511,7 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream) {
   // as many rows a launch as a cluster's shared memory takes: all of them but for very long ones
   const int block_bytes = w4::BlockBytes(p.w.group);
   int most = p.rows;
-  while (most > 1 && w4::SmemBytes(false, w4::kMaxRanks, most, a.steps, p.x_type, block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
+  while (most > 1 && w4::SmemBytes(false, w4::kMaxRanks, most, a.steps, w4::HalfPieces(p.x_type), block_bytes) > w4::kSmemLimit) most = (most + 1) / 2;
   for (int first = 0; first < p.rows; first += most) {
     a.rows = std::min(most, p.rows - first);
     a.x = static_cast<const std::uint8_t*>(p.x) + (first * p.x_stride * xb);

@@ -52,6 +52,39 @@ __host__ __device__ constexpr int TypeBytes(int t) { return t == kF32 ? 4 : 2; }
 __host__ __device__ constexpr int HalfPieces(int t) { return t == kF32 ? 2 : 1; }
 __host__ __device__ constexpr int BfloatPieces(int t) { return t == kF32 ? 3 : t == kF16 ? 2 : 1; }
 
+// Columns a token takes, tokens an MMA's 8 columns hold.
+__host__ __device__ constexpr int Cols(int pieces) { return pieces == 3 ? 4 : pieces; }
+__host__ __device__ constexpr int TokensATile(int pieces) { return 8 / Cols(pieces); }
+
+// ---- the vector product's shared memory (w4.cu): rings, two buffers of sums, the staged activations
+// Two CTAs of eight warps an SM, or one of sixteen where the activations take the shared memory of both; rings of what fits.
+__host__ __device__ constexpr int Warps(bool wide) { return wide ? 16 : 8; }
+__host__ __device__ constexpr int Reducers(bool wide) { return wide ? 2 : 1; }
+__host__ __device__ constexpr int Slots(bool wide) { return wide ? 3 : 5; }
+__host__ __device__ constexpr int Threads(bool wide) { return (Warps(wide) + Reducers(wide)) * 32; }
+// Staged activations: a column's values at a pitch of 64 more bytes than whole steps, so the two
+// columns that a quarter warp reads (64 bytes each) lie in different halves of the banks.
+__host__ __device__ constexpr int Pitch(int steps) { return (steps * kStep * 2) + 64; }
+// Column tiles that the kernel for `rows` rows multiplies, all of them: 1, 2 or 4.
+__host__ __device__ constexpr int ColumnTiles(int rows, int pieces) {
+  return rows <= TokensATile(pieces) ? 1 : rows <= 2 * TokensATile(pieces) ? 2 : 4;
+}
+// The staged column that an MMA column reads, for the token and piece that it stands for.  Where the tiles hold more tokens
+// than there are rows, a column of zeros follows the rows' for the tokens that are none.
+__host__ __device__ constexpr bool ZeroColumn(int rows, int pieces) {
+  return rows < ColumnTiles(rows, pieces) * TokensATile(pieces);
+}
+__host__ __device__ constexpr int StagedColumn(int token, int piece, int rows, int pieces) {
+  return token < rows ? (token * pieces) + piece : rows * pieces;
+}
+__host__ __device__ constexpr int StagedAt(bool wide, int rows, int block_bytes) {
+  return (Warps(wide) * Slots(wide) * block_bytes) + (2 * Warps(wide) * kTileRows * rows * 4);
+}
+constexpr std::int64_t SmemBytes(bool wide, int ranks, int rows, int steps, int pieces, int block_bytes) {
+  const int columns = (rows * pieces) + (ZeroColumn(rows, pieces) ? 1 : 0);
+  return StagedAt(wide, rows, block_bytes) + (columns * static_cast<std::int64_t>(Pitch((steps + ranks - 1) / ranks)));
+}
+
 // A product in bf16 leaves this much larger.
 __host__ __device__ constexpr float Up(bool half) { return half ? 1.0f : 0x1p+11f; }
 
@@ -173,10 +206,6 @@ __device__ __forceinline__ int ScaleExponent(std::uint32_t magnitude) {
   return min(126, 141 - static_cast<int>(magnitude >> 23));  // 14 - (exponent - 127); at least 14 - 127
 }
 __device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<std::uint32_t>(e + 127) << 23); }
-
-// Columns a token takes, tokens an MMA's 8 columns hold.
-__host__ __device__ constexpr int Cols(int pieces) { return pieces == 3 ? 4 : pieces; }
-__host__ __device__ constexpr int TokensATile(int pieces) { return 8 / Cols(pieces); }
 
 // c += A B, or c = A B (kFirst: no registers to clear); kHalf: f16 operands, else bf16.
 template <bool kHalf, bool kFirst>

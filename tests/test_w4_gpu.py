@@ -168,3 +168,21 @@ def test_relayout_and_product_back_to_back(cuda):
         m = ops.w4_relayout(*source)
         slabs.append(m)
         assert torch.equal(ops.w4_vector(m, x), want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [4, 6, 7, 10, 11, 12, 13, 14, 15])
+def test_the_other_row_counts(cuda, kind, rows):
+    """With those above every count from 1 to 16: rows that do and do not fill the MMAs' columns."""
+    import llmp_b200 as ops
+    source, x = _case(cuda, 40 + rows, rows, 77, 704, 64, kind=kind)
+    _check(cuda, ops, source, x, 77, 64)
+
+
+@pytest.mark.parametrize("kind,rows,k", [("f32", 12, 2048), ("f32", 12, 4096), ("f32", 12, 8192), ("f32", 12, 16384),
+                                         ("f32", 13, 4096), ("f16", 12, 8192), ("bf16", 15, 16384)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_rows_that_leave_columns_spare_beside_full_shared_memory(cuda, kind, rows, k, group):
+    import llmp_b200 as ops
+    source, x = _case(cuda, rows + k, rows, 133, k, group, kind=kind)
+    _check(cuda, ops, source, x, 133, group)
