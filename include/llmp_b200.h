@@ -681,7 +681,7 @@ int llmp_b200_w4_relayout(const llmp_b200_w4_source* source, const llmp_b200_w4_
  * k up to 131072.  Codes and 16-bit activations multiply exactly, F32 ones within a unit of their last bit (within
  * 2^-51 of the row's largest finite value where they are below 2^-29 of it); sums are F32, the result is
  * rounded once, to y's type.  How a sum is divided depends on the number of rows, never on the other rows' values.
- * y apart from x. */
+ * A NaN among gate or up survives the GLU's clamps.  y apart from x. */
 typedef struct llmp_b200_w4_product {
   llmp_b200_w4_matrix w;
   const void* x;
@@ -704,7 +704,8 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream);
  *   y[t] = sum_j weights[j] * down_e glu(gate_e x[t], up_e x[t]),  e = ids[t][j], added in slot order
  * Logits are added in 64 bits, up to 128 values at a time in F32; expert sums are F32 over exact products,
  * the GLU rows stay 16 bits wide (F32 activations: 24).  A token's results do not depend on the
- * others of the call.  Each call that may overlap another brings its own scratch; nothing in it outlives the call. */
+ * others of the call; a NaN stays one, in the GLU's clamps too.  Each call that may overlap another brings its
+ * own scratch; nothing in it outlives the call. */
 #define LLMP_B200_SCORE_SOFTMAX 0
 #define LLMP_B200_SCORE_SIGMOID 1
 typedef struct llmp_b200_moe_layer_desc {

@@ -663,7 +663,7 @@ FirstKernel(const LayerArgs a) {
           }
           constexpr int kGlu = GluPieces(kType);
           std::uint32_t bits[kGlu];
-          Split<kGlu>(Glu(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
+          Split<kGlu>(GluOf(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
           unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[first + c]) * kGlu * a.inter) + out;
 #pragma unroll
           for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);

@@ -338,7 +338,7 @@ VectorKernel(const VectorArgs a) {
             first.z = fmaf(sum.z, up, first.z), first.w = fmaf(sum.w, up, first.w);
           }
           float out[4] = {first.x, first.y, first.z, first.w};
-          if (glu) out[0] = Glu(a.glu, first.x, first.z, a.limit), out[1] = Glu(a.glu, first.y, first.w, a.limit);
+          if (glu) out[0] = GluOf(a.glu, first.x, first.z, a.limit), out[1] = GluOf(a.glu, first.y, first.w, a.limit);
           const int row = (tile * (glu ? 8 : 16)) + lane_row;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {

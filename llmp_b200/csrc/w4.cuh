@@ -107,6 +107,16 @@ __device__ __forceinline__ void StoreValue(void* p, std::int64_t i, int type, fl
   }
 }
 
+// common.cuh's GLU with clamps that keep a NaN: fminf and fmaxf, as the reference's products have them, return the
+// other operand, and a gate that is no number would come out as silu(limit).
+__device__ __forceinline__ float GluOf(int glu, float gate, float up, float limit) {
+  if (glu != LLMP_B200_GLU_SWIGLU_CLAMP) return Glu(glu, gate, up, limit);
+  gate = gate > limit ? limit : gate;
+  up = up > limit ? limit : up;
+  up = up < -limit ? -limit : up;
+  return Silu(gate) * up;
+}
+
 // The pieces of x, in bf16 bits: truncations, so each remainder is exact and none overflows.
 template <int kPieces>
 __device__ __forceinline__ void Split(float x, std::uint32_t (&bits)[kPieces]) {

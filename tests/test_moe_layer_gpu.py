@@ -170,3 +170,18 @@ def test_two_streams_at_once_and_a_graph(cuda):
         graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b.flip(0)) for a, b in zip(held, want))
+
+
+@pytest.mark.parametrize("glu", ["swiglu", "swiglu_clamp", "geglu"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_a_nan_of_an_expert_reaches_the_tokens_that_name_it(cuda, glu, kind):
+    torch = cuda
+    import llmp_b200 as ops
+    c = _case(torch, 15, 9, 12, 256, 64, kind=kind)
+    c["gate_up"][1][3, 7, 1] = float("nan")         # a scale of expert 3's gate row 7
+    c["gate_up"][1][8, 64 + 20, 0] = float("nan")   # of expert 8's up row 20
+    y, ids, weights = ops.moe_layer(c["x"], c["router"], ops.w4_relayout(*c["gate_up"], glu=True), ops.w4_relayout(*c["down"]), 3,
+                                    glu=ref.GLUS[glu], limit=0.5 if glu == "swiglu_clamp" else 0.0)
+    named = ((ids == 3) | (ids == 8)).any(-1)
+    assert bool(named.any() and not named.all() and weights.isfinite().all())
+    assert torch.equal(y.isnan(), named[:, None].expand_as(y))

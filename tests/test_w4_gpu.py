@@ -186,3 +186,21 @@ def test_rows_that_leave_columns_spare_beside_full_shared_memory(cuda, kind, row
     import llmp_b200 as ops
     source, x = _case(cuda, rows + k, rows, 133, k, group, kind=kind)
     _check(cuda, ops, source, x, 133, group)
+
+
+@pytest.mark.parametrize("glu", ["swiglu", "swiglu_clamp", "geglu"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_a_nan_survives_the_glu(cuda, glu, kind):
+    """In an activation, in a gate row's scale, in an up row's: silu(limit) * limit is no answer to any of them."""
+    torch = cuda
+    import llmp_b200 as ops
+    n, k, group = 40, 256, 64
+    source, x = _case(torch, 9, 3, n, k, group, kind=kind, glu=True)
+    x[1, 31] = float("nan")
+    source[1][5, 2] = float("nan")              # a group of gate row 5
+    source[1][n + 17, 0] = float("nan")         # of up row 17
+    limit = 0.5 if glu == "swiglu_clamp" else 0.0
+    y = ops.w4_vector(ops.w4_relayout(*source, glu=True), x, glu=ref.GLUS[glu], limit=limit)
+    want = torch.zeros((3, n), dtype=torch.bool, device="cuda")
+    want[1], want[:, 5], want[:, 17] = True, True, True
+    assert torch.equal(y.isnan(), want)
