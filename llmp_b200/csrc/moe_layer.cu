@@ -68,6 +68,7 @@ struct LayerArgs {
   float* weights;
   Choice* choice;
   unsigned short* h;  // bf16 pieces of the GLU rows: [pair][piece][inter]
+  int glu_pieces;     // of them, 2 or 3
   int cap;            // tokens staged at a time
   int group_cap;      // tokens of a group
   int x_pitch;        // bytes of a staged piece of a token
@@ -82,8 +83,24 @@ struct LayerArgs {
 // Column tiles that a group's tokens take in the products: one or two, in registers.
 __host__ __device__ constexpr int GroupTokens(int type) { return type == kF32 ? 4 : 8; }
 __host__ __device__ constexpr int GroupTiles(int tokens, int pieces) { return (tokens + TokensATile(pieces) - 1) / TokensATile(pieces); }
-// Pieces of a GLU value: 16-bit activations keep 16 bits of it, F32 ones all 24.
-__host__ __device__ constexpr int GluPieces(int type) { return type == kF32 ? 3 : 2; }
+// bf16 pieces that a GLU value travels in between the kernels.  Three hold all 24 bits of its F32 form: where activations or
+// output are F32.  Two, each rounded to nearest, are within 2^-17 of it, which a 16-bit output rounds away (half its
+// step is 2^-9 or 2^-12): four tokens instead of two fill an MMA's columns (sixteen bf16 tokens, 128 experts, top 8,
+// 2048 x 768: 106 us, with three pieces 120; one token 22.8 and 24.0).
+constexpr int GluPieces(int x_type, int y_type) { return x_type == kF32 || y_type == kF32 ? 3 : 2; }
+// The two: a first that would round to infinity is cut off, the second then holds the rest.
+__device__ __forceinline__ void SplitNearest(float x, std::uint32_t (&bits)[2]) {
+  const std::uint32_t b = __float_as_uint(x), magnitude = b & 0x7fffffffu;
+  if (magnitude >= 0x7f800000u) {
+    Split<2>(x, bits);
+    return;
+  }
+  std::uint32_t first = magnitude + 0x7fffu + ((magnitude >> 16) & 1u);
+  if (first >= 0x7f800000u) first = magnitude;
+  first = (first | (b & 0x80000000u)) & 0xffff0000u;
+  bits[0] = first >> 16;
+  bits[1] = __bfloat16_as_ushort(__float2bfloat16_rn(x - __uint_as_float(first)));
+}
 
 // Unsigned order of floats: NaN below everything, the two zeros alike; 0 is no float's.
 __device__ __forceinline__ std::uint32_t OrderKey(float v) {
@@ -661,12 +678,22 @@ FirstKernel(const LayerArgs a) {
             gate += p[((q * a.group_cap) + c) * kTileRows];
             up += p[(((q * a.group_cap) + c) * kTileRows) + 8];
           }
-          constexpr int kGlu = GluPieces(kType);
-          std::uint32_t bits[kGlu];
-          Split<kGlu>(GluOf(a.glu, gate * Up(false), up * Up(false), a.limit), bits);
-          unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[first + c]) * kGlu * a.inter) + out;
+          const float value = GluOf(a.glu, gate * Up(false), up * Up(false), a.limit);
+          const int glu_pieces = kType == kF32 ? 3 : a.glu_pieces;
+          unsigned short* h = a.h + (static_cast<std::size_t>(s.choice.pairs[first + c]) * glu_pieces * a.inter) + out;
+          auto store = [&](auto& bits) {
 #pragma unroll
-          for (int q = 0; q < kGlu; ++q) h[static_cast<std::size_t>(q) * a.inter] = static_cast<unsigned short>(bits[q]);
+            for (std::uint32_t b : bits) *h = static_cast<unsigned short>(b), h += a.inter;
+          };
+          if (glu_pieces == 3) {
+            std::uint32_t bits[3];
+            Split<3>(value, bits);
+            store(bits);
+          } else {
+            std::uint32_t bits[2];
+            SplitNearest(value, bits);
+            store(bits);
+          }
         }
       }
       BarrierArrive(3 + buffer, kThreads);
@@ -681,11 +708,10 @@ FirstKernel(const LayerArgs a) {
 constexpr int kParts = 2;
 constexpr int kSecondWarps = 16;
 
-template <int kType, int kGroups>
+template <int kTokens, int kGlu, int kGroups>
 __global__ void __launch_bounds__(kSecondWarps * 32, 1)
 SecondKernel(const LayerArgs a) {
-  constexpr int kGlu = GluPieces(kType);
-  constexpr int kTiles = GroupTiles(GroupTokens(kType), kGlu);
+  constexpr int kTiles = GroupTiles(kTokens, kGlu);
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ Choice choice;
@@ -896,16 +922,16 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   return e == cudaSuccess ? 0 : Failed(e, "moe_layer launch");
 }
 
-template <int kType, int kGroups>
+template <int kTokens, int kGlu, int kGroups>
 int LaunchSecond(const LayerArgs& a, cudaStream_t stream) {
   static thread_local int configured_device = -1;
-  if (const cudaError_t e = Configure(SecondKernel<kType, kGroups>, configured_device, 160 * 1024); e != cudaSuccess) {
+  if (const cudaError_t e = Configure(SecondKernel<kTokens, kGlu, kGroups>, configured_device, 160 * 1024); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
   // sixteen warps a tile while there are no more tiles than SMs, else eight, two CTAs an SM
   const int warps = a.tiles_down <= SmCount() ? kSecondWarps : kSecondWarps / 2;
   const int smem = (warps * kSecondSlots * BlockBytes(kStep / kGroups)) + (a.tokens * a.used * kParts * kTileRows * 4);
-  const cudaError_t e = LaunchPdl(SecondKernel<kType, kGroups>, dim3(static_cast<unsigned>(a.tiles_down)),
+  const cudaError_t e = LaunchPdl(SecondKernel<kTokens, kGlu, kGroups>, dim3(static_cast<unsigned>(a.tiles_down)),
                                   dim3(static_cast<unsigned>(warps * 32)), static_cast<std::size_t>(smem), stream, a);
   return e == cudaSuccess ? 0 : Failed(e, "moe_layer down launch");
 }
@@ -916,9 +942,17 @@ int LaunchLayer(int group_up, int group_down, const LayerArgs& a, cudaStream_t s
                : group_up == 64 ? LaunchFirst<kType, 2>(a, stream)
                                 : LaunchFirst<kType, 4>(a, stream);
   if (status != 0) return status;
-  status = group_down == 128  ? LaunchSecond<kType, 1>(a, stream)
-           : group_down == 64 ? LaunchSecond<kType, 2>(a, stream)
-                              : LaunchSecond<kType, 4>(a, stream);
+  auto second = [&](auto pieces) {
+    constexpr int kTokens = GroupTokens(kType), kGlu = decltype(pieces)::value;
+    return group_down == 128  ? LaunchSecond<kTokens, kGlu, 1>(a, stream)
+           : group_down == 64 ? LaunchSecond<kTokens, kGlu, 2>(a, stream)
+                              : LaunchSecond<kTokens, kGlu, 4>(a, stream);
+  };
+  if constexpr (kType == kF32) {
+    status = second(std::integral_constant<int, 3>{});
+  } else {
+    status = a.glu_pieces == 3 ? second(std::integral_constant<int, 3>{}) : second(std::integral_constant<int, 2>{});
+  }
   return status > 0 ? -1 : status;  // the first kernel is queued
 }
 
@@ -994,6 +1028,7 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.parts = std::min(tile_warps, a.steps_up);
   a.block_down = BlockBytes(d.down.group);
   a.prefetch_down = static_cast<double>(std::min(experts, d.tokens * d.used)) * a.tiles_down * a.steps_down * a.block_down <= 32e6;
+  a.glu_pieces = GluPieces(d.x_type, d.y_type);
   a.cap = d.tokens;
   a.group_cap = std::min(d.tokens, GroupTokens(d.x_type));
   auto bytes = [&](int slots) {

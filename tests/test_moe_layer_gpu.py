@@ -185,3 +185,44 @@ def test_a_nan_of_an_expert_reaches_the_tokens_that_name_it(cuda, glu, kind):
     named = ((ids == 3) | (ids == 8)).any(-1)
     assert bool(named.any() and not named.all() and weights.isfinite().all())
     assert torch.equal(y.isnan(), named[:, None].expand_as(y))
+
+
+@pytest.mark.parametrize("out", ["f16", "f32"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tokens", [1, 7])
+def test_how_wide_the_glu_rows_are(cuda, tokens, kind, out):
+    """Down is the identity and one expert has all the weight, so the result is the GLU row: rounded to F16 from within
+    2^-17 of it, and whole where activations or output are F32.  Each token has one value that is not zero, so gate and
+    up are single products of 8 bits, 4 bits and the activation's 11: exact, and what is lost is the GLU's."""
+    torch = cuda
+    import llmp_b200 as ops
+    size, group = 512, 64
+    c = _case(torch, 16, tokens, 1, size, size, group, group, kind=kind)
+    x = c["x"].to(torch.bfloat16 if kind == "bf16" else torch.float16).to(ref.TYPES[kind]) * 8
+    c["x"] = torch.where(torch.arange(size, device="cuda") == (torch.arange(tokens, device="cuda") * 67 + 5)[:, None], x, 0.0)
+    codes = torch.full((1, size, size // 2), 0x88, dtype=torch.uint8)      # the zero point: weights of nothing
+    at = torch.arange(size)
+    codes[0, at, at // 2] = torch.where(at % 2 == 0, 0x89, 0x98).to(torch.uint8)
+    down = ops.w4_relayout(codes.cuda(), torch.ones((1, size, size // group), dtype=torch.float16).cuda())
+    y = torch.empty((tokens, size), dtype=ref.TYPES[out], device="cuda")
+    ops.moe_layer(c["x"], c["router"], ops.w4_relayout(*c["gate_up"], glu=True), down, 1, out=y)
+    both = c["x"].double() @ ref.w4_values(*(a[0] for a in c["gate_up"])).T
+    none = torch.zeros_like(both)
+    h, h_slack = ref.glu_rows("swiglu", both[:, :size], none[:, :size], both[:, size:], none[:, size:], 0.0)
+    lost = 2.0 ** -23 if "f32" in (kind, out) else 2.0 ** -17
+    ref.assert_within(y, h, h_slack + h.abs() * lost)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("tokens,experts,used", [(1, 24, 4), (16, 24, 4), (16, 3, 2)])
+def test_an_f32_output_of_16_bit_activations(cuda, kind, group, tokens, experts, used):
+    """The same values' bounds in F32."""
+    torch = cuda
+    import llmp_b200 as ops
+    c = _case(torch, 17, tokens, experts, 384, 256, 64, group, kind=kind)
+    y = torch.empty((tokens, 384), device="cuda")
+    ops.moe_layer(c["x"], c["router"], ops.w4_relayout(*c["gate_up"], glu=True), ops.w4_relayout(*c["down"]), used, out=y)
+    want, slack, *_ = ref.moe(c["x"].float(), c["router"], None, c["gate_up"], c["down"], used, "softmax", True, 1.0, "swiglu",
+                              0.0, 64, group)
+    ref.assert_within(y, want, slack)
