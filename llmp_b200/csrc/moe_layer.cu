@@ -186,8 +186,12 @@ __device__ __forceinline__ void RouterTile(const LayerArgs& a, const std::uint8_
           Mma<false, false>(sum, qa[q][r].x, qb[q][r].x, qa[q][r].y, qb[q][r].y, x.x, x.y);
           Mma<false, false>(sum, qa[q][r].z, qb[q][r].z, qa[q][r].w, qb[q][r].w, x.z, x.w);
         }
+        // an infinity is its first piece alone: zeros times it in the sums of other pieces are no part of the product
 #pragma unroll
-        for (int c = 0; c < 4; ++c) total[nt][c] += sum[c];
+        for (int c = 0; c < 4; ++c) {
+          const bool first_pieces = r == 0 && ((2 * t) + (c & 1)) % Cols(kPieces) == 0;
+          if (first_pieces || isfinite(sum[c])) total[nt][c] += sum[c];
+        }
       }
     }
   }

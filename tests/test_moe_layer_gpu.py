@@ -226,3 +226,32 @@ def test_an_f32_output_of_16_bit_activations(cuda, kind, group, tokens, experts,
     want, slack, *_ = ref.moe(c["x"].float(), c["router"], None, c["gate_up"], c["down"], used, "softmax", True, 1.0, "swiglu",
                               0.0, 64, group)
     ref.assert_within(y, want, slack)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("router", ["f32", "bf16", "f16"])
+def test_infinities_in_the_router_s_product(cuda, kind, router):
+    """An infinite activation, or an infinite router value, makes a logit an infinity of its sign, no NaN."""
+    torch = cuda
+    import llmp_b200 as ops
+    c = _case(torch, 18, 11, 16, 512, 64, kind=kind, router=router)
+    gate_up, down = ops.w4_relayout(*c["gate_up"], glu=True), ops.w4_relayout(*c["down"])
+    for change in ("x", "router"):
+        x, weights = c["x"].clone(), c["router"].clone()
+        if change == "x":
+            x[3, 100], x[4, 7], x[10, 500] = float("inf"), -float("inf"), float("nan")
+        else:
+            weights[6, 33], weights[13, 400] = float("inf"), -float("inf")
+        logits = x.double() @ weights.double().T
+        assert bool(logits[:, 6].isinf().any())
+        _, ids, got = ops.moe_layer(x, weights, gate_up, down, 16, score=ops.SCORE_SIGMOID, renormalize=False)
+        finite = logits.isfinite().all(-1)
+        want, w = ref.choose(torch.where(logits.isnan(), -torch.inf, logits), 16, "sigmoid", None, False, 1.0)
+        plain = ~logits.isnan().any(-1)
+        assert torch.equal(ids[plain].long(), want[plain])
+        # (a logit's error, up to 130 unit roundings of its products' magnitudes, moves a sigmoid by a quarter of it)
+        slack = (x.double().abs().nan_to_num(posinf=0.0) @ weights.double().abs().nan_to_num(posinf=0.0).T).amax() * 130 * ref.U + 8 * ref.U
+        ref.assert_within(got[plain], w[plain], slack.expand_as(w)[plain])
+        if change == "x":
+            assert ids[10].tolist() == list(range(16)) and bool(got[10].isnan().all())
+            assert finite.sum() == 8
