@@ -863,10 +863,10 @@ cudaError_t Configure(Kernel kernel, int& configured_device, int smem) {
   return e;
 }
 
-// Clusters of `size` CTAs of the first kernel that the device holds at once (a GPC holds whole clusters: more would be a
+// Clusters of `size` CTAs of one first kernel that the device holds at once (a GPC holds whole clusters: more would be a
 // second wave).
-template <typename Kernel>
-int ResidentClusters(Kernel kernel, int size, int smem) {
+template <auto kKernel>
+int ResidentClusters(int size, int smem) {
   struct Known {
     int device = -1, size = 0, smem = -1, clusters = 1;
   };
@@ -886,7 +886,7 @@ int ResidentClusters(Kernel kernel, int size, int smem) {
   config.attrs = attribute;
   config.numAttrs = 1;
   int clusters = 0;
-  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) != cudaSuccess || clusters < 1) {
+  if (cudaOccupancyMaxActiveClusters(&clusters, kKernel, &config) != cudaSuccess || clusters < 1) {
     cudaGetLastError();
     clusters = std::max(1, SmCount() / (2 * size));
   }
@@ -907,7 +907,7 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   // Clusters of four fill more of the device's SMs (on B200 36 against 15 of eight), each working the whole router out:
   // worth it where the products outlast that.
   const int size = rounds > 8 * SmCount() ? kMaxCluster / 2 : kMaxCluster;
-  const std::int64_t most = ResidentClusters(FirstKernel<kType, kGroups>, size, smem);
+  const std::int64_t most = ResidentClusters<FirstKernel<kType, kGroups>>(size, smem);
   const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + size - 1) / size));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(clusters * size));
