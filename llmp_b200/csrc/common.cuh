@@ -80,12 +80,6 @@ __device__ __forceinline__ uint2 LoadStream8(const void* p) {
                : "l"(p));
   return v;
 }
-__device__ __forceinline__ std::uint32_t LoadStream4(const void* p) {
-  std::uint32_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
-
 __device__ __forceinline__ float HalfBitsToFloat(std::uint32_t bits16) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
 }

@@ -393,13 +393,6 @@ __device__ __forceinline__ void Choose(const LayerArgs& a, const float* row, int
   }
 }
 
-__device__ __forceinline__ void BarrierSync(int id, int threads) {
-  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void BarrierArrive(int id, int threads) {
-  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 template <int kType, int kGroups>
 __global__ void __launch_bounds__(kThreads, 1)
 FirstKernel(const LayerArgs a) {

@@ -143,13 +143,6 @@ struct VectorArgs {
 // SMs idle and their barrier waits for the copies in flight.)
 constexpr int kMaxRows = 16;
 
-__device__ __forceinline__ void BarrierSync(int id, int threads) {
-  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void BarrierArrive(int id, int threads) {
-  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 template <int kTiles, int kType, int kGroups, bool kWide>
 __global__ void __launch_bounds__(Threads(kWide), kWide ? 1 : 2)
 VectorKernel(const VectorArgs a) {

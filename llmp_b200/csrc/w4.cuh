@@ -303,6 +303,14 @@ __device__ __forceinline__ void CopyAsyncWait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
+// Barriers of some of a CTA's warps: those that wait, and those that only arrive.
+__device__ __forceinline__ void BarrierSync(int id, int threads) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void BarrierArrive(int id, int threads) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // Eight 16-bit values as they are (zero from `valid` on) into shared memory: in the thread's open group of copies
 // where they may be copied 16 bytes at a time.
 __device__ __forceinline__ void Stage8(void* shared, const void* row, std::int64_t at, int valid, bool vec) {
@@ -327,31 +335,21 @@ template <int kGroups>
 struct StepWeights {
   uint4 a, b;                                // rows g and g + 8
   std::uint32_t word_a[kGroups], word_b[kGroups];
-  template <typename Load16, typename Load8, typename Load4>
-  __device__ __forceinline__ void From(const std::uint8_t* block, int lane, Load16 load16, Load8 load8, Load4 load4) {
-    a = load16(block + (lane * 16));
-    b = load16(block + 512 + (lane * 16));
+  __device__ __forceinline__ void LoadShared(const std::uint8_t* block, int lane) {
+    a = *reinterpret_cast<const uint4*>(block + (lane * 16));
+    b = *reinterpret_cast<const uint4*>(block + 512 + (lane * 16));
     const std::uint8_t* words = block + 1024 + ((lane >> 2) * (kGroups * 4));
     if constexpr (kGroups == 1) {
-      word_a[0] = load4(words);
-      word_b[0] = load4(words + 32);
+      word_a[0] = *reinterpret_cast<const std::uint32_t*>(words);
+      word_b[0] = *reinterpret_cast<const std::uint32_t*>(words + 32);
     } else if constexpr (kGroups == 2) {
-      const uint2 wa = load8(words), wb = load8(words + 64);
+      const uint2 wa = *reinterpret_cast<const uint2*>(words), wb = *reinterpret_cast<const uint2*>(words + 64);
       word_a[0] = wa.x, word_a[1] = wa.y, word_b[0] = wb.x, word_b[1] = wb.y;
     } else {
-      const uint4 wa = load16(words), wb = load16(words + 128);
+      const uint4 wa = *reinterpret_cast<const uint4*>(words), wb = *reinterpret_cast<const uint4*>(words + 128);
       word_a[0] = wa.x, word_a[1] = wa.y, word_a[2] = wa.z, word_a[3] = wa.w;
       word_b[0] = wb.x, word_b[1] = wb.y, word_b[2] = wb.z, word_b[3] = wb.w;
     }
-  }
-  __device__ __forceinline__ void LoadShared(const std::uint8_t* block, int lane) {
-    From(block, lane, [](const void* p) { return *static_cast<const uint4*>(p); },
-         [](const void* p) { return *static_cast<const uint2*>(p); },
-         [](const void* p) { return *static_cast<const std::uint32_t*>(p); });
-  }
-  __device__ __forceinline__ void Load(const std::uint8_t* block, int lane) {
-    From(block, lane, [](const void* p) { return LoadStream16(p); }, [](const void* p) { return LoadStream8(p); },
-         [](const void* p) { return LoadStream4(p); });
   }
 };
 
