@@ -255,3 +255,26 @@ def test_infinities_in_the_router_s_product(cuda, kind, router):
         if change == "x":
             assert ids[10].tolist() == list(range(16)) and bool(got[10].isnan().all())
             assert finite.sum() == 8
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("router", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("experts,used,hidden,inter,out", [(32, 4, 512, 128, None), (3, 2, 512, 96, None), (32, 4, 512, 128, "f32"),
+                                                          (2, 1, 8192, 64, None), (100, 6, 288, 160, "bf16")])
+def test_company_of_every_type_and_size(cuda, kind, router, experts, used, hidden, inter, out):
+    """A token's results are the same bits alone and among others: where tokens name the same experts and their groups are cut,
+    where not all of a call's tokens are staged at once, for every type of activations, router and output."""
+    torch = cuda
+    import llmp_b200 as ops
+    c = _case(torch, 19, 16, experts, hidden, inter, 32, 32, kind=kind, router=router)
+    gate_up, down = ops.w4_relayout(*c["gate_up"], glu=True), ops.w4_relayout(*c["down"])
+    out = ref.TYPES[out or kind]
+
+    def layer(x):
+        y = torch.empty(x.shape, dtype=out, device="cuda")
+        return ops.moe_layer(x, c["router"], gate_up, down, used, out=y)
+    y, ids, weights = layer(c["x"])
+    for chosen in ([0], [15], [3, 9], [1, 2, 4, 8, 13], list(range(15, -1, -1))):
+        some = layer(c["x"][chosen].contiguous())
+        assert torch.equal(some[1], ids[chosen]) and torch.equal(some[2], weights[chosen])
+        assert torch.equal(some[0], y[chosen])

@@ -204,3 +204,50 @@ def test_a_nan_survives_the_glu(cuda, glu, kind):
     want = torch.zeros((3, n), dtype=torch.bool, device="cuda")
     want[1], want[:, 5], want[:, 17] = True, True, True
     assert torch.equal(y.isnan(), want)
+
+
+@pytest.mark.parametrize("glu", ["none", "geglu"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_arrays_of_experts_with_strides(cuda, glu, group):
+    """Experts and rows further apart than they are long, arrays that begin at odd bytes, plain and GLU slabs: the slab is
+    that of the packed arrays."""
+    torch = cuda
+    import llmp_b200 as ops
+    g = torch.Generator().manual_seed(11)
+    experts, n, k = 5, 38, group * 3
+    packed = ref.w4_source(g, (experts,), n, k, group, "f16", True)
+
+    def apart(t, rows, before, behind):
+        wide = torch.randint(0, 200, (experts, n + rows, t.shape[-1] + before + behind), generator=g).to(t.dtype).cuda()
+        view = wide[:, rows // 2:rows // 2 + n, before:before + t.shape[-1]]
+        view.copy_(t)
+        return view
+    want = ops.w4_relayout(*packed, glu=glu != "none").slab
+    for rows, before, behind in ((0, 0, 0), (3, 1, 2), (2, 4, 4), (0, 3, 0)):
+        moved = [apart(t, rows, before, behind) for t in packed]
+        got = ops.w4_relayout(*moved, glu=glu != "none")
+        assert torch.equal(got.slab, want)
+    order = [2, 0, 4, 1, 3]                       # experts in an order of their own: one array, transposed places
+    turned = [t[order].transpose(0, 1).contiguous().transpose(0, 1) for t in packed]
+    got = ops.w4_relayout(*turned, glu=glu != "none").slab.view(experts, -1)
+    assert torch.equal(got, want.view(experts, -1)[order])
+    # what the slab's experts multiply to, one by one
+    x = torch.randn((3, k), generator=g).cuda()
+    for e in range(experts):
+        _check(torch, ops, [t[e] for t in moved], x, n // 2 if glu != "none" else n, group, glu)
+
+
+@pytest.mark.parametrize("glu", ["swiglu", "geglu"])
+def test_a_glu_slab_from_strided_rows(cuda, glu):
+    torch = cuda
+    import llmp_b200 as ops
+    n, k, group = 45, 320, 32
+    source, x = _case(torch, 12, 6, n, k, group, kind="f16", glu=True)
+    _, want = _check(torch, ops, source, x, n, group, glu)
+    for before, behind in ((1, 2), (4, 8), (3, 0)):
+        moved = []
+        for t in source:
+            wide = torch.zeros((2 * n, t.shape[1] + before + behind), dtype=t.dtype, device="cuda")
+            wide[:, before:before + t.shape[1]] = t
+            moved.append(wide[:, before:before + t.shape[1]])
+        assert torch.equal(ops.w4_vector(ops.w4_relayout(*moved, glu=True), x, glu=ref.GLUS[glu]), want)
