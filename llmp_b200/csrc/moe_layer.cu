@@ -76,8 +76,6 @@ struct LayerArgs {
   int router_rows;    // experts of a router tile: 16, or 8 where those would leave CTAs of the cluster without one
   int parts;          // warps that divide a tile's steps of hidden
   int round_tiles;    // tiles that a round's warps work on
-  int block_down;     // bytes of a step of the down slab
-  bool prefetch_down; // small enough for L2 while the first kernel works
 };
 
 // Column tiles that a group's tokens take in the products: one or two, in registers.
@@ -649,16 +647,6 @@ FirstKernel(const LayerArgs a) {
       for (int i = tid - (kWarps * 32); i <= s.choice.groups; i += kReducers * 32) a.choice->first[i] = s.choice.first[i];
       if (tid == kWarps * 32) a.choice->groups = s.choice.groups;
     }
-    if (a.prefetch_down) {  // the named experts' down rows, on their way while this kernel works
-      const int lines = a.tiles_down * a.steps_down * (a.block_down / 64) / 2;  // of 128 bytes, an expert's
-      const int first_line = (static_cast<int>(blockIdx.x) * kReducers * 32) + tid - (kWarps * 32);
-      for (int n = 0; n < s.choice.groups; ++n) {
-        const std::uint8_t* rows = a.down + (static_cast<std::size_t>(s.choice.expert[n]) * a.tiles_down * a.steps_down * a.block_down);
-        for (int i = first_line; i < lines; i += static_cast<int>(gridDim.x) * kReducers * 32) {
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(rows + (static_cast<std::size_t>(i) * 128)));
-        }
-      }
-    }
     // a warp every other tile of the round; a lane a row of every fourth token
     const int row = lane & 7;
     int group = first_group, pair = first_pair, buffer = 0;
@@ -1023,8 +1011,6 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   while (tile_warps < kWarps && a.steps_up >= 8 * tile_warps) tile_warps *= 2;
   a.round_tiles = kWarps / tile_warps;
   a.parts = std::min(tile_warps, a.steps_up);
-  a.block_down = BlockBytes(d.down.group);
-  a.prefetch_down = static_cast<double>(std::min(experts, d.tokens * d.used)) * a.tiles_down * a.steps_down * a.block_down <= 32e6;
   a.glu_pieces = GluPieces(d.x_type, d.y_type);
   a.cap = d.tokens;
   a.group_cap = std::min(d.tokens, GroupTokens(d.x_type));
