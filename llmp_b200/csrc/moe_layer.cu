@@ -29,8 +29,8 @@ using namespace w4;
 
 constexpr int kWarps = 16, kReducers = 2;          // of the first kernel: that multiply, that add up
 constexpr int kThreads = (kWarps + kReducers) * 32;
-constexpr int kFewSlots = 4, kManySlots = 6;       // steps a warp's ring of the first kernel holds, where they fit
-constexpr int kSecondSlots = 6;
+constexpr int kSlots = 4, kSecondSlots = 6;        // steps a warp's ring of the first and the second kernel holds (six in the
+                                                   // first: sixteen bf16 tokens 106 us, not 104)
 constexpr int kMaxCluster = 8;
 constexpr int kMaxTokens = 16, kMaxUsed = 16, kMaxExperts = 512;
 constexpr int kMaxPairs = kMaxTokens * kMaxUsed;
@@ -72,7 +72,6 @@ struct LayerArgs {
   int cap;            // tokens staged at a time
   int group_cap;      // tokens of a group
   int x_pitch;        // bytes of a staged piece of a token
-  int slots;          // of the first kernel's rings
   int router_rows;    // experts of a router tile: 16, or 8 where those would leave CTAs of the cluster without one
   int parts;          // warps that divide a tile's steps of hidden
   int round_tiles;    // tiles that a round's warps work on
@@ -120,8 +119,8 @@ struct FirstShared {
 // Dynamic shared memory of the first kernel: the rings (before the products: the router's partial sums), two buffers of partial sums, the staged tokens, logits.
 struct FirstLayout {
   int ring, meet, staged, logits, bytes;
-  __host__ __device__ FirstLayout(int block_bytes, int slots, int cap, int group_cap, int pieces, int x_pitch, int tokens, int experts) {
-    ring = kWarps * slots * block_bytes;
+  __host__ __device__ FirstLayout(int block_bytes, int cap, int group_cap, int pieces, int x_pitch, int tokens, int experts) {
+    ring = kWarps * kSlots * block_bytes;
     const int before = kWarps * kTileRows * kMaxTokens * 8;
     if (ring < before) ring = (before + 255) / 256 * 256;
     meet = ring;
@@ -399,7 +398,7 @@ FirstKernel(const LayerArgs a) {
   constexpr int kBlock = BlockBytes(kStep / kGroups);
   extern __shared__ __align__(128) std::uint8_t smem[];
   __shared__ FirstShared s;
-  const FirstLayout at(kBlock, a.slots, a.cap, a.group_cap, kPieces, a.x_pitch, a.tokens, a.experts);
+  const FirstLayout at(kBlock, a.cap, a.group_cap, kPieces, a.x_pitch, a.tokens, a.experts);
   std::uint8_t* staged = smem + at.staged;
   float* logits = reinterpret_cast<float*>(smem + at.logits);
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
@@ -544,8 +543,7 @@ FirstKernel(const LayerArgs a) {
   float* meet = reinterpret_cast<float*>(smem + at.meet);
   const int meet_floats = kWarps * kTileRows * a.group_cap;
   if (warp < kWarps) {
-    const int slots = a.slots;
-    std::uint8_t* ring = smem + (warp * slots * kBlock);
+    std::uint8_t* ring = smem + (warp * kSlots * kBlock);
     // where the next request reads
     int load_group = first_group, load_pair = first_pair;
     int load_rounds = steps > 0 ? end_round - first_round : 0, load_left = 0;
@@ -577,7 +575,8 @@ FirstKernel(const LayerArgs a) {
       }
       CopyAsyncCommit();
     };
-    for (int i = 0; i < slots - 1; ++i) request(i);
+#pragma unroll
+    for (int i = 0; i < kSlots - 1; ++i) request(i);
     const int piece = g % Cols(kPieces);
     int group = first_group, pair = first_pair;
     int slot = 0, buffer = 0, staged_group = -1, column_group = -1, tiles = 1;
@@ -605,15 +604,15 @@ FirstKernel(const LayerArgs a) {
       Sums total[kTiles];
       if ((pair * round_tiles) + my_tile < a.tiles_up) {
         for (int step = 0; step < steps; ++step) {
-          if (slots == kManySlots) CopyAsyncWait<kManySlots - 2>(); else CopyAsyncWait<kFewSlots - 2>();
+          CopyAsyncWait<kSlots - 2>();
           __syncwarp();  // all lanes' copies of this step are in, and the slot before it has been read
-          request(slot == 0 ? slots - 1 : slot - 1);
+          request(slot == 0 ? kSlots - 1 : slot - 1);
           StepWeights<kGroups> w;
-          w.LoadShared(smem + (((warp * slots) + slot) * kBlock), lane);
+          w.LoadShared(smem + (((warp * kSlots) + slot) * kBlock), lane);
           MultiplyStep<false, kGroups, kTiles>(w, tiles, total, [&](int nt, int i) {
             return *reinterpret_cast<const uint4*>(smem + column[nt] + (step * 256) + (i * 64));
           });
-          slot = slot == slots - 1 ? 0 : slot + 1;
+          slot = slot == kSlots - 1 ? 0 : slot + 1;
         }
       }
       // barriers 1, 2: buffer 0, 1 holds a round's sums; 3, 4: it may be written again
@@ -881,7 +880,7 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   if (const cudaError_t e = Configure(FirstKernel<kType, kGroups>, configured_device, kFirstSmemLimit); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.slots, a.cap, a.group_cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
+  const int smem = FirstLayout(BlockBytes(kStep / kGroups), a.cap, a.group_cap, BfloatPieces(kType), a.x_pitch, a.tokens, a.experts).bytes;
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
   const std::int64_t rounds = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) *
                               ((a.tiles_up + a.round_tiles - 1) / a.round_tiles);
@@ -1014,11 +1013,10 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.glu_pieces = GluPieces(d.x_type, d.y_type);
   a.cap = d.tokens;
   a.group_cap = std::min(d.tokens, GroupTokens(d.x_type));
-  auto bytes = [&](int slots) {
-    return FirstLayout(BlockBytes(d.gate_up.group), slots, a.cap, a.group_cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes;
+  auto bytes = [&]() {
+    return FirstLayout(BlockBytes(d.gate_up.group), a.cap, a.group_cap, BfloatPieces(d.x_type), a.x_pitch, d.tokens, experts).bytes;
   };
-  a.slots = bytes(kManySlots) <= kFirstSmemLimit ? kManySlots : kFewSlots;
-  while (a.cap > 1 && bytes(a.slots) > kFirstSmemLimit) {
+  while (a.cap > 1 && bytes() > kFirstSmemLimit) {
     --a.cap;
     a.group_cap = std::min(a.group_cap, a.cap);
   }
