@@ -31,7 +31,9 @@ constexpr int kWarps = 16, kReducers = 2;          // of the first kernel: that 
 constexpr int kThreads = (kWarps + kReducers) * 32;
 constexpr int kSlots = 4, kSecondSlots = 6;        // steps a warp's ring of the first and the second kernel holds (six in the
                                                    // first: sixteen bf16 tokens 106 us, not 104)
-constexpr int kMaxCluster = 8;
+// CTAs of a cluster of the first kernel.  (Of four, more SMs hold one, but each CTA works twice as much of the router out: five F32
+// tokens of 60 experts 38.7 us, not 31.1; sixteen bf16 tokens of 128 experts 104 and 104.)
+constexpr int kCluster = 8;
 constexpr int kMaxTokens = 16, kMaxUsed = 16, kMaxExperts = 512;
 constexpr int kMaxPairs = kMaxTokens * kMaxUsed;
 constexpr int kFirstSmemLimit = 211 * 1024;        // dynamic; the choice's lists are static (one token of 16384 F32
@@ -843,34 +845,29 @@ cudaError_t Configure(Kernel kernel, int& configured_device, int smem) {
   return e;
 }
 
-// Clusters of `size` CTAs of one first kernel that the device holds at once (a GPC holds whole clusters: more would be a
-// second wave).
+// Clusters of one first kernel that the device holds at once (a GPC holds whole clusters: more would be a second wave).
 template <auto kKernel>
-int ResidentClusters(int size, int smem) {
-  struct Known {
-    int device = -1, size = 0, smem = -1, clusters = 1;
-  };
-  static thread_local Known known[2];
-  Known& k = known[size == kMaxCluster ? 1 : 0];
+int ResidentClusters(int smem) {
+  static thread_local int known_device = -1, known_smem = -1, known = 1;
   int device = -1;
   cudaGetDevice(&device);
-  if (k.device == device && k.size == size && k.smem == smem) return k.clusters;
+  if (known_device == device && known_smem == smem) return known;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(SmCount() / size * size));
+  config.gridDim = dim3(static_cast<unsigned>(SmCount() / kCluster * kCluster));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = static_cast<std::size_t>(smem);
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attribute[0].val.clusterDim.x = kCluster;
   attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
   int clusters = 0;
   if (cudaOccupancyMaxActiveClusters(&clusters, kKernel, &config) != cudaSuccess || clusters < 1) {
     cudaGetLastError();
-    clusters = std::max(1, SmCount() / (2 * size));
+    clusters = std::max(1, SmCount() / (2 * kCluster));
   }
-  k.device = device, k.size = size, k.smem = smem, k.clusters = clusters;
+  known_device = device, known_smem = smem, known = clusters;
   return clusters;
 }
 
@@ -884,19 +881,16 @@ int LaunchFirst(const LayerArgs& a, cudaStream_t stream) {
   if (smem > kFirstSmemLimit) return Reject("moe_layer: %d bytes of shared memory", smem);
   const std::int64_t rounds = static_cast<std::int64_t>(std::min(a.experts, a.tokens * a.used)) *
                               ((a.tiles_up + a.round_tiles - 1) / a.round_tiles);
-  // Clusters of four fill more of the device's SMs (on B200 36 against 15 of eight), each working the whole router out:
-  // worth it where the products outlast that.
-  const int size = rounds > 8 * SmCount() ? kMaxCluster / 2 : kMaxCluster;
-  const std::int64_t most = ResidentClusters<FirstKernel<kType, kGroups>>(size, smem);
-  const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + size - 1) / size));
+  const std::int64_t most = ResidentClusters<FirstKernel<kType, kGroups>>(smem);
+  const std::int64_t clusters = std::max<std::int64_t>(1, std::min(most, (rounds + kCluster - 1) / kCluster));
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(clusters * size));
+  config.gridDim = dim3(static_cast<unsigned>(clusters * kCluster));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = static_cast<std::size_t>(smem);
   config.stream = stream;
   cudaLaunchAttribute attribute[2];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attribute[0].val.clusterDim.x = kCluster;
   attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
   attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute[1].val.programmaticStreamSerializationAllowed = 1;
@@ -995,7 +989,7 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.down = static_cast<const std::uint8_t*>(d.down.slab);
   a.experts = experts, a.used = d.used, a.tokens = d.tokens, a.hidden = hidden, a.inter = inter;
   a.tiles_up = Tiles(d.gate_up.n, 1), a.steps_up = Steps(hidden);
-  a.router_rows = experts <= 8 * kMaxCluster ? 8 : 16;
+  a.router_rows = experts <= 8 * kCluster ? 8 : 16;
   a.tiles_down = Tiles(d.down.n, 0), a.steps_down = Steps(inter);
   a.glu = d.glu, a.limit = d.limit;
   a.y = d.y, a.y_stride = d.y_stride, a.y_type = d.y_type;
