@@ -363,7 +363,9 @@ int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream
   }
   const int ctas = std::max(1, SmCount() * (smem <= kSmemOfTwo ? 2 : 1) / ranks);
   // The busiest CTA's rounds times a warp's steps in one, a round costing about 0.7 of a step besides: many parts balance
-  // the CTAs where tiles are few, few parts make long runs where they are many, two rounds a CTA and more.  In a cluster
+  // the CTAs where tiles are few, few parts make long runs where they are many, two rounds a CTA and more.  (4096 -> 32003,
+  // sixteen F16 rows: 28.1 us; with a round at nothing 31.4, at two steps 30.8.  2560 -> 2 x 10240, four F32 rows: 15.6,
+  // 16.3, 15.6.)  In a cluster
   // every round ends in a barrier of all its CTAs, worth a dozen steps: as few rounds as keep the clusters busy
   // (16 rows of 16384 F16 values -> 4096: 56 us by the other rule, 25 by this; of 8192 F32 values 44 and 37).
   const double round_cost = ranks > 1 ? 12.0 : 0.7;
@@ -374,7 +376,7 @@ int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream
     const int rounds = (a.tiles + (kWarps / parts) - 1) / (kWarps / parts);
     if (best != 0.0 && rounds < (ranks > 1 ? ctas : 2 * ctas)) break;
     const double cost = ((rounds + ctas - 1) / ctas) * (((steps + parts - 1) / parts) + round_cost);
-    if (best == 0.0 || cost < 0.97 * best) best = cost, a.parts = parts;
+    if (best == 0.0 || cost < best) best = cost, a.parts = parts;
   }
   a.rounds = (a.tiles + (kWarps / a.parts) - 1) / (kWarps / a.parts);
   a.meet_floats = kWarps * kTileRows * a.rows;
