@@ -34,10 +34,13 @@ __device__ __forceinline__ float BlockSum(float v, float* shared) {
   return v;
 }
 
-// A CTA a row.  A thread holds kUnits units of eight values in registers from the first load to the
+// A CTA a row.  A thread holds kUnits units of eight values from the first load to the
 // last store, every row operand's loads in flight together, so a row is read once and the kernel is bound by
 // memory where there are many rows (4096 rows of 4096 bf16 values with a gate a token: 32 to 34 us, 5.0 to 5.3 TB/s, 76 to
-// 81 % of the copy rate) and by two reductions and three trips to memory where there is one (2560 F32 values: 2.6 us).
+// 81 % of the copy rate; of F32 values 58 us, 5.8 TB/s, 88 %) and by two reductions and three trips to memory where there is
+// one (2560 F32 values: 2.6 us).  One unit, and two of 16-bit values, stay in registers.  Four do not: 1024 threads leave 64
+// registers each, 112 to 252 bytes a thread go to local memory (two units of F32 vectors: 16), and rows above 8192 values take
+// more of the copy rate's time: 1024 rows of 16384 bf16 values with a gate a token 47 us, 3.6 TB/s, 54 %, of F32 values 96.
 // A thread a value 1024 threads apart, unpacked as it comes, took 395 and 9.2 us.  kVec: 16-byte loads (whole rows of eight
 // values, aligned); otherwise unit u's value i is column (8 u + i) threads + tid, so that a warp's
 // loads are still neighbours.
@@ -263,11 +266,13 @@ int LaunchNorm(const llmp_b200_block_norm_desc& a, int threads, cudaStream_t str
 
 template <int kType, bool kVec>
 int LaunchUnits(const llmp_b200_block_norm_desc& a, cudaStream_t stream) {
-  // one unit a thread for short rows and while the rows are too few to hide a thread's loads behind each other's; two
-  // for many longer ones; four where 1024 threads need them
+  // One unit a thread up to 512 threads, two up to 1024, then four.  Many rows of single-element loads take two from 256
+  // threads on, or a row's CTA is too large for its work.  (Vectors, one unit and two: 600 rows of 4096 bf16 values 8.6 and
+  // 10.2 us, 4096 rows 33.6 and 33.5, of F32 values 58 and 65; one bf16 row of 2048 2.2 and 2.7.  Elements of bf16: 128 rows
+  // of 4095 values 6.3 and 7.7, 320 rows 10.6 and 8.1, 2048 rows 38.8 and 34.4.)
   const int units = (a.width + 7) / 8;
   auto threads = [&](int each) { return std::max(32, (((units + each - 1) / each) + 31) / 32 * 32); };
-  if (units <= 256 || (a.rows < 2 * SmCount() && units <= 512)) return LaunchNorm<kType, 1, kVec>(a, threads(1), stream);
+  if (units <= 256 || ((kVec || a.rows < 2 * SmCount()) && units <= 512)) return LaunchNorm<kType, 1, kVec>(a, threads(1), stream);
   if (units <= 1024) return LaunchNorm<kType, 2, kVec>(a, threads(2), stream);
   return LaunchNorm<kType, 4, kVec>(a, threads(4), stream);
 }
