@@ -699,7 +699,7 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream);
  * llmp_b200_moe_decode takes the choice of experts, this makes it:
  *   logits[t] = router x[t];  p = softmax(logits) over all experts, or sigmoid of each
  *   the `used` experts of the greatest logit (with a bias: of the greatest p + bias), best first,
- *     ties to the lowest index, a NaN below everything
+ *     ties to the lowest index, a NaN below everything; the logits, and p + bias, are F32 when they are compared
  *   weights = p of those (renormalize: over their sum) * scale
  *   y[t] = sum_j weights[j] * down_e glu(gate_e x[t], up_e x[t]),  e = ids[t][j], added in slot order
  * Logits are added in 64 bits, up to 128 values at a time in F32; expert sums are F32 over exact products,
@@ -765,7 +765,8 @@ int llmp_b200_block_norm(const llmp_b200_block_norm_desc* desc, void* stream);
  *   entropy[row] = -sum p log p
  *   top_ids / top_logprobs[row]: the `top` largest logits, best first, ties to the lowest index
  * A masked logit is -inf: its log probability is -inf, and so are all of a row that has nothing else (entropy 0).
- * A NaN or +inf makes a row's log probabilities and entropy NaN; in the order a NaN is below -inf.  A
+ * A NaN or +inf makes a row's log probabilities and entropy NaN.  Among the alternatives a NaN comes behind -inf; a rank
+ * counts what compares as larger, which nothing does than a NaN: a token whose logit is one has rank 1.  A
  * token outside the vocabulary has NaN and rank 0. */
 typedef struct llmp_b200_logprobs_desc {
   const void* logits;    /* [rows, vocab], rows stride elements apart */

@@ -8,10 +8,12 @@
 // eighth of the experts, and meets through its own hardware barrier: 0.5 MB of router weights from
 // L2 a cluster instead of a kernel of its own or a grid barrier, and no counter that two calls
 // could share.  Then every CTA knows the choice and takes its share of (expert, tile) units.
-// What bounds it, 128 experts, top 8, 2048 x 768: one bf16 token 23 us, of which the first kernel's way to the choice is 8
+// What bounds it, 128 experts, top 8, 2048 x 768: one bf16 token 22 us, of which the first kernel's way to the choice is 8
 // (staging, the router's rows through one SM's share of L2, two cluster barriers, the picks one after the other),
-// its products 5 and the second kernel 7; sixteen tokens 105 us for 211 MB, issue slots 50 and 70 % full, 250 and 330
-// instructions a warp and step of 1.1 KB: the steps' own, and a round's or item's shares of addresses and meetings.
+// its products 5 and the second kernel 7; sixteen tokens 102 us for 211 MB, issue slots 56 and 70 % full, 250 and 330
+// instructions a warp and step of 1.1 KB where the product's own are about 120: the rest is a round's or item's share of
+// addresses and meetings, as a warp's run is four steps and three.  The MMAs' columns that stand for no token read the
+// first one's values (sixteen bf16 tokens 106.5 us; zeros of their own 107.4, eight F16 tokens 77.8 and 79.8).
 // The second kernel's CTA owns 16 output rows and adds a token's experts up in slot order, so a
 // token's sums do not depend on the other tokens of the call.
 #include <cooperative_groups.h>
@@ -79,7 +81,8 @@ struct LayerArgs {
   int round_tiles;    // tiles that a round's warps work on
 };
 
-// Column tiles that a group's tokens take in the products: one or two, in registers.
+// Tokens of a group, and the column tiles that they take in the products, in registers: one or two (four in the second kernel
+// where 16-bit activations have an F32 output).
 __host__ __device__ constexpr int GroupTokens(int type) { return type == kF32 ? 4 : 8; }
 __host__ __device__ constexpr int GroupTiles(int tokens, int pieces) { return (tokens + TokensATile(pieces) - 1) / TokensATile(pieces); }
 // bf16 pieces that a GLU value travels in between the kernels.  Three hold all 24 bits of its F32 form: where activations or
@@ -430,7 +433,7 @@ FirstKernel(const LayerArgs a) {
   for (int e = tid; e < a.experts; e += kThreads) s.mask[e] = 0;
   GridDependencyWait();
 
-  // ---- the router's product: 16 experts at a time, CTA rank r the tiles r, r + 8, ...
+  // ---- the router's product: a tile of 8 or 16 experts at a time, CTA rank r the tiles r, r + 8, ...
   auto* partial = reinterpret_cast<double(*)[kTileRows][kMaxTokens]>(smem);
   bool met = false;
   for (int first = 0; first < a.tokens; first += a.cap) {

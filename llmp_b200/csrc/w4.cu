@@ -134,13 +134,16 @@ struct VectorArgs {
 // next round's other buffer of sums.  Where the activations of all of k do not fit, the CTAs of a
 // cluster divide k as well and read each other's sums.
 //
-// What bounds it: the instructions of a step (about 120 to 200 a warp for 1.1 to 1.3 KB: taking the codes apart on
-// the logic and half-precision pipes, the MMAs, a round's share of the meeting), and for small matrices a launch's trips
-// to memory.  Measured, weights from HBM: 4096 x 4096, one bf16 row 5.2 us; 4096 -> 14336 10.0 us (3.0 TB/s); 4096 -> 20480
-// 13.7 us (3.2 TB/s); gate | up 2560 -> 10240, four F32 rows 15.8 us, eight F16 rows 11.9 us; 4096 -> 32003 in groups of 32,
-// sixteen F16 rows 28.5 us (2.7 TB/s; issue slots 56 % full, tensor pipe 24 %).  (Clusters of eight dividing k in
-// every call, so that each CTA stages an eighth of the activations: 31 and 83 us for the last two, the clusters leave
-// SMs idle and their barrier waits for the copies in flight.)
+// What bounds it: the weights' way through the rings with the rounds' meetings, and on top of it the instructions of a step
+// (about 120 to 200 a warp for 1.1 to 1.3 KB: taking the codes apart on the logic and half-precision pipes, the MMAs) and the
+// staging, which all of a CTA's warps wait for.  Measured, weights from HBM, in brackets without the products, without the
+// staging, without both: 4096 x 4096, one bf16 row 5.1 us (3.4, 5.0, 3.2); 4096 -> 14336 11.0 us, 2.8 TB/s (7.4, 11.0, 7.1: 3.03
+// rounds a CTA, the busiest does four); 4096 -> 20480 14.0 us, 3.1 TB/s (9.4, 13.9, 9.1); gate | up 2560 -> 10240, eight F16
+// rows 11.1 us (8.5, 9.9, 7.3), four F32 rows 15.6 us (12.8, 9.7, 7.1: rows read twice behind two barriers);
+// 4096 -> 32003 in groups of 32, sixteen F16 rows 28.1 us, 2.7 TB/s (18.9, 26.4, 17: issue slots 56 % full, tensor pipe 24 %,
+// rings of three steps beside 131 KB of activations); 8192 -> 4096, sixteen F32 rows 36.4 us (29.5, 19.6, 12.8).  (Clusters of
+// eight dividing k in every call, so that each CTA stages an eighth of the activations: 31 and 83 us for the four F32 rows and
+// the sixteen F16 ones, the clusters leave SMs idle and their barrier waits for the copies in flight.)
 constexpr int kMaxRows = 16;
 
 template <int kTiles, int kType, int kGroups, bool kWide>
@@ -367,7 +370,7 @@ int LaunchVector(VectorArgs a, int ranks, std::int64_t smem, cudaStream_t stream
   // sixteen F16 rows: 28.1 us; with a round at nothing 31.4, at two steps 30.8.  2560 -> 2 x 10240, four F32 rows: 15.6,
   // 16.3, 15.6.)  In a cluster
   // every round ends in a barrier of all its CTAs, worth a dozen steps: as few rounds as keep the clusters busy
-  // (16 rows of 16384 F16 values -> 4096: 56 us by the other rule, 25 by this; of 8192 F32 values 44 and 37).
+  // (16 rows of 16384 F16 values -> 4096: 56 us by the other rule, 25 by this; of 8192 F32 values 44 and 36).
   const double round_cost = ranks > 1 ? 12.0 : 0.7;
   const int steps = a.steps / ranks;
   double best = 0.0;

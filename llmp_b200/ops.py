@@ -978,7 +978,7 @@ def w4_relayout(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor |
 def w4_vector(w: W4Matrix, x: torch.Tensor, *, glu: int = GLU_NONE, limit: float = 0.0,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """x F32, F16 or BF16 [rows <= 16, k] times 4-bit weights -> [rows, n] (glu: of gate and up
-    products), in x's type or `out`'s."""
+    products), in x's type or `out`'s.  `out` and x share no memory."""
     device = _current(x, "w4_vector x")
     kind, between = _rows(x, device, "w4_vector x")
     rows, k = x.shape
@@ -997,7 +997,8 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, gate_up: W4Matrix, down: W4
     of `used` experts a token, their products over 4-bit weights, weighted sum.  x [tokens, hidden],
     router [experts, hidden] in F32, F16 or BF16, bias F32 [experts]; gate_up of [experts, 2 inter, hidden]
     (w4_relayout glu=True), down of [experts, hidden, inter].  Returns (y [tokens, hidden] in x's type or
-    `out`'s, ids I32 [tokens, used], weights F32 [tokens, used])."""
+    `out`'s, ids I32 [tokens, used], weights F32 [tokens, used]).  `out` and x share no memory; an F32 `out` of
+    16-bit activations keeps the GLU rows whole as well."""
     device = _current(x, "moe_layer x")
     kind, between = _rows(x, device, "moe_layer x")
     router_kind, router_between = _rows(router, device, "moe_layer router")
@@ -1097,7 +1098,7 @@ def logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, top: i
              temperature: float = 1.0) -> Logprobs:
     """Log probabilities and ranks of given tokens (I32 [rows, given <= 16] or None), the entropy and the
     `top` <= 32 largest of logits F32, F16 or BF16 [rows, vocab] (llmp_b200_logprobs).  Masked logits are
-    -inf."""
+    -inf; masked by the type's lowest value they are right as well, but slow where fewer than `top` are left."""
     device = _current(logits, "logprobs logits")
     kind, between = _rows(logits, device, "logprobs logits")
     rows, vocab = logits.shape
