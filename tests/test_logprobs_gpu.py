@@ -150,3 +150,15 @@ def test_graph_and_stream(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b.flip(0)) for a, b in zip(held, want))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("temperature", [1e-6, 1e6])
+@pytest.mark.parametrize("rows", [2, 600])
+def test_the_first_and_the_last_temperature(cuda, kind, temperature, rows):
+    import llmp_b200 as ops
+    logits, g = _logits(cuda, 7, rows, 3000, kind)
+    tokens = cuda.randint(0, 3000, (rows, 2), generator=g, dtype=cuda.int32).cuda()
+    tokens[:, 1] = tokens[:, 0]                       # the same token twice
+    got = _check(cuda, ops, logits, tokens, 3, temperature)
+    assert cuda.equal(got.logprobs[:, 0], got.logprobs[:, 1]) and cuda.equal(got.ranks[:, 0], got.ranks[:, 1])

@@ -278,3 +278,20 @@ def test_company_of_every_type_and_size(cuda, kind, router, experts, used, hidde
         some = layer(c["x"][chosen].contiguous())
         assert torch.equal(some[1], ids[chosen]) and torch.equal(some[2], weights[chosen])
         assert torch.equal(some[0], y[chosen])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("experts", [16, 40, 512])
+def test_the_most_pairs(cuda, kind, experts):
+    """Sixteen experts for each of sixteen tokens: all of the lists' 256 places, named by all tokens or by one."""
+    import llmp_b200 as ops
+    c = _case(cuda, 20, 16, experts, 128, 64, 64, 32, kind=kind)
+    _check(cuda, ops, c, 16)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+@pytest.mark.parametrize("hidden,inter", [(64, 65536), (32, 20000)])
+def test_long_inter(cuda, kind, hidden, inter):
+    import llmp_b200 as ops
+    c = _case(cuda, 21, 3, 2, hidden, inter, 32, 32, kind=kind)
+    _check(cuda, ops, c, 1)
