@@ -703,10 +703,9 @@ int llmp_b200_w4_vector(const llmp_b200_w4_product* product, void* stream);
  *   weights = p of those (renormalize: over their sum) * scale
  *   y[t] = sum_j weights[j] * down_e glu(gate_e x[t], up_e x[t]),  e = ids[t][j], added in slot order
  * Logits are added in 64 bits, up to 128 values at a time in F32; expert sums are F32 over exact products,
- * the GLU rows are within 2^-17 of their F32 values, which a 16-bit y rounds away, and those values themselves where x or y
- * is F32.  A token's results do not depend on the
- * others of the call; a NaN stays one, in the GLU's clamps too.  Each call that may overlap another brings its
- * own scratch; nothing in it outlives the call. */
+ * the GLU rows are within 2^-17 of their F32 values, which a 16-bit y rounds away, and those values themselves where x
+ * or y is F32.  A token's results do not depend on the others of the call; a NaN stays one, in the GLU's clamps too.
+ * Each call that may overlap another brings its own scratch; nothing in it outlives the call. */
 #define LLMP_B200_SCORE_SOFTMAX 0
 #define LLMP_B200_SCORE_SIGMOID 1
 typedef struct llmp_b200_moe_layer_desc {

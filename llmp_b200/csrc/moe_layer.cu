@@ -76,7 +76,7 @@ struct LayerArgs {
   int cap;            // tokens staged at a time
   int group_cap;      // tokens of a group
   int x_pitch;        // bytes of a staged piece of a token
-  int router_rows;    // experts of a router tile: 16, or 8 where those would leave CTAs of the cluster without one
+  int router_rows;    // experts of a router tile: 16, or 8 of an F32 router where 16 would leave CTAs of the cluster without one
   int parts;          // warps that divide a tile's steps of hidden
   int round_tiles;    // tiles that a round's warps work on
 };
@@ -909,7 +909,8 @@ int LaunchSecond(const LayerArgs& a, cudaStream_t stream) {
   if (const cudaError_t e = Configure(SecondKernel<kTokens, kGlu, kGroups>, configured_device, 160 * 1024); e != cudaSuccess) {
     return Failed(e, "moe_layer attribute");
   }
-  // sixteen warps a tile while there are no more tiles than SMs, else eight, two CTAs an SM
+  // Sixteen warps a tile while there are no more tiles than SMs, else eight, two CTAs an SM.  (Sixteen and eight, bf16: 128 tiles,
+  // one token 21.3 and 23.1 us, sixteen 102 and 132; 256 tiles, one 26.7 and 22.4, sixteen 72 and 68.)
   const int warps = a.tiles_down <= SmCount() ? kSecondWarps : kSecondWarps / 2;
   const int smem = (warps * kSecondSlots * BlockBytes(kStep / kGroups)) + (a.tokens * a.used * kParts * kTileRows * 4);
   const cudaError_t e = LaunchPdl(SecondKernel<kTokens, kGlu, kGroups>, dim3(static_cast<unsigned>(a.tiles_down)),
@@ -992,7 +993,9 @@ int llmp_b200_moe_layer(const llmp_b200_moe_layer_desc* desc, void* stream) {
   a.down = static_cast<const std::uint8_t*>(d.down.slab);
   a.experts = experts, a.used = d.used, a.tokens = d.tokens, a.hidden = hidden, a.inter = inter;
   a.tiles_up = Tiles(d.gate_up.n, 1), a.steps_up = Steps(hidden);
-  a.router_rows = experts <= 8 * kCluster ? 8 : 16;
+  // (Tiles of 8 and 16: 60 experts in F32, five tokens 30.4 and 30.9 us; in bf16, one token, 32 experts of 2560 values 23.5 and 22.9, 64 of 1024
+  // 14.8 and 14.4: an MMA has 16 rows either way.)
+  a.router_rows = d.router_type == kF32 && experts <= 8 * kCluster ? 8 : 16;
   a.tiles_down = Tiles(d.down.n, 0), a.steps_down = Steps(inter);
   a.glu = d.glu, a.limit = d.limit;
   a.y = d.y, a.y_stride = d.y_stride, a.y_type = d.y_type;
